@@ -166,7 +166,8 @@ int smallm_gemv_residual_sum(smallm_ctx* ctx, const smallm_qmatrix* W, const flo
 /* The device error word that the bounded waits of the GEMV and attention
  * kernels raise when they give up (0 = none): bit 0 a GEMV producer's stage
  * wait, bits 1-2 a GEMV or attention pipeline wait, bit 3 a residual part's
- * arrival flag, bit 5 the decode position changed during a step.  Waits for
+ * arrival flag, bit 5 the decode position changed during a step, bit 6 a wait
+ * of the tensor-core GEMM, bit 7 a bad row list (smallm_cache_move).  Waits for
  * the device; clear != 0 resets the word. */
 int smallm_ctx_device_errors(smallm_ctx* ctx, uint32_t* flags, int clear);
 
@@ -212,6 +213,95 @@ int smallm_attention_noalloc(smallm_ctx* ctx, const float* q_dev, const float* k
                              const float* vcache_dev, uint32_t n_heads, uint32_t n_kv_heads,
                              uint32_t head_dim, uint32_t max_ctx, uint32_t pos, float* out_dev,
                              void* stream);
+
+/* ---- drafted tokens over a bounded cache (no counterpart in the reference,
+ * which decodes one token at a time and only truncates its cache) ----
+ *
+ * Device pointers, asynchronous on `stream` (NULL = the context stream), no
+ * allocation and no host synchronisation; the calls can be captured into a
+ * graph, which replays them with the sizes they were captured with.  All of
+ * them keep results independent of timing: the same call on the same data
+ * gives the same bits. */
+
+/* Attention of n_tokens drafted tokens, the verification step of speculative
+ * decoding and, with one token, ordinary decoding.  The tokens' K and V rows
+ * are already in the cache at rows n_past .. n_past + n_tokens - 1 (their RoPE
+ * positions are the caller's business: siblings of a tree share one).
+ *
+ *   out[t][h] = softmax over the seen rows k of (q[t][h] . K[g][k] / sqrt(head_dim)) . V[g],
+ *               g = h / (n_heads / n_kv_heads)
+ *
+ * Token t sees every row below n_past, and drafted row n_past + u where bit
+ * u % 32 of mask_dev[t * words + u / 32] is set (words = ceil(n_tokens / 32);
+ * a token sees itself only if its own bit is set; bits at n_tokens and above
+ * are ignored).  mask_dev NULL is a chain: u <= t.  A token that sees nothing
+ * gets zeros.  Rows that a token does not see do not affect it, NaN and
+ * infinities included; where a seen row or q holds them, or a score passes
+ * f32's range, the output is not finite.
+ *
+ * q_dev [n_tokens][q_stride] and out_dev [n_tokens][out_stride] hold
+ * n_heads * head_dim f32 per row (strides in floats, multiples of 4, so q may
+ * be a slice of fused QKV rows); kcache_dev and vcache_dev are
+ * [n_kv_heads][max_ctx][head_dim].  These four are 16-byte aligned.
+ *
+ * weights_dev, unless NULL, is [n_kv_heads][max_ctx]: row k of KV head g gains
+ * the weight that it got in this call, summed over the tokens and the query
+ * heads of g (smallm_cache_select reads these totals); rows at
+ * n_past + n_tokens and above are left as they are.
+ *
+ * work_dev: at least smallm_attention_tree_workspace bytes, 16-byte aligned,
+ * contents irrelevant before and after.  Calls that may overlap in time need
+ * a workspace each.
+ *
+ * Limits: head_dim 32, 64 or 128; n_heads a multiple of n_kv_heads, at most
+ * 64 to 1; n_kv_heads <= 1024; n_tokens <= 1024; n_past + n_tokens <= max_ctx
+ * and <= 2^30.  n_tokens 0 does nothing. */
+int smallm_attention_tree(smallm_ctx* ctx, const float* q_dev, uint32_t q_stride, const float* kcache_dev,
+                          const float* vcache_dev, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                          uint32_t max_ctx, uint32_t n_past, uint32_t n_tokens, const uint32_t* mask_dev,
+                          float* out_dev, uint32_t out_stride, float* weights_dev, void* work_dev,
+                          uint64_t work_bytes, void* stream);
+/* Bytes of workspace of one call (with_weights: weights_dev is not NULL). */
+int smallm_attention_tree_workspace(smallm_ctx* ctx, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                    uint32_t n_past, uint32_t n_tokens, int with_weights, uint64_t* bytes);
+
+/* Which rows of a cache to keep: for each KV head the n_first first and
+ * n_last last of rows 0..n-1 and, of the rows between, the
+ * n_keep - n_first - n_last with the largest totals (equal totals: the lower
+ * row; NaN counts as less than everything).  rows_dev [n_kv_heads][n_keep]
+ * receives them in ascending order.  weights_dev is [n_kv_heads][max_ctx].
+ * n_first + n_last <= n_keep <= n <= max_ctx. */
+int smallm_cache_select(smallm_ctx* ctx, const float* weights_dev, uint32_t n_kv_heads, uint32_t max_ctx, uint32_t n,
+                        uint32_t n_keep, uint32_t n_first, uint32_t n_last, uint32_t* rows_dev, void* stream);
+
+/* Move listed cache rows together, in place: row dst + i of every KV head's K
+ * and V becomes row rows[i], i < n_rows; other rows are left as they are.
+ * rows_dev is [n_rows], one list for all heads (an accepted path of a drafted
+ * tree), or with per_head != 0 [n_kv_heads][n_rows] (what smallm_cache_select
+ * kept).  A list is strictly ascending with rows[i] >= dst + i.  weights_dev,
+ * unless NULL, is [n_kv_heads][max_ctx] and moves along.  Keys keep the
+ * rotary position they were stored with.
+ * An entry that breaks the rules, or names a row at max_ctx or above, raises
+ * bit 7 of the device error word; nothing outside the caches is touched, but
+ * the rows from dst on then hold unspecified rows of the cache. */
+int smallm_cache_move(smallm_ctx* ctx, float* kcache_dev, float* vcache_dev, float* weights_dev, uint32_t n_kv_heads,
+                      uint32_t head_dim, uint32_t max_ctx, const uint32_t* rows_dev, int per_head, uint32_t n_rows,
+                      uint32_t dst, void* stream);
+
+/* Log probabilities under softmax(logits), natural logarithm, one row of
+ * logits_dev [n_rows][stride] (stride in floats, >= vocab) at a time:
+ *   logprob_dev[r]  log probability of token tokens_dev[r] (both NULL: not
+ *                   wanted; a token at vocab or above gives NaN)
+ *   entropy_dev[r]  the distribution's entropy (NULL: not wanted)
+ *   top_ids_dev, top_logprobs_dev [n_rows][n_top]: the most likely tokens,
+ *                   largest first, equal logits in order of their ids
+ *                   (n_top <= 64 and <= vocab; 0: both may be NULL)
+ * A logit of -inf has probability 0.  A row that holds NaN or +inf, or nothing
+ * above -inf, has no distribution: its log probabilities and entropy are NaN,
+ * and its alternatives are still ordered (NaN logits last). */
+int smallm_logprobs(smallm_ctx* ctx, const float* logits_dev, uint32_t n_rows, uint32_t vocab, uint32_t stride,
+                    const uint32_t* tokens_dev, float* logprob_dev, float* entropy_dev, uint32_t n_top,
+                    uint32_t* top_ids_dev, float* top_logprobs_dev, void* stream);
 
 /* Samplers (src/runtime/sampler/*.cpp): one token from `n` HOST logits.
  * kind 0 = GreedySampler (first maximum), 1 = TemperatureSampler(temperature),

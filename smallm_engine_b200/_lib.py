@@ -73,6 +73,12 @@ SIGNATURES = {
     "smallm_qmatrix_dequantize": (_I, [_P, _P, _P, _P]),
     "smallm_dequantize": (_I, [_P, _U32, _P, ctypes.c_uint64, _P]),
     "smallm_attention_noalloc": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _U32, _P, _P]),
+    "smallm_attention_tree": (_I, [_P, _P, _U32, _P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _P, _P, _U32, _P, _P,
+                                   ctypes.c_uint64, _P]),
+    "smallm_attention_tree_workspace": (_I, [_P, _U32, _U32, _U32, _U32, _U32, _I, ctypes.POINTER(ctypes.c_uint64)]),
+    "smallm_cache_select": (_I, [_P, _P, _U32, _U32, _U32, _U32, _U32, _U32, _P, _P]),
+    "smallm_cache_move": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _P, _I, _U32, _U32, _P]),
+    "smallm_logprobs": (_I, [_P, _P, _U32, _U32, _U32, _P, _P, _P, _U32, _P, _P, _P]),
     "smallm_sample": (_I, [_P, _P, _U32, _U32, _U32, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                            ctypes.POINTER(_U32)]),
     "smallm_model_sample": (_I, [_P, _U32, _U32, ctypes.c_float, ctypes.c_float, ctypes.c_float,

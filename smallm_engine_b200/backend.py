@@ -107,6 +107,59 @@ class CUDABackend:
         check(lib().smallm_dequantize(self.h, type_, raw.ctypes.data, count, out.ctypes.data))
         return out
 
+    # ---- drafted tokens over a bounded cache ----
+    # Pointers are device addresses (int); stream None is the context's own.
+    # Sizes must fit the C types: they are checked by the library.
+    def attention_tree_workspace(self, n_heads: int, n_kv_heads: int, head_dim: int, n_past: int, n_tokens: int,
+                                 weights: bool = False) -> int:
+        """Bytes of workspace one attention_tree call needs."""
+        n = ctypes.c_uint64()
+        check(lib().smallm_attention_tree_workspace(self.h, n_heads, n_kv_heads, head_dim, n_past, n_tokens,
+                                                    int(weights), ctypes.byref(n)))
+        return n.value
+
+    def attention_tree(self, q: int, kcache: int, vcache: int, out: int, n_heads: int, n_kv_heads: int,
+                       head_dim: int, max_ctx: int, n_past: int, n_tokens: int, work: int, work_bytes: int,
+                       mask: int | None = None, weights: int | None = None, q_stride: int = 0, out_stride: int = 0,
+                       stream: int | None = None):
+        """smallm_attention_tree: n_tokens drafted tokens (rows n_past.. of the
+        cache) against the n_past cached rows and each other as the mask bits
+        say (None: a chain); weights: running totals per cache row.  A stride
+        of 0 is n_heads * head_dim."""
+        row = n_heads * head_dim
+        check(lib().smallm_attention_tree(self.h, q, q_stride or row, kcache, vcache, n_heads, n_kv_heads, head_dim,
+                                          max_ctx, n_past, n_tokens, mask, out, out_stride or row, weights, work,
+                                          work_bytes, stream))
+
+    def cache_select(self, weights: int, n_kv_heads: int, max_ctx: int, n: int, n_keep: int, n_first: int,
+                     n_last: int, rows: int, stream: int | None = None):
+        """smallm_cache_select: the rows of each KV head worth keeping, ascending,
+        into rows [n_kv_heads][n_keep]."""
+        check(lib().smallm_cache_select(self.h, weights, n_kv_heads, max_ctx, n, n_keep, n_first, n_last, rows,
+                                        stream))
+
+    def cache_move(self, kcache: int, vcache: int, n_kv_heads: int, head_dim: int, max_ctx: int, rows: int,
+                   n_rows: int, dst: int, per_head: bool = False, weights: int | None = None,
+                   stream: int | None = None):
+        """smallm_cache_move: row dst + i of K, V (and the totals) becomes row
+        rows[i], in place."""
+        check(lib().smallm_cache_move(self.h, kcache, vcache, weights, n_kv_heads, head_dim, max_ctx, rows,
+                                      int(per_head), n_rows, dst, stream))
+
+    def logprobs(self, logits: int, n_rows: int, vocab: int, tokens: int | None, logprob: int | None,
+                 entropy: int | None, n_top: int, top_ids: int | None, top_logprobs: int | None, stride: int = 0,
+                 stream: int | None = None):
+        """smallm_logprobs: log probability of tokens[r], entropy and the n_top
+        most likely tokens of each row of logits.  A stride of 0 is vocab."""
+        check(lib().smallm_logprobs(self.h, logits, n_rows, vocab, stride or vocab, tokens, logprob, entropy, n_top,
+                                    top_ids, top_logprobs, stream))
+
+    def device_errors(self, clear: bool = True) -> int:
+        """smallm_ctx_device_errors: the device error word (0 = none)."""
+        f = ctypes.c_uint32()
+        check(lib().smallm_ctx_device_errors(self.h, ctypes.byref(f), int(clear)))
+        return f.value
+
     def upload(self, W, type_: int, rows: int, cols: int) -> "QMatrix":
         return QMatrix(self, W, type_, rows, cols)
 

@@ -370,6 +370,86 @@ int smallm_attention_noalloc(smallm_ctx* ctx, const float* q_dev, const float* k
     });
 }
 
+int smallm_attention_tree(smallm_ctx* ctx, const float* q_dev, uint32_t q_stride, const float* kcache_dev,
+                          const float* vcache_dev, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                          uint32_t max_ctx, uint32_t n_past, uint32_t n_tokens, const uint32_t* mask_dev,
+                          float* out_dev, uint32_t out_stride, float* weights_dev, void* work_dev,
+                          uint64_t work_bytes, void* stream) {
+    return guard([&] {
+        need(ctx && ((q_dev && kcache_dev && vcache_dev && out_dev) || !n_tokens), "NULL argument");
+        set_dev(ctx->device);
+        smallm::TreeArgs a{};
+        a.q = q_dev;
+        a.kcache = kcache_dev;
+        a.vcache = vcache_dev;
+        a.mask = mask_dev;
+        a.weights = weights_dev;
+        a.out = out_dev;
+        a.q_stride = q_stride;
+        a.out_stride = out_stride;
+        a.n_heads = n_heads;
+        a.n_kv = n_kv_heads;
+        a.hd = head_dim;
+        a.max_ctx = max_ctx;
+        a.n_past = n_past;
+        a.n_tokens = n_tokens;
+        smallm::launch_attention_tree(a, work_dev, work_bytes, stream ? (cudaStream_t)stream : ctx->stream);
+    });
+}
+
+int smallm_attention_tree_workspace(smallm_ctx* ctx, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                    uint32_t n_past, uint32_t n_tokens, int with_weights, uint64_t* bytes) {
+    return guard([&] {
+        need(ctx && bytes, "NULL argument");
+        set_dev(ctx->device);
+        *bytes = smallm::tree_workspace_bytes(n_heads, n_kv_heads, head_dim, n_past, n_tokens, with_weights != 0);
+    });
+}
+
+int smallm_cache_select(smallm_ctx* ctx, const float* weights_dev, uint32_t n_kv_heads, uint32_t max_ctx, uint32_t n,
+                        uint32_t n_keep, uint32_t n_first, uint32_t n_last, uint32_t* rows_dev, void* stream) {
+    return guard([&] {
+        need(ctx && ((weights_dev && rows_dev) || !n_kv_heads || !n_keep), "NULL argument");
+        set_dev(ctx->device);
+        smallm::launch_cache_select(weights_dev, n_kv_heads, max_ctx, n, n_keep, n_first, n_last, rows_dev,
+                                    stream ? (cudaStream_t)stream : ctx->stream);
+    });
+}
+
+int smallm_cache_move(smallm_ctx* ctx, float* kcache_dev, float* vcache_dev, float* weights_dev, uint32_t n_kv_heads,
+                      uint32_t head_dim, uint32_t max_ctx, const uint32_t* rows_dev, int per_head, uint32_t n_rows,
+                      uint32_t dst, void* stream) {
+    return guard([&] {
+        need(ctx && ((kcache_dev && vcache_dev && rows_dev) || !n_kv_heads || !n_rows), "NULL argument");
+        set_dev(ctx->device);
+        smallm::launch_cache_move(kcache_dev, vcache_dev, weights_dev, n_kv_heads, head_dim, max_ctx, rows_dev,
+                                  per_head != 0, n_rows, dst, stream ? (cudaStream_t)stream : ctx->stream);
+    });
+}
+
+int smallm_logprobs(smallm_ctx* ctx, const float* logits_dev, uint32_t n_rows, uint32_t vocab, uint32_t stride,
+                    const uint32_t* tokens_dev, float* logprob_dev, float* entropy_dev, uint32_t n_top,
+                    uint32_t* top_ids_dev, float* top_logprobs_dev, void* stream) {
+    return guard([&] {
+        need(ctx && (logits_dev || !n_rows), "NULL argument");
+        need(!tokens_dev == !logprob_dev, "tokens and logprob go together");
+        need(!n_top || (top_ids_dev && top_logprobs_dev) || !n_rows, "NULL argument");
+        set_dev(ctx->device);
+        smallm::LogprobArgs a{};
+        a.logits = logits_dev;
+        a.n_rows = n_rows;
+        a.vocab = vocab;
+        a.stride = stride;
+        a.tokens = tokens_dev;
+        a.logprob = logprob_dev;
+        a.entropy = entropy_dev;
+        a.n_top = n_top;
+        a.top_ids = top_ids_dev;
+        a.top_logprobs = top_logprobs_dev;
+        smallm::launch_logprobs(a, stream ? (cudaStream_t)stream : ctx->stream);
+    });
+}
+
 static void check_sampler(uint32_t kind, uint32_t k, float temperature) {
     need(kind <= SMALLM_SAMPLE_TOP_P, "unknown sampler kind");
     need(kind != SMALLM_SAMPLE_TOP_K || k >= 1, "top-k needs k >= 1");

@@ -246,6 +246,44 @@ void launch_f32_to_f16(const float* src, __half* dst, uint64_t n, cudaStream_t s
 void launch_sample(const float* logits, uint32_t n, uint32_t kind, uint32_t k, float p, float temp, float r,
                    uint32_t* scratch, uint32_t* out, cudaStream_t stream);
 
+// Attention of n_tokens drafted tokens over n_past cached rows and their own
+// rows n_past .. n_past + n_tokens - 1 (tree_attention.cu).
+struct TreeArgs {
+    const float* q;          // [n_tokens][q_stride], n_heads * hd values per row (after RoPE)
+    const float* kcache;     // [n_kv][max_ctx][hd]
+    const float* vcache;
+    const uint32_t* mask;    // [n_tokens][ceil(n_tokens / 32)] words, null: a chain
+    float* weights;          // [n_kv][max_ctx] running totals, null: not kept
+    float* out;              // [n_tokens][out_stride]
+    uint32_t q_stride, out_stride, n_heads, n_kv, hd, max_ctx, n_past, n_tokens;
+};
+constexpr uint32_t kTreeMaxTokens = 1024, kTreeMaxGroup = 64, kTreeMaxKv = 1024, kTreeMaxKeys = 1u << 30;
+size_t tree_workspace_bytes(uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t n_past, uint32_t n_tokens,
+                            bool weights);
+void launch_attention_tree(const TreeArgs& a, void* work, size_t work_bytes, cudaStream_t stream);
+
+// Rows worth keeping and the move that closes the gaps (cache.cu).
+void launch_cache_select(const float* weights, uint32_t n_kv, uint32_t max_ctx, uint32_t n, uint32_t n_keep,
+                         uint32_t n_first, uint32_t n_last, uint32_t* rows, cudaStream_t stream);
+// rows: [n_rows] for every head, or [n_kv][n_rows] (per_head).  An entry that
+// breaks the list's rules raises bit 7 of the device error word and is skipped.
+void launch_cache_move(float* kcache, float* vcache, float* weights, uint32_t n_kv, uint32_t hd, uint32_t max_ctx,
+                       const uint32_t* rows, bool per_head, uint32_t n_rows, uint32_t dst, cudaStream_t stream);
+
+// Log probabilities, entropy and top alternatives of rows of logits (logprobs.cu).
+struct LogprobArgs {
+    const float* logits;     // [n_rows][stride]
+    uint32_t n_rows, vocab, stride;
+    const uint32_t* tokens;  // [n_rows], null: no given tokens
+    float* logprob;          // [n_rows]
+    float* entropy;          // [n_rows], may be null
+    uint32_t n_top;
+    uint32_t* top_ids;       // [n_rows][n_top]
+    float* top_logprobs;
+};
+constexpr uint32_t kLogprobMaxTop = 64;
+void launch_logprobs(const LogprobArgs& a, cudaStream_t stream);
+
 // Op-level kernels (Backend semantics on device pointers).
 void launch_rmsnorm(const float* x, const float* w, uint32_t n, float eps, float* y, cudaStream_t s);
 void launch_softmax(float* x, uint32_t n, cudaStream_t s);
