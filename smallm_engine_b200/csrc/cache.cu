@@ -3,16 +3,27 @@
 //
 // select: of rows 0..n-1 of a KV head keep the first n_first, the last n_last
 // and, of those between, the n_keep - n_first - n_last with the largest totals
-// (equal totals: the lower row; NaN below everything).  The k-th largest key
-// is found digit by digit (8 bits, most significant first, a histogram of the
-// keys that match the digits so far); every larger key is kept, and of the
-// equal ones the first few in row order.  Rows come out ascending.
+// (equal totals: the lower row; NaN below everything).  A cluster of up to 16
+// CTAs owns a head, each a contiguous range of its keys in shared memory.  The
+// k-th largest key is found digit by digit (11, 11 and 10 bits, most
+// significant first): histograms of the keys that match the digits so far,
+// summed over the cluster's shared memory, then the bin that holds the rank.
+// 11 bits take in two of the mantissa, so that totals within a few powers of
+// two do not all count into the same bins.  Every larger key is kept, and of
+// the equal ones the first few in row order; rows come out ascending.  Bound by
+// latency: one read of the totals and four cluster barriers.
 //
 // move: row dst + i of K and V (and the totals) becomes row rows[i], for a
-// strictly ascending list with rows[i] >= dst + i.  In place: a CTA owns a
-// slice of columns of one head and walks the list in chunks, all of a chunk's
-// loads before any of its stores.  A later chunk's source rows[j], j >= i, is
-// at least dst + j, so no store of an earlier chunk can have overwritten it.
+// strictly ascending list with rows[i] >= dst + i.  In place: a cluster owns a
+// slice of columns of one head and walks the list in waves, all of a wave's
+// loads (in registers) before any of its stores, by a cluster barrier.  A later
+// wave's source rows[j], j >= i, is at least dst + j, so no store of an
+// earlier wave can have overwritten it, and its loads are in flight before
+// the wave's barrier.  Bound by the bytes moved.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "common.cuh"
 #include "engine.h"
 #include "smallm_cuda.h"
@@ -20,130 +31,235 @@
 namespace smallm {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kSelThreads = 1024;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr uint32_t kSelBins = 2048;
+constexpr uint32_t kSelCached = 40960;  // keys of a CTA that fit shared memory
+constexpr uint32_t kSelMaxCluster = 16;
 
 // Order-preserving key, NaN lowest, -0 equal to +0.
 __device__ __forceinline__ uint32_t total_key(float x) { return x == x ? float_order_key(x + 0.f) : 0u; }
 
-__global__ void __launch_bounds__(kSelThreads)
+struct SelShared {
+    uint32_t hist[3][kSelBins];
+    uint32_t warp[kSelWarps];
+    uint32_t warp_eq[kSelWarps];
+    uint32_t digit, rank, above;
+    uint32_t gt, eq;  // this CTA's keys above / equal to the k-th largest
+};
+
+__global__ void __launch_bounds__(kSelThreads, 1)
     smallm_cache_select_kernel(const float* __restrict__ weights, uint32_t stride, uint32_t n, uint32_t n_keep,
-                               uint32_t n_first, uint32_t n_last, uint32_t* __restrict__ rows) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t sh_digit, sh_rank;
-    __shared__ uint32_t wsum[2][32];
+                               uint32_t n_first, uint32_t n_last, uint32_t per_cta, uint32_t cached,
+                               uint32_t* __restrict__ rows) {
+    extern __shared__ uint32_t cache[];
+    __shared__ SelShared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t C = cluster.num_blocks(), cr = cluster.block_rank(), head = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const float* w = weights + (size_t)blockIdx.x * stride + n_first;
-    uint32_t* out = rows + (size_t)blockIdx.x * n_keep;
     const uint32_t m = n - n_first - n_last, k = n_keep - n_first - n_last;
-    for (uint32_t i = tid; i < n_first; i += kSelThreads) out[i] = i;
-    for (uint32_t i = tid; i < n_last; i += kSelThreads) out[n_first + k + i] = n - n_last + i;
+    const uint32_t b0 = min(m, cr * per_cta), len = min(m, b0 + per_cta) - b0;
+    const float* w = weights + (size_t)head * stride + n_first + b0;
+    uint32_t* out = rows + (size_t)head * n_keep;
+    if (cr == 0) {
+        for (uint32_t i = tid; i < n_first; i += kSelThreads) out[i] = i;
+        for (uint32_t i = tid; i < n_last; i += kSelThreads) out[n_first + k + i] = n - n_last + i;
+    }
     if (!k) return;
-    uint32_t prefix = 0, want = k;  // the want-th largest of the keys that match the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
-        __syncthreads();
-        const uint32_t high = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-        for (uint32_t i = tid; i < m; i += kSelThreads) {
-            const uint32_t key = total_key(w[i]);
-            if ((key & high) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t left = want;
-            int d = 255;
-            for (; d > 0 && hist[d] < left; --d) left -= hist[d];
-            sh_digit = (uint32_t)d;
-            sh_rank = left;
-        }
-        __syncthreads();
-        prefix |= sh_digit << shift;
-        want = sh_rank;
+    for (uint32_t i = tid; i < 3 * kSelBins; i += kSelThreads) (&sh.hist[0][0])[i] = 0;
+    if (cached) {
+#pragma unroll 8
+        for (uint32_t i = tid; i < len; i += kSelThreads) cache[i] = total_key(w[i]);
     }
-    // keys above `prefix` are kept, and the first `want` that equal it
-    uint32_t done_gt = 0, done_eq = 0;
-    for (uint32_t b = 0; b < m; b += kSelThreads) {
-        const uint32_t i = b + tid;
-        const uint32_t key = i < m ? total_key(w[i]) : 0u;
-        const bool gt = i < m && key > prefix, eq = i < m && key == prefix;
-        const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0) {
-            wsum[0][warp] = __popc(bg);
-            wsum[1][warp] = __popc(be);
+    auto key_of = [&](uint32_t i) { return cached ? cache[i] : total_key(w[i]); };
+    __syncthreads();
+    uint32_t prefix = 0, want = k, my_gt = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+        const uint32_t bins = pass == 2 ? 1024u : 2048u;
+        const uint32_t high = pass == 0 ? 0u : (pass == 1 ? 0xFFFFFFFFu << 21 : 0xFFFFFFFFu << 10);
+        uint32_t* hist = sh.hist[pass];
+#pragma unroll 4
+        for (uint32_t i = tid; i < len; i += kSelThreads) {
+            const uint32_t key = key_of(i);
+            if ((key & high) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
         }
-        __syncthreads();
-        uint32_t g0 = done_gt, e0 = done_eq, tg = 0, te = 0;
-        for (int v = 0; v < kSelThreads / 32; ++v) {
-            if (v < warp) {
-                g0 += wsum[0][v];
-                e0 += wsum[1][v];
+        if (C > 1) cluster.sync();
+        else __syncthreads();
+        // thread t: bins 2t', 2t'+1 counted from the top
+        const uint32_t top = bins - 2 - 2 * tid;
+        uint2 sum = make_uint2(0, 0), own = make_uint2(0, 0);
+        if (2u * tid < bins) {
+            own = *reinterpret_cast<const uint2*>(&hist[top]);
+            sum = own;
+            for (uint32_t r = 1; r < C; ++r) {
+                const uint32_t peer = cr + r < C ? cr + r : cr + r - C;
+                const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[top], peer));
+                sum.x += v.x;
+                sum.y += v.y;
             }
-            tg += wsum[0][v];
-            te += wsum[1][v];
         }
-        const uint32_t lt = (1u << lane) - 1u;
-        g0 += __popc(bg & lt);
-        e0 += __popc(be & lt);
-        if (gt || (eq && e0 < want)) out[n_first + g0 + min(e0, want)] = n_first + i;
-        done_gt += tg;
-        done_eq += te;
+        // inclusive scan of the pairs from the top: keys in this pair's bins or above
+        uint32_t incl = sum.x + sum.y, iown = own.x + own.y;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o), z = __shfl_up_sync(0xffffffffu, iown, o);
+            if (lane >= o) incl += y, iown += z;
+        }
+        if (lane == 31) {
+            sh.warp[warp] = incl;
+            sh.warp_eq[warp] = iown;
+        }
         __syncthreads();
+        uint32_t before = incl - sum.x - sum.y, obefore = iown - own.x - own.y;
+        for (int v = 0; v < warp; ++v) {
+            before += sh.warp[v];
+            obefore += sh.warp_eq[v];
+        }
+        // the bin where the count from the top reaches `want`
+        if (before < want && want <= before + sum.x + sum.y) {
+            const bool up = want <= before + sum.y;  // the higher bin of the pair
+            sh.digit = top + (up ? 1 : 0);
+            sh.rank = want - before - (up ? 0 : sum.y);
+            sh.above = obefore + (up ? 0 : own.y);
+        }
+        __syncthreads();
+        prefix |= sh.digit << shift;
+        want = sh.rank;
+        my_gt += sh.above;  // this CTA's keys in higher bins
     }
+    // keys above `prefix` are kept, and the first `want` of the head that equal it
+    if (tid == 0) {
+        sh.gt = my_gt;
+        sh.eq = sh.hist[2][prefix & 1023u];
+    }
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+    uint32_t gt0 = 0, eq0 = 0;
+    for (uint32_t r = 0; r < cr; ++r) {
+        const SelShared* o = cluster.map_shared_rank(&sh, r);
+        gt0 += o->gt;
+        eq0 += o->eq;
+    }
+    // each warp owns a contiguous run of the range
+    const uint32_t run = (len + kSelThreads - 1) / kSelThreads * 32;
+    const uint32_t wb = min(len, warp * run), we = min(len, wb + run);
+    uint32_t cg_ = 0, ce = 0;
+    for (uint32_t i = wb + lane; i - lane < we; i += 32) {
+        const uint32_t key = i < we ? key_of(i) : 0u;
+        cg_ += __popc(__ballot_sync(0xffffffffu, i < we && key > prefix));
+        ce += __popc(__ballot_sync(0xffffffffu, i < we && key == prefix));
+    }
+    if (lane == 0) {
+        sh.warp[warp] = cg_;
+        sh.warp_eq[warp] = ce;
+    }
+    __syncthreads();
+    for (int v = 0; v < warp; ++v) {
+        gt0 += sh.warp[v];
+        eq0 += sh.warp_eq[v];
+    }
+    const uint32_t lt = (1u << lane) - 1u;
+    for (uint32_t i = wb + lane; i - lane < we; i += 32) {
+        const uint32_t key = i < we ? key_of(i) : 0u;
+        const bool gt = i < we && key > prefix, eq = i < we && key == prefix;
+        const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
+        const uint32_t g = gt0 + __popc(bg & lt), e = eq0 + __popc(be & lt);
+        if (gt || (eq && e < want)) out[n_first + g + min(e, want)] = n_first + b0 + i;
+        gt0 += __popc(bg);
+        eq0 += __popc(be);
+    }
+    if (C > 1) cluster.sync();  // a peer may still read this CTA's counts
 }
 
-constexpr int kMoveThreads = 256;
-constexpr int kMoveUnroll = 4;
+constexpr int kMoveThreads = 512;
+constexpr int kMoveUnroll = 8;
+constexpr uint32_t kMoveWave = kMoveThreads * kMoveUnroll;  // vectors of a CTA per wave
+constexpr uint32_t kMoveMaxCluster = 8;
 constexpr unsigned kErrMoveList = 128u;
 
-// Whether entry i of the list may be moved; raises bit 7 of the error word if not.
-__device__ __forceinline__ bool move_entry(const uint32_t* rows, uint32_t i, uint32_t dst, uint32_t max_ctx,
-                                           unsigned int* err, uint32_t& src) {
-    src = __ldg(rows + i);
-    const bool ok = src < max_ctx && src >= dst + i && (i == 0 || __ldg(rows + i - 1) < src);
-    if (!ok) atomicOr(err, kErrMoveList);
-    return ok && src != dst + i;
+struct MoveArgs {
+    const uint32_t* rows;
+    uint32_t n_rows, dst, max_ctx;
+    unsigned int* err;
+};
+
+// Source row of entry i, or UINT32_MAX where there is nothing to do; an entry
+// that breaks the list's rules raises bit 7 of the error word.
+__device__ __forceinline__ uint32_t move_source(const MoveArgs& a, uint32_t i) {
+    if (i >= a.n_rows) return 0xFFFFFFFFu;
+    const uint32_t src = __ldg(a.rows + i);
+    const bool ok = src < a.max_ctx && src >= a.dst + i && (i == 0 || __ldg(a.rows + i - 1) < src);
+    if (!ok) atomicOr(a.err, kErrMoveList);
+    return ok && src != a.dst + i ? src : 0xFFFFFFFFu;
 }
 
-// grid (hd / 16, n_kv, 2): 16 columns of one head of K or V
-__global__ void __launch_bounds__(kMoveThreads)
-    smallm_cache_move_kernel(float* kc, float* vc, uint32_t hd, uint32_t max_ctx, const uint32_t* __restrict__ lists,
-                             uint32_t list_stride, uint32_t n_rows, uint32_t dst, unsigned int* err) {
-    const uint32_t* rows = lists + (size_t)blockIdx.y * list_stride;
-    float* base = (blockIdx.z ? vc : kc) + (size_t)blockIdx.y * max_ctx * hd + blockIdx.x * 16 + (threadIdx.x & 3) * 4;
-    constexpr uint32_t kStep = kMoveThreads / 4;
-    for (uint32_t b = 0; b < n_rows; b += kStep * kMoveUnroll) {
-        float4 v[kMoveUnroll];
-        bool go[kMoveUnroll];
+// base[(dst + i) * pitch + c] = base[rows[i] * pitch + c] for c < width
+// (vectors of type V); the cluster's CTAs take consecutive parts of a wave.
+template <typename V>
+__device__ __forceinline__ void move_rows(V* base, uint32_t pitch, uint32_t width, const MoveArgs& a, uint32_t C,
+                                          uint32_t cr) {
+    const uint32_t wave = kMoveWave * C / width;  // rows per wave (width divides kMoveWave)
+    const uint32_t c = threadIdx.x % width, r0 = (cr * kMoveWave + threadIdx.x) / width;
+    constexpr uint32_t kStep = kMoveThreads;
+    uint32_t src[kMoveUnroll];
+    V v[kMoveUnroll];
+    auto sources = [&](uint32_t first) {
 #pragma unroll
-        for (int u = 0; u < kMoveUnroll; ++u) {
-            const uint32_t i = b + u * kStep + (threadIdx.x >> 2);
-            uint32_t src = 0;
-            go[u] = i < n_rows && move_entry(rows, i, dst, max_ctx, err, src);
-            if (go[u]) v[u] = *reinterpret_cast<const float4*>(base + (size_t)src * hd);
-        }
-        __syncthreads();
+        for (int u = 0; u < kMoveUnroll; ++u) src[u] = move_source(a, first + r0 + u * (kStep / width));
+    };
+    sources(0);
+    for (uint32_t first = 0; first < a.n_rows; first += wave) {
+        uint32_t go = 0;
 #pragma unroll
-        for (int u = 0; u < kMoveUnroll; ++u) {
-            const uint32_t i = b + u * kStep + (threadIdx.x >> 2);
-            if (go[u]) *reinterpret_cast<float4*>(base + (size_t)(dst + i) * hd) = v[u];
-        }
-        __syncthreads();
+        for (int u = 0; u < kMoveUnroll; ++u)
+            if (src[u] != 0xFFFFFFFFu) {
+                v[u] = base[(size_t)src[u] * pitch + c];
+                go |= 1u << u;
+            }
+        if (first + wave < a.n_rows) sources(first + wave);
+        if (C > 1) cg::this_cluster().sync();
+        else __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kMoveUnroll; ++u)
+            if (go >> u & 1)
+                base[(size_t)(a.dst + first + r0 + u * (kStep / width)) * pitch + c] = v[u];
     }
 }
 
-__global__ void __launch_bounds__(1024)
-    smallm_cache_move_totals_kernel(float* weights, uint32_t max_ctx, const uint32_t* __restrict__ lists,
-                                    uint32_t list_stride, uint32_t n_rows, uint32_t dst, unsigned int* err) {
-    const uint32_t* rows = lists + (size_t)blockIdx.x * list_stride;
-    float* w = weights + (size_t)blockIdx.x * max_ctx;
-    for (uint32_t b = 0; b < n_rows; b += 1024) {
-        const uint32_t i = b + threadIdx.x;
-        uint32_t src = 0;
-        const bool go = i < n_rows && move_entry(rows, i, dst, max_ctx, err, src);
-        const float v = go ? w[src] : 0.f;
-        __syncthreads();
-        if (go) w[dst + i] = v;
-        __syncthreads();
+// grid.x: (slice of columns) x cluster, grid.y: head, grid.z: K, V, totals
+__global__ void __launch_bounds__(kMoveThreads, 1)
+    smallm_cache_move_kernel(float* kc, float* vc, float* totals, uint32_t hd, uint32_t slice, MoveArgs a,
+                             uint32_t list_stride) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t C = cluster.num_blocks(), cr = cluster.block_rank(), part = blockIdx.x / C;
+    a.rows += (size_t)blockIdx.y * list_stride;
+    if (blockIdx.z == 2) {
+        if (part == 0) move_rows<float>(totals + (size_t)blockIdx.y * a.max_ctx, 1, 1, a, C, cr);
+        return;
     }
+    float4* base = reinterpret_cast<float4*>((blockIdx.z ? vc : kc) + (size_t)blockIdx.y * a.max_ctx * hd) +
+                   part * slice;
+    move_rows<float4>(base, hd / 4, slice, a, C, cr);
+}
+
+void launch_cluster(const void* fn, dim3 grid, uint32_t threads, size_t smem, uint32_t C, cudaStream_t stream,
+                    void** args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
 }
 
 }  // namespace
@@ -155,8 +271,16 @@ void launch_cache_select(const float* weights, uint32_t n_kv, uint32_t max_ctx, 
         throw Error(SMALLM_ERR_INVALID, "cache_select: needs n_first + n_last <= n_keep <= n");
     if (n_kv > 65535) throw Error(SMALLM_ERR_RANGE, "cache_select: at most 65535 KV heads");
     if (!n_kv || !n_keep) return;
-    smallm_cache_select_kernel<<<n_kv, kSelThreads, 0, stream>>>(weights, max_ctx, n, n_keep, n_first, n_last, rows);
-    SM_CUDA(cudaGetLastError());
+    // CTAs per head: a couple of keys per thread at least, one CTA per SM in all
+    const uint32_t m = n - n_first - n_last, sms = (uint32_t)device_sm_count();
+    uint32_t C = 1;
+    while (C < kSelMaxCluster && m > C * 2 * kSelThreads && n_kv * C * 2 <= sms) C *= 2;
+    uint32_t per_cta = (m + C - 1) / C, cached = per_cta <= kSelCached;
+    const void* fn = (const void*)smallm_cache_select_kernel;
+    set_smem_limit_once(fn, (int)(4 * kSelCached));
+    if (C > 8) SM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    void* args[] = {&weights, &max_ctx, &n, &n_keep, &n_first, &n_last, &per_cta, &cached, &rows};
+    launch_cluster(fn, dim3(n_kv * C), kSelThreads, cached ? 4ull * per_cta : 0, C, stream, args);
 }
 
 void launch_cache_move(float* kcache, float* vcache, float* weights, uint32_t n_kv, uint32_t hd, uint32_t max_ctx,
@@ -169,15 +293,17 @@ void launch_cache_move(float* kcache, float* vcache, float* weights, uint32_t n_
     if ((reinterpret_cast<uintptr_t>(kcache) | reinterpret_cast<uintptr_t>(vcache)) & 15u)
         throw Error(SMALLM_ERR_INVALID, "cache_move: kcache and vcache must be 16-byte aligned");
     if (!n_kv || !n_rows) return;
-    unsigned int* err = device_error_flag();
-    const uint32_t stride = per_head ? n_rows : 0;
-    smallm_cache_move_kernel<<<dim3(hd / 16, n_kv, 2), kMoveThreads, 0, stream>>>(kcache, vcache, hd, max_ctx, rows,
-                                                                                stride, n_rows, dst, err);
-    SM_CUDA(cudaGetLastError());
-    if (weights) {
-        smallm_cache_move_totals_kernel<<<n_kv, 1024, 0, stream>>>(weights, max_ctx, rows, stride, n_rows, dst, err);
-        SM_CUDA(cudaGetLastError());
-    }
+    // CTAs of a cluster: no more than the rows fill a wave of; then slices of
+    // columns (16 floats, two 32-byte sectors, at least) until the SMs are used
+    const uint32_t sms = (uint32_t)device_sm_count();
+    uint32_t C = 1, slices = 1;
+    while (C < kMoveMaxCluster && (uint64_t)n_rows * hd / 4 > (uint64_t)C * kMoveWave && n_kv * 2 * C * 2 <= sms) C *= 2;
+    while (hd / slices > 16 && n_kv * 2 * C * slices * 2 <= sms && n_rows > 64) slices *= 2;
+    MoveArgs a{rows, n_rows, dst, max_ctx, device_error_flag()};
+    uint32_t slice = hd / 4 / slices, stride = per_head ? n_rows : 0;
+    void* args[] = {&kcache, &vcache, &weights, &hd, &slice, &a, &stride};
+    launch_cluster((const void*)smallm_cache_move_kernel, dim3(slices * C, n_kv, weights ? 3 : 2), kMoveThreads, 0, C,
+                   stream, args);
 }
 
 }  // namespace smallm

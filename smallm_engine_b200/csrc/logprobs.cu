@@ -8,6 +8,23 @@
 // order of their ids (NaN last).  A logit of -inf has probability 0 and adds
 // nothing to the entropy; a row that holds NaN or +inf, or nothing above
 // -inf, has no distribution, and its log probabilities and entropy are NaN.
+//
+// Bound by the one read of the logits.  A cluster of 1 to 16 CTAs owns a row
+// (more CTAs when there are few rows), each a contiguous range of it, 16
+// elements of a thread at a time with the next 16 already in flight:
+//   - (m, S0, S1) run per thread; a larger maximum m' rescales them,
+//     S1' = e^(m - m') (S1 + (m - m') S0);
+//   - alternatives are 64-bit keys (value, then lower id), unique in a row.  A
+//     threshold below which nothing can be among the n_top best lets nearly
+//     every chunk pass with one comparison per thread; what is above it is
+//     collected in shared memory, and when much is, the list is ranked and cut
+//     to n_top, its last key the new threshold.  Where half the threads or
+//     more hold something above it (the first chunk; ascending rows), the
+//     n_top-th largest of 128 group maxima (2 threads, 32 elements) raises it
+//     first: n_top groups reach it, so at most 32 n_top elements do.
+// Rank 0 joins the ranges through distributed shared memory.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "engine.h"
 #include "smallm_cuda.h"
@@ -15,72 +32,257 @@
 namespace smallm {
 namespace {
 
-constexpr int kLpThreads = 1024;
-constexpr int kLpWarps = kLpThreads / 32;
+namespace cg = cooperative_groups;
 
-// Larger key = earlier alternative; keys are unique within a row.
-__device__ __forceinline__ unsigned long long alt_key(float x, uint32_t i) {
+constexpr int kLpThreads = 256;
+constexpr int kLpVec = 4;                          // float4s of a thread per chunk
+constexpr uint32_t kLpChunk = kLpThreads * kLpVec;  // float4s of a CTA per chunk
+constexpr uint32_t kLpMaxCluster = 16;
+constexpr uint32_t kLpGroups = kLpThreads / 2;
+constexpr uint32_t kLpCut = 128;  // collected keys that make a cut worth its barriers
+constexpr uint32_t kLpKeys = kLogprobMaxTop * 2 * kLpVec * 4 + kLpCut + kLogprobMaxTop;
+static_assert(kLpGroups >= kLogprobMaxTop && kLpKeys >= kLpMaxCluster * kLogprobMaxTop, "key buffer");
+
+typedef unsigned long long u64;
+
+struct LpShared {
+    u64 keys[kLpKeys];          // collected
+    u64 best[kLogprobMaxTop];   // ranked
+    u64 group[kLpGroups];
+    u64 floor;                  // only larger keys matter
+    uint32_t count, n_best;
+    float m, s0, s1;
+    uint32_t bad;
+    float wm[kLpThreads / 32], w0[kLpThreads / 32], w1[kLpThreads / 32];
+};
+
+// Larger key = earlier alternative; never 0.
+__device__ __forceinline__ u64 alt_key(float x, uint32_t i) {
     const uint32_t o = x == x ? float_order_key(x + 0.f) : 0u;
-    return ((unsigned long long)o << 32) | (0xFFFFFFFFu - i);
+    return ((u64)o << 32) | (0xFFFFFFFFu - i);
+}
+__device__ __forceinline__ float alt_value(u64 k) {
+    const uint32_t o = (uint32_t)(k >> 32);
+    return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// e^d of d <= 0; 0 below -200.
+__device__ __forceinline__ float exp_neg(float d) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+    return r;
+}
+// (m, s0, s1) joined with another range's.
+__device__ __forceinline__ void join(float& m, float& s0, float& s1, float om, float o0, float o1) {
+    const float M = fmaxf(m, om);
+    if (M == -INFINITY) return;
+    const float da = fmaxf(m - M, -200.f), db = fmaxf(om - M, -200.f);
+    const float fa = exp_neg(da), fb = exp_neg(db);
+    s1 = fa * fmaf(da, s0, s1) + fb * fmaf(db, o0, o1);
+    s0 = fa * s0 + fb * o0;
+    m = M;
 }
 
-__device__ unsigned long long block_max_key(unsigned long long k, unsigned long long* red) {
+// Rank the collected keys (unique) and keep the `want` largest: best[0..),
+// largest first, and again at the front of keys.  All threads call it.
+__device__ void lp_cut(LpShared& sh, uint32_t want) {
+    const uint32_t c = sh.count;
+    for (uint32_t i = threadIdx.x; i < c; i += kLpThreads) {
+        const u64 k = sh.keys[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < c; ++j) rank += sh.keys[j] > k;
+        if (rank < want) sh.best[rank] = k;
+    }
+    __syncthreads();
+    const uint32_t n = min(c, want);
+    if (threadIdx.x < n) sh.keys[threadIdx.x] = sh.best[threadIdx.x];
+    if (threadIdx.x == 0) {
+        sh.count = sh.n_best = n;
+        if (n == want && sh.best[n - 1] > sh.floor) sh.floor = sh.best[n - 1];
+    }
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(kLpThreads, 4) smallm_logprobs_kernel(const LogprobArgs a, uint32_t per_cta) {
+    __shared__ LpShared sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / C;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float* x = a.logits + (size_t)row * a.stride;
+    // float4s of the row from the 16-byte boundary at or before its start
+    const uint32_t mis = (uint32_t)(reinterpret_cast<uintptr_t>(x) >> 2) & 3u;
+    const uint32_t nq = (uint32_t)(((uint64_t)a.vocab + mis + 3) / 4);
+    const uint32_t qb = min(nq, rank * per_cta), qe = min(nq, qb + per_cta);
+    auto load = [&](uint32_t q, float (&v)[4]) {
+        const uint32_t i = 4 * q - mis;  // wraps below the row's start
+        if (q < qe && i < a.vocab && i + 3 < a.vocab) {
+            *reinterpret_cast<float4*>(v) = __ldcs(reinterpret_cast<const float4*>(x - mis) + q);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = q < qe && i + c < a.vocab ? x[i + c] : -INFINITY;
+        }
+    };
+    if (tid == 0) {
+        sh.floor = 0;
+        sh.count = 0;
+        sh.n_best = 0;
+    }
+    float m = -INFINITY, s0 = 0.f, s1 = 0.f;
+    bool bad = false;
+    float next[kLpVec][4];
+#pragma unroll
+    for (int u = 0; u < kLpVec; ++u) load(qb + u * kLpThreads + tid, next[u]);
+    __syncthreads();
+    for (uint32_t q0 = qb; q0 < qe; q0 += kLpChunk) {
+        float v[kLpVec][4];
+#pragma unroll
+        for (int u = 0; u < kLpVec; ++u)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[u][c] = next[u][c];
+        if (q0 + kLpChunk < qe) {
+#pragma unroll
+            for (int u = 0; u < kLpVec; ++u) load(q0 + kLpChunk + u * kLpThreads + tid, next[u]);
+        }
+        float xm = v[0][0];
+#pragma unroll
+        for (int u = 0; u < kLpVec; ++u)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) xm = max_nan(xm, v[u][c]);
+        bad |= !(xm < INFINITY);
+        if (xm > m) {
+            const float d = fmaxf(m - xm, -200.f), f = exp_neg(d);
+            s1 = f * fmaf(d, s0, s1);
+            s0 *= f;
+            m = xm;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float c0 = 0.f, c1 = 0.f;
+#pragma unroll
+        for (int u = 0; u < kLpVec; ++u)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float d = fmaxf(v[u][c] - ref, -200.f), e = exp_neg(d);
+                c0 += e;
+                c1 = fmaf(e, d, c1);
+            }
+        s0 += c0;
+        s1 += c1;
+        if (!a.n_top) continue;
+        // ids of this thread's elements: first of float4 u, or past vocab
+        auto id_of = [&](int u, int c) { return 4 * (q0 + u * kLpThreads + tid) - mis + c; };
+        auto in_row = [&](int u, int c) {
+            return q0 + u * kLpThreads + tid < qe && id_of(u, c) < a.vocab;
+        };
+        u64 floor = sh.floor;
+        const bool over = !(xm < INFINITY) || float_order_key(xm + 0.f) >= (uint32_t)(floor >> 32);
+        const int n_over = __syncthreads_count(over);
+        if (!n_over) continue;
+        if (n_over > kLpThreads / 2) {
+            u64 k = 0;
+#pragma unroll
+            for (int u = 0; u < kLpVec; ++u)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (in_row(u, c)) {
+                        const u64 y = alt_key(v[u][c], id_of(u, c));
+                        k = y > k ? y : k;
+                    }
+            const u64 other = __shfl_xor_sync(0xffffffffu, k, 1);
+            k = other > k ? other : k;
+            if (!(tid & 1)) sh.group[tid >> 1] = k;
+            __syncthreads();
+            if (tid < (int)kLpGroups) {
+                const u64 mine = sh.group[tid];
+                uint32_t larger = 0;
+                const ulonglong2* gk = reinterpret_cast<const ulonglong2*>(sh.group);
+#pragma unroll 8
+                for (uint32_t j = 0; j < kLpGroups / 2; ++j) {
+                    const ulonglong2 y = gk[j];
+                    larger += (y.x > mine) + (y.y > mine);
+                }
+                if (mine && larger == a.n_top - 1 && mine - 1 > sh.floor) sh.floor = mine - 1;
+            }
+            __syncthreads();
+            floor = sh.floor;
+        }
+        if (over) {
+#pragma unroll
+            for (int u = 0; u < kLpVec; ++u)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const u64 k = alt_key(v[u][c], id_of(u, c));
+                    if (k > floor && in_row(u, c)) sh.keys[atomicAdd(&sh.count, 1u)] = k;
+                }
+        }
+        __syncthreads();
+        if (sh.count > kLpCut) lp_cut(sh, a.n_top);
+    }
+    if (a.n_top) lp_cut(sh, a.n_top);
+    // this CTA's (m, s0, s1)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long y = __shfl_xor_sync(0xffffffffu, k, o);
-        k = y > k ? y : k;
+        const float om = __shfl_xor_sync(0xffffffffu, m, o), o0 = __shfl_xor_sync(0xffffffffu, s0, o),
+                    o1 = __shfl_xor_sync(0xffffffffu, s1, o);
+        join(m, s0, s1, om, o0, o1);
     }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = k;
-    __syncthreads();
-    for (int w = 0; w < kLpWarps; ++w) k = red[w] > k ? red[w] : k;
-    return k;
-}
-
-__global__ void __launch_bounds__(kLpThreads) smallm_logprobs_kernel(const LogprobArgs a) {
-    __shared__ float red[32];
-    __shared__ unsigned long long kred[kLpWarps];
-    const float* x = a.logits + (size_t)blockIdx.x * a.stride;
-    unsigned long long best = 0;
-    bool bad = false;
-    for (uint32_t i = threadIdx.x; i < a.vocab; i += kLpThreads) {
-        const float v = x[i];
-        bad |= !(v < INFINITY);
-        const unsigned long long k = alt_key(v, i);
-        best = k > best ? k : best;
+    if (lane == 0) {
+        sh.wm[warp] = m;
+        sh.w0[warp] = s0;
+        sh.w1[warp] = s1;
     }
-    best = block_max_key(best, kred);
-    const float m = x[0xFFFFFFFFu - (uint32_t)best];
-    bad = __syncthreads_or(bad) || m == -INFINITY;
-    float s0 = 0.f, s1 = 0.f;
-    for (uint32_t i = threadIdx.x; i < a.vocab; i += kLpThreads) {
-        const float d = x[i] - m, e = expf(d);
-        s0 += e;
-        s1 += e > 0.f ? e * d : 0.f;
+    bad = __syncthreads_or(bad);
+    if (tid == 0) {
+        for (int w = 1; w < kLpThreads / 32; ++w) join(m, s0, s1, sh.wm[w], sh.w0[w], sh.w1[w]);
+        sh.m = m;
+        sh.s0 = s0;
+        sh.s1 = s1;
+        sh.bad = bad;
     }
-    s0 = block_sum(s0, red);
-    s1 = block_sum(s1, red);
+    if (C > 1) {
+        cluster.sync();
+        if (rank == 0) {
+            // own ranked keys stay at the front of keys; the others' follow
+            const uint32_t top = a.n_top;
+            for (uint32_t i = tid; i < (C - 1) * top; i += kLpThreads) {
+                const uint32_t r = 1 + i / top, j = i % top;
+                const LpShared* o = cluster.map_shared_rank(&sh, r);
+                if (j < o->n_best) sh.keys[atomicAdd(&sh.count, 1u)] = o->best[j];
+            }
+            if (tid == 0) {
+                for (uint32_t r = 1; r < C; ++r) {
+                    const LpShared* o = cluster.map_shared_rank(&sh, r);
+                    join(m, s0, s1, o->m, o->s0, o->s1);
+                    sh.bad |= o->bad;
+                }
+                sh.m = m;
+                sh.s0 = s0;
+                sh.s1 = s1;
+            }
+            __syncthreads();
+            if (top) lp_cut(sh, top);
+        }
+        cluster.sync();
+        if (rank) return;
+    } else {
+        __syncthreads();
+    }
     const float nan = __int_as_float(0x7FC00000);
-    const float ls = bad ? nan : logf(s0);
-    if (threadIdx.x == 0) {
-        if (a.entropy) a.entropy[blockIdx.x] = ls - s1 / s0;
+    const float M = sh.m, ls = sh.bad || M == -INFINITY ? nan : logf(sh.s0);
+    if (tid == 0) {
+        if (a.entropy) a.entropy[row] = ls - sh.s1 / sh.s0;
         if (a.tokens) {
-            const uint32_t t = a.tokens[blockIdx.x];
-            a.logprob[blockIdx.x] = t < a.vocab ? (x[t] - m) - ls : nan;
+            const uint32_t t = a.tokens[row];
+            a.logprob[row] = t < a.vocab ? (x[t] - M) - ls : nan;
         }
     }
-    for (uint32_t r = 0; r < a.n_top; ++r) {
-        if (threadIdx.x == 0) {
-            const uint32_t id = 0xFFFFFFFFu - (uint32_t)best;
-            a.top_ids[(size_t)blockIdx.x * a.n_top + r] = id;
-            a.top_logprobs[(size_t)blockIdx.x * a.n_top + r] = (x[id] - m) - ls;
-        }
-        unsigned long long next = 0;
-        for (uint32_t i = threadIdx.x; i < a.vocab; i += kLpThreads) {
-            const unsigned long long k = alt_key(x[i], i);
-            if (k < best && k > next) next = k;
-        }
-        best = block_max_key(next, kred);
+    for (uint32_t i = tid; i < a.n_top; i += kLpThreads) {
+        const u64 k = sh.best[i];
+        a.top_ids[(size_t)row * a.n_top + i] = 0xFFFFFFFFu - (uint32_t)k;
+        a.top_logprobs[(size_t)row * a.n_top + i] = (alt_value(k) - M) - ls;
     }
 }
 
@@ -88,12 +290,33 @@ __global__ void __launch_bounds__(kLpThreads) smallm_logprobs_kernel(const Logpr
 
 void launch_logprobs(const LogprobArgs& a, cudaStream_t stream) {
     if (!a.vocab) throw Error(SMALLM_ERR_INVALID, "logprobs: an empty vocabulary");
+    if (a.vocab > 1u << 30) throw Error(SMALLM_ERR_RANGE, "logprobs: at most 2^30 logits per row");
     if (a.stride < a.vocab) throw Error(SMALLM_ERR_INVALID, "logprobs: stride must be at least vocab");
     if (a.n_top > kLogprobMaxTop || a.n_top > a.vocab)
         throw Error(SMALLM_ERR_RANGE, "logprobs: at most 64 alternatives, and no more than vocab");
+    if (a.n_rows > 1u << 26) throw Error(SMALLM_ERR_RANGE, "logprobs: at most 2^26 rows");
     if (!a.n_rows) return;
-    smallm_logprobs_kernel<<<a.n_rows, kLpThreads, 0, stream>>>(a);
-    SM_CUDA(cudaGetLastError());
+    // CTAs per row: two per SM in all, each with a chunk to itself at least
+    const uint32_t nq = (a.vocab + 6) / 4, sms = (uint32_t)device_sm_count();
+    uint32_t C = 1;
+    while (C < kLpMaxCluster && a.n_rows * C < 2 * sms && nq > C * kLpChunk) C *= 2;
+    const void* fn = (const void*)smallm_logprobs_kernel;
+    if (C > 8) SM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.n_rows * C);
+    cfg.blockDim = dim3(kLpThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    LogprobArgs aa = a;
+    uint32_t per_cta = (nq + C - 1) / C;
+    void* args[] = {&aa, &per_cta};
+    SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
 }
 
 }  // namespace smallm
