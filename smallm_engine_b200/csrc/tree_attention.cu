@@ -229,11 +229,12 @@ __global__ void __launch_bounds__(kVecThreads, 2) smallm_tree_vec_kernel(const T
 // lo hi) leave out 2^-24 of the operands' size.  e brings the largest
 // magnitude of the tile (K, V) or row (q) to [2^14, 2^15), so an element loses
 // bits only below 2^-39 of that.  The small products are accumulated first.
-//   - warps 12..19 convert: 256 threads hold the next K and V tile in
-//     registers (64 KB in flight), find the tile's exponent and write hi and
-//     lo in the MMA's swizzled layout, three slots for each of K and V;
-//   - warp 20, one lane, issues S = Q K^T (Q in tensor memory) and, a tile
-//     behind, O = P V (P in tensor memory, V MN-major);
+//   - warps 12..15 (K) and 16..19 (V) convert: a group holds the next tile in
+//     registers (32 KB in flight each), finds its exponent and writes hi and
+//     lo in the MMA's swizzled layout, three slots for each of K and V; the
+//     load of the tile after goes out as soon as a register is free;
+//   - warp 20 issues S = Q K^T (Q in tensor memory) and, a tile behind,
+//     O = P V (P in tensor memory, over S's columns; V MN-major);
 //   - warps 0..3, lane = row: running maximum (a whole number in base 2, so
 //     rescaling is exact), P = 2^(s - m + 14) as hi and lo, sum;
 //   - warps 4..11, lane = row: O of each tile leaves tensor memory and is added
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kVecThreads, 2) smallm_tree_vec_kernel(const T
 // Every wait is bounded; one that gives up raises bit 8 of the error word.
 constexpr uint32_t kTcRows = 128, kTcKeys = 64, kTcSlots = 3, kTcRing = 8, kTcCorr = 4;
 // six warpgroups; registers per thread 80 at launch (480 over the six), then
-// 104 softmax + 2 x 88 output + 2 x 88 converters + 24 issuer = 480
+// 104 softmax + 2 x 88 output + 2 x 80 converters + 40 issuer = 480
 constexpr uint32_t kTcThreads = 32 * 24;
 constexpr unsigned kErrTreeWait = 256u;
 constexpr float kPShift = 14.f;
@@ -256,18 +257,18 @@ struct TcTree {
     static constexpr uint32_t slot = 2 * half;
     static constexpr size_t smem = 1024 + 2ull * kTcSlots * slot + 8192;
     static constexpr uint32_t pv_n = HD < 64 ? 64 : HD;         // columns past HD are never read
-    // tensor-memory columns
-    static constexpr uint32_t q_hi = 0, q_lo = 64, s0 = 128, p0 = 256, o = 384;
+    // tensor-memory columns; P (hi 32, lo 32) takes the place of its S
+    static constexpr uint32_t q_hi = 0, q_lo = 64, s0 = 128, o0 = 256;
     static constexpr uint32_t idesc_s = (1u << 4) | ((kTcKeys >> 3) << 17) | ((kTcRows >> 4) << 24);
     static constexpr uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((pv_n >> 3) << 17) | ((kTcRows >> 4) << 24);
 };
 
 struct TcShared {
     uint64_t k_full[kTcSlots], k_empty[kTcSlots], v_full[kTcSlots], v_empty[kTcSlots];
-    uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2], o_full, o_empty, q_full, ml_full, done;
+    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, ml_full, done;
     float k_scale[kTcRing], v_scale[kTcRing];
-    unsigned long long bad[kTcRing];
-    uint32_t wmax[3][8];
+    unsigned long long k_bad[kTcRing], v_bad[kTcRing];
+    alignas(16) uint32_t wmax[2][2][4];
     uint32_t tmem;
     float corr[kTcCorr][kTcRows];
     float2 ml[kTcRows];
@@ -287,14 +288,14 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
-// Barrier of the 256 converter threads; true where any of them says so.
-__device__ __forceinline__ bool conv_any(bool v) {
+// Barrier of the 128 threads of converter group `id`; true where any says so.
+__device__ __forceinline__ bool conv_any(int id, bool v) {
     uint32_t r;
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 256, p;\n"
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 128, p;\n"
         " selp.u32 %0, 1, 0, q;\n}"
         : "=r"(r)
-        : "r"((uint32_t)v)
+        : "r"((uint32_t)v), "r"(id)
         : "memory");
     return r != 0;
 }
@@ -303,75 +304,116 @@ __device__ __forceinline__ float ex2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-
-// One tile's K or V of a converter thread: units of 8 consecutive floats.
-template <int HD>
-struct TcUnits {
-    static constexpr int n = (int)(kTcKeys * (HD / 8) / 256);
-    float x[n][8];
-    __device__ __forceinline__ void load(const float* base, uint32_t key0, uint32_t n_keys, int tid) {
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            const uint32_t u = i * 256 + tid, key = key0 + u / (HD / 8);
-            const float4* p = reinterpret_cast<const float4*>(base + (size_t)key * HD + u % (HD / 8) * 8);
-            const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(&x[i][0]) = key < n_keys ? __ldg(p) : z;
-            *reinterpret_cast<float4*>(&x[i][4]) = key < n_keys ? __ldg(p + 1) : z;
-        }
-    }
-    __device__ __forceinline__ uint32_t max_bits() const {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < n; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
-        return m;
-    }
-    // Infinities and NaN become 0 and mark their key.
-    __device__ __forceinline__ void clean(unsigned long long* bad, int tid) {
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            bool any = false;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if ((__float_as_uint(x[i][j]) & 0x7FFFFFFFu) >= 0x7F800000u) {
-                    x[i][j] = 0.f;
-                    any = true;
-                }
-            if (any) atomicOr(bad, 1ull << ((i * 256 + tid) / (HD / 8)));
-        }
-    }
-    __device__ __forceinline__ void store(uint8_t* slot, float mult, int tid) const {
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            const uint32_t u = i * 256 + tid, row = u / (HD / 8), c8 = u % (HD / 8);
-            uint8_t* dst = slot + (c8 >> 3) * (kTcKeys * 128) + row * 128 + (((c8 & 7) ^ (row & 7)) << 4);
-            uint4 hi, lo;
-            split_f16(x[i][0] * mult, x[i][1] * mult, hi.x, lo.x);
-            split_f16(x[i][2] * mult, x[i][3] * mult, hi.y, lo.y);
-            split_f16(x[i][4] * mult, x[i][5] * mult, hi.z, lo.z);
-            split_f16(x[i][6] * mult, x[i][7] * mult, hi.w, lo.w);
-            *reinterpret_cast<uint4*>(dst) = hi;
-            *reinterpret_cast<uint4*>(dst + TcTree<HD>::half) = lo;
-        }
-    }
-};
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+    float r;
+    asm("{\n .reg .f32 t;\n abs.f32 t, %2;\n max.NaN.f32 %0, %1, t;\n}" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// A streaming load that stays where it is written (a plain one may sink to its use).
+__device__ __forceinline__ float4 load_stream(const float* p) {
+    float4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "l"(p));
+    return v;
+}
 
 // Bits of the 64 keys from key0 that row token t sees.
-__device__ __forceinline__ unsigned long long tc_seen(const TreeParams& p, uint32_t t, uint32_t key0) {
+__device__ __forceinline__ unsigned long long tc_seen(const uint32_t* mask, uint32_t n_past, uint32_t n_tokens,
+                                                   uint32_t t, uint32_t key0) {
+    const uint32_t words = (n_tokens + 31) / 32;
     unsigned long long m = 0;
-    const int64_t u0 = (int64_t)key0 - p.a.n_past;  // drafted index of the tile's first key
+    const int64_t u0 = (int64_t)key0 - n_past;  // drafted index of the tile's first key
     if (u0 < 0) m = u0 <= -64 ? ~0ull : (1ull << -u0) - 1;
     for (int w = 0; w < 3; ++w) {  // mask words that overlap [u0, u0 + 64)
         const int64_t word = (u0 < 0 ? 0 : u0 >> 5) + w, at = word * 32 - u0;
-        if (word >= p.words || at >= 64) break;
+        if (word >= words || at >= 64) break;
         uint32_t bits;
-        if (p.a.mask) bits = p.a.mask[(size_t)t * p.words + word];
+        if (mask) bits = mask[(size_t)t * words + word];
         else bits = t >= word * 32 + 31 ? ~0u : (t < word * 32 ? 0u : (2u << (t & 31)) - 1u);
-        if (word == p.words - 1 && p.a.n_tokens % 32) bits &= (1u << (p.a.n_tokens % 32)) - 1u;
+        if (word == words - 1 && n_tokens % 32) bits &= (1u << (n_tokens % 32)) - 1u;
         m |= at >= 0 ? (unsigned long long)bits << at : (unsigned long long)(bits >> -at);
     }
     return m;
+}
+
+// One converter group: tiles t0 .. t0 + nt - 1 of `src` into `slots`.
+template <int HD>
+__device__ __forceinline__ bool tc_convert(const float* src, uint32_t n, uint32_t t0, uint32_t nt, int group, int tid,
+                                           uint8_t* slots, uint64_t* full, uint64_t* empty, float* scales,
+                                           unsigned long long* bads, uint32_t (*wmax)[4]) {
+    using C = TcTree<HD>;
+    constexpr int N = (int)kTcKeys * HD / 4 / 128;  // float4s of a thread
+    constexpr uint32_t W = HD / 4;                  // float4s of a row
+    const uint32_t c4 = tid % W, row0 = tid / W;    // row of unit i: row0 + i * (128 / W)
+    const float* p = src + (size_t)(t0 * kTcKeys + row0) * HD + 4 * c4;
+    uint32_t key = t0 * kTcKeys + row0;
+    float4 x[N];
+    auto load = [&](int i) {
+        x[i] = key + i * (128 / W) < n ? load_stream(p + (size_t)i * (128 / W) * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+#pragma unroll
+    for (int i = 0; i < N; ++i) load(i);
+    const uint32_t dst0 = (c4 >> 4) * (kTcKeys * 128) + (c4 & 1) * 8;
+    const int lane = tid & 31, cw = tid >> 5;
+    for (uint32_t t = 0; t < nt; ++t) {
+        const uint32_t slot = t % kTcSlots, use = t / kTcSlots, ring = t % kTcRing;
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            m = max_abs_nan(max_abs_nan(max_abs_nan(max_abs_nan(m, x[i].x), x[i].y), x[i].z), x[i].w);
+        const uint32_t mw = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+        if (lane == 0) wmax[t & 1][cw] = mw;
+        if (tid == 0) bads[ring] = 0;
+        const bool stuck = use > 0 && !mbar_wait(&empty[slot], (use - 1) & 1);
+        if (conv_any(1 + group, stuck)) return false;
+        uint4 mx4 = *reinterpret_cast<const uint4*>(wmax[t & 1]);
+        uint32_t mx = max(max(mx4.x, mx4.y), max(mx4.z, mx4.w));
+        if (mx >= 0x7F800000u) {  // the same for all 128 threads: clean the tile
+            m = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                bool any = false;
+                auto clean = [&](float& v) {
+                    if ((__float_as_uint(v) & 0x7FFFFFFFu) >= 0x7F800000u) {
+                        v = 0.f;
+                        any = true;
+                    }
+                    m = fmaxf(m, fabsf(v));
+                };
+                clean(x[i].x), clean(x[i].y), clean(x[i].z), clean(x[i].w);
+                if (any) atomicOr(&bads[ring], 1ull << (row0 + i * (128 / W)));
+            }
+            const uint32_t m2 = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+            conv_any(1 + group, false);  // wmax has been read by all
+            if (lane == 0) wmax[t & 1][cw] = m2;
+            conv_any(1 + group, false);
+            mx4 = *reinterpret_cast<const uint4*>(wmax[t & 1]);
+            mx = max(max(mx4.x, mx4.y), max(mx4.z, mx4.w));
+        }
+        float mult, inv;
+        tc_scale(mx, mult, inv);
+        if (tid == 0) scales[ring] = inv;
+        uint8_t* dst = slots + slot * C::slot + dst0;
+        key += kTcKeys;
+        p += (size_t)kTcKeys * HD;
+        const bool more = t + 1 < nt;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t row = row0 + i * (128 / W);
+            uint8_t* d = dst + row * 128 + ((((c4 & 15) >> 1) ^ (row & 7)) << 4);
+            uint2 hi, lo;
+            split_f16(x[i].x * mult, x[i].y * mult, hi.x, lo.x);
+            split_f16(x[i].z * mult, x[i].w * mult, hi.y, lo.y);
+            *reinterpret_cast<uint2*>(d) = hi;
+            *reinterpret_cast<uint2*>(d + C::half) = lo;
+            if (more) load(i);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[slot]);
+    }
+    return true;
 }
 
 template <int HD>
@@ -383,26 +425,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
     uint8_t* vs = smem + kTcSlots * C::slot;
     TcShared& sh = *reinterpret_cast<TcShared*>(vs + kTcSlots * C::slot);
     const TreeArgs& a = p.a;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t r0 = blockIdx.x * kTcRows, split = blockIdx.y, g = blockIdx.z;
     const uint32_t tiles = (p.n + kTcKeys - 1) / kTcKeys;
     const uint32_t t0 = split * p.tiles_per_split, nt = min(tiles, t0 + p.tiles_per_split) - t0;
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kTcSlots; ++i) {
-            mbar_init(&sh.k_full[i], 8);
+            mbar_init(&sh.k_full[i], 4);
             mbar_init(&sh.k_empty[i], 1);
-            mbar_init(&sh.v_full[i], 8);
+            mbar_init(&sh.v_full[i], 4);
             mbar_init(&sh.v_empty[i], 1);
         }
         for (uint32_t b = 0; b < 2; ++b) {
             mbar_init(&sh.s_full[b], 2);   // the MMA's commit and the issuing thread
-            mbar_init(&sh.s_empty[b], 4);
             mbar_init(&sh.p_full[b], 4);
-            mbar_init(&sh.p_empty[b], 1);
+            mbar_init(&sh.o_full[b], 2);
+            mbar_init(&sh.o_empty[b], 8);
         }
-        mbar_init(&sh.o_full, 2);
-        mbar_init(&sh.o_empty, 8);
         mbar_init(&sh.q_full, 4);
         mbar_init(&sh.ml_full, 4);
         mbar_init(&sh.done, 1);
@@ -417,7 +457,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tm = sh.tmem;
+    const uint32_t tm = __shfl_sync(0xffffffffu, sh.tmem, 0);
     bool ok = true;
 
     if (warp < 4) {
@@ -430,6 +470,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
         const float4* q = reinterpret_cast<const float4*>(a.q + (size_t)tok * a.q_stride +
                                                           ((size_t)g * p.G + (valid ? r % p.G : 0)) * HD);
         uint32_t mb = 0;
+#pragma unroll 8
         for (int i = 0; i < HD / 4; ++i) {
             const float4 x = __ldg(q + i);
             mb = max(max(mb, __float_as_uint(x.x) & 0x7FFFFFFFu), __float_as_uint(x.y) & 0x7FFFFFFFu);
@@ -437,7 +478,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
         }
         float mult, qinv;
         tc_scale(mb, mult, qinv);
-        if (!valid) mult = 0.f;
 #pragma unroll 1
         for (int i = 0; i < HD / 16; ++i) {
             uint32_t hi[8], lo[8];
@@ -457,38 +497,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
         float m = -INFINITY, l = 0.f;
         float* sc = p.scores && valid ? p.scores + ((size_t)g * p.R + r) * p.sc_stride : nullptr;
         for (uint32_t t = 0; t < nt; ++t) {
-            const uint32_t b = t & 1, use = t >> 1, key0 = (t0 + t) * kTcKeys, ring = t % kTcRing;
-            ok = mbar_wait(&sh.s_full[b], use & 1);
+            const uint32_t b = t & 1, key0 = (t0 + t) * kTcKeys, ring = t % kTcRing;
+            // V's slot is not reused before this tile's P is read, so its phase can be waited for here
+            ok = mbar_wait(&sh.v_full[t % kTcSlots], (t / kTcSlots) & 1) && mbar_wait(&sh.s_full[b], (t >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
+            const uint32_t sp = lanes + C::s0 + b * kTcKeys;
             float s[kTcKeys];
             {
                 uint32_t x[32];
-                tmem_ld32(lanes + C::s0 + b * kTcKeys, x);
+                tmem_ld32(sp, x);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(x[i]);
-                tmem_ld32(lanes + C::s0 + b * kTcKeys + 32, x);
+                tmem_ld32(sp + 32, x);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) s[32 + i] = __uint_as_float(x[i]);
             }
             // (never 0: an unseen key's -inf times it stays -inf)
             const float raw = fmaxf(qinv * sh.k_scale[ring], 0x1p-120f);
-            const unsigned long long bad = sh.bad[ring];
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.s_empty[b]);
-            unsigned long long seen = ~0ull;
-            if (key0 + kTcKeys > a.n_past) {
-                seen = tc_seen(p, tok, key0);
+            const unsigned long long bad = sh.k_bad[ring] | sh.v_bad[ring];
+            if (key0 + kTcKeys > a.n_past || bad) {
+                const unsigned long long seen = tc_seen(a.mask, a.n_past, a.n_tokens, tok, key0);
 #pragma unroll
-                for (int i = 0; i < (int)kTcKeys; ++i)
+                for (int i = 0; i < (int)kTcKeys; ++i) {
                     if (!((seen >> i) & 1)) s[i] = -INFINITY;
-            }
-            if (bad & seen) {
-#pragma unroll
-                for (int i = 0; i < (int)kTcKeys; ++i)
-                    if ((bad & seen) >> i & 1) s[i] = __uint_as_float(0x7FC00000u);
+                    else if ((bad >> i) & 1) s[i] = __uint_as_float(0x7FC00000u);
+                }
             }
             if (sc) {
 #pragma unroll
@@ -496,24 +531,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
                     *reinterpret_cast<float4*>(sc + key0 + i) =
                         make_float4(s[i] * raw, s[i + 1] * raw, s[i + 2] * raw, s[i + 3] * raw);
             }
-            float mx = s[0];
+            float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 1; i < (int)kTcKeys; ++i) mx = fmaxf(mx, s[i]);
+            for (int i = 4; i < (int)kTcKeys; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const float ct = raw * p.c;
-            const float mn = fmaxf(m, mx == -INFINITY ? -INFINITY : ceilf(mx * ct));
+            const float mn = fmaxf(m, top == -INFINITY ? -INFINITY : ceilf(top * ct));
             const float ref = mn == -INFINITY ? 0.f : mn;
             const float corr = ex2_approx(m - ref);
             sh.corr[t % kTcCorr][rl] = corr;
             m = mn;
-            // P's buffer is free once the product two tiles back has read it
-            if (t >= 2) {
-                ok = mbar_wait(&sh.p_empty[b], (use - 1) & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
-            }
             const float off = kPShift - ref;
-            float sum = 0.f;
+            float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < (int)kTcKeys; i += 16) {
                 uint32_t hi[8], lo[8];
@@ -521,13 +550,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
                 for (int j = 0; j < 8; ++j) {
                     const float x = ex2_approx(fmaf(s[i + 2 * j], ct, off));
                     const float y = ex2_approx(fmaf(s[i + 2 * j + 1], ct, off));
-                    sum += x + y;
+                    sum[0] += x;
+                    sum[1] += y;
                     split_f16(x, y, hi[j], lo[j]);
                 }
-                tmem_st8(lanes + C::p0 + b * 64 + i / 2, hi);
-                tmem_st8(lanes + C::p0 + b * 64 + 32 + i / 2, lo);
+                tmem_st8(sp + i / 2, hi);
+                tmem_st8(sp + 32 + i / 2, lo);
             }
-            l = fmaf(l, corr, sum);
+            l = fmaf(l, corr, sum[0] + sum[1]);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -544,9 +574,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
 #pragma unroll
         for (int i = 0; i < OC; ++i) o[i] = 0.f;
         const uint32_t rl = (warp & 3) * 32 + lane, r = r0 + rl, col = warp < 8 ? 0 : OC;
-        const uint32_t src = tm + (((warp & 3) * 32u) << 16) + C::o + col;
+        const uint32_t src = tm + (((warp & 3) * 32u) << 16) + C::o0 + col;
         for (uint32_t t = 0; t < nt; ++t) {
-            ok = mbar_wait(&sh.o_full, t & 1);
+            const uint32_t b = t & 1;
+            ok = mbar_wait(&sh.o_full[b], (t >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
@@ -554,13 +585,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
 #pragma unroll
             for (int c = 0; c < OC; c += 16) {
                 uint32_t x[16];
-                tmem_ld16(src + c, x);
+                tmem_ld16(src + b * 128 + c, x);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[c + i] = fmaf(__uint_as_float(x[i]), scale, o[c + i] * corr);
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.o_empty);
+            if (lane == 0) mbar_arrive(&sh.o_empty[b]);
         }
         ok = mbar_wait(&sh.ml_full, 0) && ok;
         if (r < p.R) {
@@ -582,111 +613,76 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
                 *reinterpret_cast<float4*>(dst + i) =
                     make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
         }
+    } else if (warp < 16) {
+        ok = tc_convert<HD>(a.kcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, 0, (int)threadIdx.x - 384, ks,
+                            sh.k_full, sh.k_empty, sh.k_scale, sh.k_bad, sh.wmax[0]);
     } else if (warp < 20) {
-        // ---- converters
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
-        const int tid = (int)threadIdx.x - 384;
-        const uint32_t cw = warp - 12;
-        const float* kb = a.kcache + (size_t)g * a.max_ctx * HD;
-        const float* vb = a.vcache + (size_t)g * a.max_ctx * HD;
-        TcUnits<HD> ku, vu;
-        vu.load(vb, t0 * kTcKeys, p.n, tid);
-        ku.load(kb, t0 * kTcKeys, p.n, tid);
-        auto convert = [&](TcUnits<HD>& u, uint32_t t, int which, uint8_t* slots, uint64_t* full, uint64_t* empty,
-                           float* scales) -> bool {
-            const uint32_t slot = t % kTcSlots, use = t / kTcSlots, ring = t % kTcRing;
-            const uint32_t mw = __reduce_max_sync(0xffffffffu, u.max_bits());
-            if (lane == 0) sh.wmax[which][cw] = mw;
-            if (which == 0 && tid == 0) sh.bad[ring] = 0;
-            const bool stuck = use > 0 && !mbar_wait(&empty[slot], (use - 1) & 1);
-            if (conv_any(stuck)) return false;
-            uint32_t mx = 0;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) mx = max(mx, sh.wmax[which][w]);
-            if (mx >= 0x7F800000u) {  // the same for all 256 threads
-                u.clean(&sh.bad[ring], tid);
-                const uint32_t m2 = __reduce_max_sync(0xffffffffu, u.max_bits());
-                if (lane == 0) sh.wmax[2][cw] = m2;
-                conv_any(false);
-                mx = 0;
-#pragma unroll
-                for (int w = 0; w < 8; ++w) mx = max(mx, sh.wmax[2][w]);
-                conv_any(false);
-            }
-            float mult, inv;
-            tc_scale(mx, mult, inv);
-            u.store(slots + slot * C::slot, mult, tid);
-            if (tid == 0) scales[ring] = inv;
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[slot]);
-            return true;
-        };
-        for (uint32_t t = 0; t < nt; ++t) {
-            // V first: K's arrival then covers the marks of both
-            ok = convert(vu, t, 0, vs, sh.v_full, sh.v_empty, sh.v_scale);
-            if (!ok) break;
-            if (t + 1 < nt) vu.load(vb, (t0 + t + 1) * kTcKeys, p.n, tid);
-            ok = convert(ku, t, 1, ks, sh.k_full, sh.k_empty, sh.k_scale);
-            if (!ok) break;
-            if (t + 1 < nt) ku.load(kb, (t0 + t + 1) * kTcKeys, p.n, tid);
-        }
+        ok = tc_convert<HD>(a.vcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, 1, (int)threadIdx.x - 512, vs,
+                            sh.v_full, sh.v_empty, sh.v_scale, sh.v_bad, sh.wmax[1]);
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
-      if (warp == 20 && lane == 0) {
-        // ---- MMA issuer
-        ok = mbar_wait(&sh.q_full, 0);
-        tc_fence_after();
-        auto scores = [&](uint32_t t) -> bool {
-            const uint32_t slot = t % kTcSlots, b = t & 1;
-            if (!mbar_wait(&sh.k_full[slot], (t / kTcSlots) & 1)) return false;
-            if (t >= 2 && !mbar_wait(&sh.s_empty[b], ((t >> 1) - 1) & 1)) return false;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 20) {
+            // ---- MMA issuer: the whole warp walks the loop, one lane issues
+            uint32_t leader;
+            asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
+            auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+            ok = wait(&sh.q_full, 0);
             tc_fence_after();
-            const uint8_t* hi = ks + slot * C::slot;
-            const uint32_t d = tm + C::s0 + b * kTcKeys;
+            auto scores = [&](uint32_t t) -> bool {
+                const uint32_t slot = t % kTcSlots, b = t & 1;
+                if (!wait(&sh.k_full[slot], (t / kTcSlots) & 1)) return false;
+                tc_fence_after();
+                const uint64_t desc = smem_desc_sw128(ks + slot * C::slot);
+                const uint32_t d = tm + C::s0 + b * kTcKeys;
+                if (leader) {
 #pragma unroll
-            for (int x = 0; x < 3; ++x) {  // lo hi, hi lo, hi hi
+                    for (int x = 0; x < 3; ++x) {  // lo hi, hi lo, hi hi
 #pragma unroll
-                for (int j = 0; j < HD / 16; ++j)
-                    mma_f16_ta(d, tm + (x == 0 ? C::q_lo : C::q_hi) + 8 * j,
-                               smem_desc_sw128(hi + (x == 1 ? C::half : 0) + (j >> 2) * (kTcKeys * 128)) + 2 * (j & 3),
-                               C::idesc_s, (x | j) != 0);
+                        for (int j = 0; j < HD / 16; ++j)
+                            mma_f16_ta(d, tm + (x == 0 ? C::q_lo : C::q_hi) + 8 * j,
+                                       desc + (((x == 1 ? C::half : 0) + (j >> 2) * (kTcKeys * 128)) >> 4) + 2 * (j & 3),
+                                       C::idesc_s, (x | j) != 0);
+                    }
+                    mma_commit(&sh.k_empty[slot]);
+                    mma_commit(&sh.s_full[b]);
+                    mbar_arrive(&sh.s_full[b]);
+                }
+                __syncwarp();
+                return true;
+            };
+            ok = ok && scores(0);
+            for (uint32_t t = 0; ok && t < nt; ++t) {
+                // S(t + 1) goes where P(t - 1) was: its product was issued before
+                if (t + 1 < nt && !scores(t + 1)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t slot = t % kTcSlots, b = t & 1;
+                ok = wait(&sh.v_full[slot], (t / kTcSlots) & 1) && wait(&sh.p_full[b], (t >> 1) & 1) &&
+                     (t < 2 || wait(&sh.o_empty[b], ((t >> 1) - 1) & 1));
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t desc = smem_desc_sw128_mn(vs + slot * C::slot, kTcKeys * 128);
+                const uint32_t pa = tm + C::s0 + b * kTcKeys, d = tm + C::o0 + b * 128;
+                if (leader) {
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) {
+#pragma unroll
+                        for (int j = 0; j < (int)kTcKeys / 16; ++j)
+                            mma_f16_ta(d, pa + (x == 0 ? 32 : 0) + 8 * j,
+                                       desc + (((x == 1 ? C::half : 0) + j * 2048) >> 4), C::idesc_pv, (x | j) != 0);
+                    }
+                    mma_commit(&sh.v_empty[slot]);
+                    mma_commit(&sh.o_full[b]);
+                    mbar_arrive(&sh.o_full[b]);
+                }
+                __syncwarp();
             }
-            mma_commit(&sh.k_empty[slot]);
-            mma_commit(&sh.s_full[b]);
-            mbar_arrive(&sh.s_full[b]);
-            return true;
-        };
-        ok = ok && scores(0);
-        for (uint32_t t = 0; ok && t < nt; ++t) {
-            if (t + 1 < nt && !scores(t + 1)) {
-                ok = false;
-                break;
-            }
-            const uint32_t slot = t % kTcSlots, b = t & 1;
-            ok = mbar_wait(&sh.v_full[slot], (t / kTcSlots) & 1) && mbar_wait(&sh.p_full[b], (t >> 1) & 1) &&
-                 (t == 0 || mbar_wait(&sh.o_empty, (t - 1) & 1));
-            if (!ok) break;
-            tc_fence_after();
-            const uint8_t* hi = vs + slot * C::slot;
-            const uint32_t pa = tm + C::p0 + b * 64;
-#pragma unroll
-            for (int x = 0; x < 3; ++x) {
-#pragma unroll
-                for (int j = 0; j < (int)kTcKeys / 16; ++j)
-                    mma_f16_ta(tm + C::o, pa + (x == 0 ? 32 : 0) + 8 * j,
-                               smem_desc_sw128_mn(hi + (x == 1 ? C::half : 0) + j * 2048, kTcKeys * 128), C::idesc_pv,
-                               (x | j) != 0);
-            }
-            mma_commit(&sh.v_empty[slot]);
-            mma_commit(&sh.p_empty[b]);
-            mma_commit(&sh.o_full);
-            mbar_arrive(&sh.o_full);
+            // tensor memory is freed only after every MMA has completed
+            if (leader) mma_commit(&sh.done);
+            __syncwarp();
+            ok = mbar_wait(&sh.done, 0) && ok;
         }
-        // tensor memory is freed only after every MMA has completed
-        mma_commit(&sh.done);
-        ok = mbar_wait(&sh.done, 0) && ok;
-      }
     }
     if (!ok) atomicOr(p.err, kErrTreeWait);
     __syncwarp();
@@ -700,35 +696,54 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
 
 // ---- joining -------------------------------------------------------------------
 
-// Join the splits' partials: one warp per (KV head, row).
+// Join the splits' partials: a CTA per (KV head, row), its threads 4 columns of
+// every (threads * 4 / HD)-th split each, so that all loads are in flight at
+// once (one warp walking the splits took 13 to 57 us of dependent loads).
+constexpr int kMergeThreads = 256;
 template <int HD>
-__global__ void __launch_bounds__(128) smallm_tree_merge_kernel(const TreeParams p) {
-    constexpr int DV = HD / 32;
+__global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const TreeParams p) {
+    constexpr int L4 = HD / 4, PARTS = kMergeThreads / L4;
+    __shared__ float4 acc[PARTS][L4];
+    __shared__ float red[32], redl[32];
     const TreeArgs& a = p.a;
-    const int lane = threadIdx.x & 31;
-    const size_t rows = (size_t)a.n_kv * p.R, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = tid % L4, part = tid / L4;
+    const size_t rows = (size_t)a.n_kv * p.R, row = blockIdx.x;
+    pdl_wait();
     float M = -INFINITY;
-    for (uint32_t s = lane; s < p.n_split; s += 32) M = fmaxf(M, p.part_ml[s * rows + row].x);
+    for (uint32_t s = tid; s < p.n_split; s += kMergeThreads) M = fmaxf(M, p.part_ml[s * rows + row].x);
     M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f, O[DV];
+    if (lane == 0) red[warp] = M;
+    __syncthreads();
+    M = red[0];
 #pragma unroll
-    for (int d = 0; d < DV; ++d) O[d] = 0.f;
+    for (int w = 1; w < kMergeThreads / 32; ++w) M = fmaxf(M, red[w]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (uint32_t s = 0; s < p.n_split; ++s) {
+    for (uint32_t s = part; s < p.n_split; s += PARTS) {
         const float2 ml = p.part_ml[s * rows + row];
+        const float4 v = reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * HD)[c];
         const float f = exp2f(ml.x - ref);
         L = fmaf(f, ml.y, L);
+        O.x = fmaf(f, v.x, O.x), O.y = fmaf(f, v.y, O.y), O.z = fmaf(f, v.z, O.z), O.w = fmaf(f, v.w, O.w);
+    }
+    acc[part][c] = O;
+    if (c == 0) redl[part] = L;
+    __syncthreads();
+    if (part) return;
+    L = redl[0];
 #pragma unroll
-        for (int d = 0; d < DV; ++d) O[d] = fmaf(f, p.part_o[(s * rows + row) * HD + lane + 32 * d], O[d]);
+    for (int k = 1; k < PARTS; ++k) {
+        const float4 v = acc[k][c];
+        O.x += v.x, O.y += v.y, O.z += v.z, O.w += v.w;
+        L += redl[k];
     }
     const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
     const uint32_t g = (uint32_t)(row / p.R), r = (uint32_t)(row % p.R);
     float* o = a.out + (size_t)(r / p.G) * a.out_stride + ((size_t)g * p.G + r % p.G) * HD;
-#pragma unroll
-    for (int d = 0; d < DV; ++d) o[lane + 32 * d] = O[d] * inv;
-    if (lane == 0 && p.scores) p.stats[row] = make_float2(ref, inv);
+    reinterpret_cast<float4*>(o)[c] = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+    if (c == 0 && p.scores) p.stats[row] = make_float2(ref, inv);
 }
 
 // weights[g][k] += sum_r 2^(s c - mc_r) / sum_r, one thread per (KV head, key):
@@ -809,8 +824,10 @@ void launch_tree(const TreeParams& p, bool tc, cudaStream_t stream) {
     }
     SM_CUDA(cudaGetLastError());
     if (p.n_split > 1) {
-        smallm_tree_merge_kernel<HD><<<(uint32_t)(((size_t)p.a.n_kv * p.R + 3) / 4), 128, 0, stream>>>(p);
-        SM_CUDA(cudaGetLastError());
+        TreeParams pp = p;
+        void* args[] = {&pp};
+        launch_kernel_ex((const void*)smallm_tree_merge_kernel<HD>, dim3(p.a.n_kv * p.R), dim3(kMergeThreads), 0,
+                         stream, true, args);
     }
     if (p.a.weights) {
         smallm_tree_weights_kernel<<<dim3((p.n + 255) / 256, p.a.n_kv), 256, 0, stream>>>(p);
