@@ -229,11 +229,11 @@ __global__ void __launch_bounds__(kVecThreads, 2) smallm_tree_vec_kernel(const T
 // lo hi) leave out 2^-24 of the operands' size.  e brings the largest
 // magnitude of the tile (K, V) or row (q) to [2^14, 2^15), so an element loses
 // bits only below 2^-39 of that.  The small products are accumulated first.
-//   - warps 12..15 (K) and 16..19 (V) convert: a group holds the next tile in
+//   - warps 12..19 (K) and 20..27 (V) convert: a group holds the next tile in
 //     registers (32 KB in flight each), finds its exponent and writes hi and
 //     lo in the MMA's swizzled layout, three slots for each of K and V; the
 //     load of the tile after goes out as soon as a register is free;
-//   - warp 20 issues S = Q K^T (Q in tensor memory) and, a tile behind,
+//   - warp 28 issues S = Q K^T (Q in tensor memory) and, a tile behind,
 //     O = P V (P in tensor memory, over S's columns; V MN-major);
 //   - warps 0..3, lane = row: running maximum (a whole number in base 2, so
 //     rescaling is exact), P = 2^(s - m + 14) as hi and lo, sum;
@@ -244,9 +244,10 @@ __global__ void __launch_bounds__(kVecThreads, 2) smallm_tree_vec_kernel(const T
 // replaced by 0 and its key marked; rows that see the key turn to NaN.
 // Every wait is bounded; one that gives up raises bit 8 of the error word.
 constexpr uint32_t kTcRows = 128, kTcKeys = 64, kTcSlots = 3, kTcRing = 8, kTcCorr = 4;
-// six warpgroups; registers per thread 80 at launch (480 over the six), then
-// 104 softmax + 2 x 88 output + 2 x 80 converters + 40 issuer = 480
-constexpr uint32_t kTcThreads = 32 * 24;
+// eight warpgroups; registers per thread 64 at launch (512 over the eight), then
+// 88 softmax + 2 x 88 output + 4 x 56 converters + 24 issuer = 512
+constexpr uint32_t kTcThreads = 32 * 32;
+constexpr uint32_t kConvThreads = 256, kConvWarps = kConvThreads / 32;
 constexpr unsigned kErrTreeWait = 256u;
 constexpr float kPShift = 14.f;
 
@@ -268,7 +269,7 @@ struct TcShared {
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, ml_full, done;
     float k_scale[kTcRing], v_scale[kTcRing];
     unsigned long long k_bad[kTcRing], v_bad[kTcRing];
-    alignas(16) uint32_t wmax[2][2][4];
+    uint32_t wmax[2][2][kConvWarps];
     uint32_t tmem;
     float corr[kTcCorr][kTcRows];
     float2 ml[kTcRows];
@@ -281,18 +282,41 @@ __device__ __forceinline__ void tc_scale(uint32_t max_bits, float& mult, float& 
     mult = __uint_as_float(f << 23);
     inv = __uint_as_float((254u - f) << 23);
 }
-__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(a, b);
+// Two f32 operations in one instruction (each element rounded as by itself).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+          "l"(reinterpret_cast<const uint64_t&>(c)));
+    return r;
+}
+__device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __float22half2_rn(x);
     const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    const __half2 l = __float22half2_rn(fma2(f, make_float2(-1.f, -1.f), x));
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
-// Barrier of the 128 threads of converter group `id`; true where any says so.
+// Barrier of the 256 threads of converter group `id`; true where any says so.
 __device__ __forceinline__ bool conv_any(int id, bool v) {
     uint32_t r;
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 128, p;\n"
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 256, p;\n"
         " selp.u32 %0, 1, 0, q;\n}"
         : "=r"(r)
         : "r"((uint32_t)v), "r"(id)
@@ -309,13 +333,13 @@ __device__ __forceinline__ float max_abs_nan(float a, float b) {
     asm("{\n .reg .f32 t;\n abs.f32 t, %2;\n max.NaN.f32 %0, %1, t;\n}" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// A streaming load that stays where it is written (a plain one may sink to its use).
-__device__ __forceinline__ float4 load_stream(const float* p) {
-    float4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "l"(p));
-    return v;
+// A streaming load, if `go`, that stays where it is written (a plain one may
+// sink to its use).
+__device__ __forceinline__ void load_stream(float4& v, const float* p, bool go) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %5, 0;\n @q ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];\n}"
+        : "+f"(v.x), "+f"(v.y), "+f"(v.z), "+f"(v.w)
+        : "l"(p), "r"((uint32_t)go));
 }
 
 // Bits of the 64 keys from key0 that row token t sees.
@@ -341,20 +365,24 @@ __device__ __forceinline__ unsigned long long tc_seen(const uint32_t* mask, uint
 template <int HD>
 __device__ __forceinline__ bool tc_convert(const float* src, uint32_t n, uint32_t t0, uint32_t nt, int group, int tid,
                                            uint8_t* slots, uint64_t* full, uint64_t* empty, float* scales,
-                                           unsigned long long* bads, uint32_t (*wmax)[4]) {
+                                           unsigned long long* bads, uint32_t (*wmax)[kConvWarps]) {
     using C = TcTree<HD>;
-    constexpr int N = (int)kTcKeys * HD / 4 / 128;  // float4s of a thread
-    constexpr uint32_t W = HD / 4;                  // float4s of a row
-    const uint32_t c4 = tid % W, row0 = tid / W;    // row of unit i: row0 + i * (128 / W)
+    constexpr int N = (int)kTcKeys * HD / 4 / kConvThreads;  // float4s of a thread
+    constexpr uint32_t W = HD / 4, STEP = kConvThreads / W;  // float4s of a row; rows between two units
+    const uint32_t c4 = tid % W, row0 = tid / W;
     const float* p = src + (size_t)(t0 * kTcKeys + row0) * HD + 4 * c4;
-    uint32_t key = t0 * kTcKeys + row0;
+    // rows left from this thread's first row of the tile; a row past the last
+    // keeps the tile before's values, which are finite and get the weight 0
+    int64_t left = (int64_t)n - t0 * kTcKeys - row0;
     float4 x[N];
-    auto load = [&](int i) {
-        x[i] = key + i * (128 / W) < n ? load_stream(p + (size_t)i * (128 / W) * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
-    };
 #pragma unroll
-    for (int i = 0; i < N; ++i) load(i);
-    const uint32_t dst0 = (c4 >> 4) * (kTcKeys * 128) + (c4 & 1) * 8;
+    for (int i = 0; i < N; ++i) {
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        load_stream(x[i], p + (size_t)i * STEP * HD, (int)(i * STEP) < left);
+    }
+    // (STEP is a multiple of 8: the swizzle is the same for all units)
+    const uint32_t dst0 =
+        (c4 >> 4) * (kTcKeys * 128) + (c4 & 1) * 8 + row0 * 128 + ((((c4 & 15) >> 1) ^ (row0 & 7)) << 4);
     const int lane = tid & 31, cw = tid >> 5;
     for (uint32_t t = 0; t < nt; ++t) {
         const uint32_t slot = t % kTcSlots, use = t / kTcSlots, ring = t % kTcRing;
@@ -367,9 +395,10 @@ __device__ __forceinline__ bool tc_convert(const float* src, uint32_t n, uint32_
         if (tid == 0) bads[ring] = 0;
         const bool stuck = use > 0 && !mbar_wait(&empty[slot], (use - 1) & 1);
         if (conv_any(1 + group, stuck)) return false;
-        uint4 mx4 = *reinterpret_cast<const uint4*>(wmax[t & 1]);
-        uint32_t mx = max(max(mx4.x, mx4.y), max(mx4.z, mx4.w));
-        if (mx >= 0x7F800000u) {  // the same for all 128 threads: clean the tile
+        uint32_t mx = 0;
+#pragma unroll
+        for (int w = 0; w < (int)kConvWarps; ++w) mx = max(mx, wmax[t & 1][w]);
+        if (mx >= 0x7F800000u) {  // the same for the whole group: clean the tile
             m = 0.f;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -382,32 +411,32 @@ __device__ __forceinline__ bool tc_convert(const float* src, uint32_t n, uint32_
                     m = fmaxf(m, fabsf(v));
                 };
                 clean(x[i].x), clean(x[i].y), clean(x[i].z), clean(x[i].w);
-                if (any) atomicOr(&bads[ring], 1ull << (row0 + i * (128 / W)));
+                if (any) atomicOr(&bads[ring], 1ull << (row0 + i * STEP));
             }
             const uint32_t m2 = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
             conv_any(1 + group, false);  // wmax has been read by all
             if (lane == 0) wmax[t & 1][cw] = m2;
             conv_any(1 + group, false);
-            mx4 = *reinterpret_cast<const uint4*>(wmax[t & 1]);
-            mx = max(max(mx4.x, mx4.y), max(mx4.z, mx4.w));
+            mx = 0;
+#pragma unroll
+            for (int w = 0; w < (int)kConvWarps; ++w) mx = max(mx, wmax[t & 1][w]);
         }
         float mult, inv;
         tc_scale(mx, mult, inv);
         if (tid == 0) scales[ring] = inv;
         uint8_t* dst = slots + slot * C::slot + dst0;
-        key += kTcKeys;
         p += (size_t)kTcKeys * HD;
-        const bool more = t + 1 < nt;
+        left -= kTcKeys;
+        const int lim = t + 1 < nt ? (int)(left < (int64_t)kTcKeys ? left : (int64_t)kTcKeys) : 0;
+        const float2 mult2 = make_float2(mult, mult);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t row = row0 + i * (128 / W);
-            uint8_t* d = dst + row * 128 + ((((c4 & 15) >> 1) ^ (row & 7)) << 4);
             uint2 hi, lo;
-            split_f16(x[i].x * mult, x[i].y * mult, hi.x, lo.x);
-            split_f16(x[i].z * mult, x[i].w * mult, hi.y, lo.y);
-            *reinterpret_cast<uint2*>(d) = hi;
-            *reinterpret_cast<uint2*>(d + C::half) = lo;
-            if (more) load(i);
+            split_f16(mul2(make_float2(x[i].x, x[i].y), mult2), hi.x, lo.x);
+            split_f16(mul2(make_float2(x[i].z, x[i].w), mult2), hi.y, lo.y);
+            *reinterpret_cast<uint2*>(dst + i * STEP * 128) = hi;
+            *reinterpret_cast<uint2*>(dst + i * STEP * 128 + C::half) = lo;
+            load_stream(x[i], p + (size_t)i * STEP * HD, (int)(i * STEP) < lim);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -432,9 +461,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kTcSlots; ++i) {
-            mbar_init(&sh.k_full[i], 4);
+            mbar_init(&sh.k_full[i], kConvWarps);
             mbar_init(&sh.k_empty[i], 1);
-            mbar_init(&sh.v_full[i], 4);
+            mbar_init(&sh.v_full[i], kConvWarps);
             mbar_init(&sh.v_empty[i], 1);
         }
         for (uint32_t b = 0; b < 2; ++b) {
@@ -448,7 +477,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
         mbar_init(&sh.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 20) {
+    if (warp == 28) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                      "r"(512u)
                      : "memory");
@@ -462,33 +491,49 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
 
     if (warp < 4) {
         // ---- softmax: lane = row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
         const uint32_t rl = threadIdx.x, r = r0 + rl;
         const uint32_t lanes = tm + ((warp * 32u) << 16);
         const bool valid = r < p.R;
         const uint32_t tok = valid ? r / p.G : 0;
         const float4* q = reinterpret_cast<const float4*>(a.q + (size_t)tok * a.q_stride +
                                                           ((size_t)g * p.G + (valid ? r % p.G : 0)) * HD);
+        // largest magnitude of each row: the warp reads a row at a time
         uint32_t mb = 0;
+        constexpr int QL = HD / 32;
 #pragma unroll 8
-        for (int i = 0; i < HD / 4; ++i) {
-            const float4 x = __ldg(q + i);
-            mb = max(max(mb, __float_as_uint(x.x) & 0x7FFFFFFFu), __float_as_uint(x.y) & 0x7FFFFFFFu);
-            mb = max(max(mb, __float_as_uint(x.z) & 0x7FFFFFFFu), __float_as_uint(x.w) & 0x7FFFFFFFu);
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t ri = min(r0 + warp * 32 + i, p.R - 1);
+            const float* qi = a.q + (size_t)(ri / p.G) * a.q_stride + ((size_t)g * p.G + ri % p.G) * HD + lane * QL;
+            float x[QL];
+            if constexpr (QL == 4) *reinterpret_cast<float4*>(x) = __ldg(reinterpret_cast<const float4*>(qi));
+            else if constexpr (QL == 2) *reinterpret_cast<float2*>(x) = __ldg(reinterpret_cast<const float2*>(qi));
+            else x[0] = __ldg(qi);
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < QL; ++j) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+            m = __reduce_max_sync(0xffffffffu, m);
+            if (lane == i) mb = m;
         }
         float mult, qinv;
         tc_scale(mb, mult, qinv);
+        const float2 mult2 = make_float2(mult, mult);
 #pragma unroll 1
-        for (int i = 0; i < HD / 16; ++i) {
-            uint32_t hi[8], lo[8];
+        for (int i = 0; i < HD / 32; ++i) {
+            float4 x[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4 x = valid ? __ldg(q + 4 * i + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                split_f16(x.x * mult, x.y * mult, hi[2 * j], lo[2 * j]);
-                split_f16(x.z * mult, x.w * mult, hi[2 * j + 1], lo[2 * j + 1]);
+            for (int j = 0; j < 8; ++j) x[j] = valid ? __ldg(q + 8 * i + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    split_f16(mul2(make_float2(x[j + u].x, x[j + u].y), mult2), hi[2 * u], lo[2 * u]);
+                    split_f16(mul2(make_float2(x[j + u].z, x[j + u].w), mult2), hi[2 * u + 1], lo[2 * u + 1]);
+                }
+                tmem_st8(lanes + C::q_hi + 16 * i + 2 * j, hi);
+                tmem_st8(lanes + C::q_lo + 16 * i + 2 * j, lo);
             }
-            tmem_st8(lanes + C::q_hi + 8 * i, hi);
-            tmem_st8(lanes + C::q_lo + 8 * i, lo);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -498,8 +543,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
         float* sc = p.scores && valid ? p.scores + ((size_t)g * p.R + r) * p.sc_stride : nullptr;
         for (uint32_t t = 0; t < nt; ++t) {
             const uint32_t b = t & 1, key0 = (t0 + t) * kTcKeys, ring = t % kTcRing;
-            // V's slot is not reused before this tile's P is read, so its phase can be waited for here
-            ok = mbar_wait(&sh.v_full[t % kTcSlots], (t / kTcSlots) & 1) && mbar_wait(&sh.s_full[b], (t >> 1) & 1);
+            ok = mbar_wait(&sh.s_full[b], (t >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
@@ -516,7 +560,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
             }
             // (never 0: an unseen key's -inf times it stays -inf)
             const float raw = fmaxf(qinv * sh.k_scale[ring], 0x1p-120f);
-            const unsigned long long bad = sh.k_bad[ring] | sh.v_bad[ring];
+            const unsigned long long bad = sh.k_bad[ring];
             if (key0 + kTcKeys > a.n_past || bad) {
                 const unsigned long long seen = tc_seen(a.mask, a.n_past, a.n_tokens, tok, key0);
 #pragma unroll
@@ -542,22 +586,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
             sh.corr[t % kTcCorr][rl] = corr;
             m = mn;
             const float off = kPShift - ref;
-            float sum[2] = {0.f, 0.f};
+            float2 sum = make_float2(0.f, 0.f);
+            const float2 ct2 = make_float2(ct, ct), off2 = make_float2(off, off);
 #pragma unroll
             for (int i = 0; i < (int)kTcKeys; i += 16) {
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float x = ex2_approx(fmaf(s[i + 2 * j], ct, off));
-                    const float y = ex2_approx(fmaf(s[i + 2 * j + 1], ct, off));
-                    sum[0] += x;
-                    sum[1] += y;
-                    split_f16(x, y, hi[j], lo[j]);
+                    float2 e = fma2(make_float2(s[i + 2 * j], s[i + 2 * j + 1]), ct2, off2);
+                    e.x = ex2_approx(e.x);
+                    e.y = ex2_approx(e.y);
+                    sum = add2(sum, e);
+                    split_f16(e, hi[j], lo[j]);
                 }
                 tmem_st8(sp + i / 2, hi);
                 tmem_st8(sp + 32 + i / 2, lo);
             }
-            l = fmaf(l, corr, sum[0] + sum[1]);
+            l = fmaf(l, corr, sum.x + sum.y);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -570,9 +615,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
         // ---- output: lane = row, warps 4..7 the first half of the columns, 8..11 the second
         asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
         constexpr int OC = HD / 2;
-        float o[OC];
+        float2 o[OC / 2];
 #pragma unroll
-        for (int i = 0; i < OC; ++i) o[i] = 0.f;
+        for (int i = 0; i < OC / 2; ++i) o[i] = make_float2(0.f, 0.f);
         const uint32_t rl = (warp & 3) * 32 + lane, r = r0 + rl, col = warp < 8 ? 0 : OC;
         const uint32_t src = tm + (((warp & 3) * 32u) << 16) + C::o0 + col;
         for (uint32_t t = 0; t < nt; ++t) {
@@ -582,12 +627,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
             if (!ok) break;
             tc_fence_after();
             const float corr = sh.corr[t % kTcCorr][rl], scale = sh.v_scale[t % kTcRing] * 0x1p-14f;
+            const float2 corr2 = make_float2(corr, corr), scale2 = make_float2(scale, scale);
 #pragma unroll
             for (int c = 0; c < OC; c += 16) {
                 uint32_t x[16];
                 tmem_ld16(src + b * 128 + c, x);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[c + i] = fmaf(__uint_as_float(x[i]), scale, o[c + i] * corr);
+                for (int i = 0; i < 8; ++i)
+                    o[c / 2 + i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2,
+                                        mul2(o[c / 2 + i], corr2));
+            }
+            const unsigned long long bad = sh.v_bad[t % kTcRing];
+            if (bad && r < p.R && (bad & tc_seen(a.mask, a.n_past, a.n_tokens, r / p.G, (t0 + t) * kTcKeys))) {
+#pragma unroll
+                for (int i = 0; i < OC / 2; ++i)
+                    o[i] = make_float2(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
             }
             tc_fence_before();
             __syncwarp();
@@ -611,17 +665,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
 #pragma unroll
             for (int i = 0; i < OC; i += 4)
                 *reinterpret_cast<float4*>(dst + i) =
-                    make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+                    make_float4(o[i / 2].x * f, o[i / 2].y * f, o[i / 2 + 1].x * f, o[i / 2 + 1].y * f);
         }
-    } else if (warp < 16) {
+    } else if (warp < 20) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         ok = tc_convert<HD>(a.kcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, 0, (int)threadIdx.x - 384, ks,
                             sh.k_full, sh.k_empty, sh.k_scale, sh.k_bad, sh.wmax[0]);
-    } else if (warp < 20) {
-        ok = tc_convert<HD>(a.vcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, 1, (int)threadIdx.x - 512, vs,
+    } else if (warp < 28) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        ok = tc_convert<HD>(a.vcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, 1, (int)threadIdx.x - 640, vs,
                             sh.v_full, sh.v_empty, sh.v_scale, sh.v_bad, sh.wmax[1]);
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 20) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+        if (warp == 28) {
             // ---- MMA issuer: the whole warp walks the loop, one lane issues
             uint32_t leader;
             asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
@@ -688,7 +744,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 20) {
+    if (warp == 28) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u) : "memory");
     }
