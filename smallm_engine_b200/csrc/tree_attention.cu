@@ -229,24 +229,29 @@ __global__ void __launch_bounds__(kVecThreads, 2) smallm_tree_vec_kernel(const T
 // lo hi) leave out 2^-24 of the operands' size.  e brings the largest
 // magnitude of the tile (K, V) or row (q) to [2^14, 2^15), so an element loses
 // bits only below 2^-39 of that.  The small products are accumulated first.
-//   - warps 12..19 (K) and 20..27 (V) convert: a group holds the next tile in
-//     registers (32 KB in flight each), finds its exponent and writes hi and
-//     lo in the MMA's swizzled layout, three slots for each of K and V; the
-//     load of the tile after goes out as soon as a register is free;
-//   - warp 28 issues S = Q K^T (Q in tensor memory) and, a tile behind,
+//   - warps 25 (K) and 26 (V) copy f32 rows with bulk copies, half a tile at a
+//     time, into two halves each: 64 KB in flight while the tile before is
+//     converted.  (Loads through registers took the load/store unit twice as
+//     long as these copies and the reads of them, and 135 us where this form
+//     takes %TC_US% for 64 tokens x 32 heads over 32683 rows.)
+//   - warps 8..15 (K) and 16..23 (V) convert: a group takes a tile into
+//     registers, finds its exponent and writes hi and lo in the MMA's swizzled
+//     layout, two slots for each of K and V;
+//   - warp 24 issues S = Q K^T (Q in tensor memory) and, a tile behind,
 //     O = P V (P in tensor memory, over S's columns; V MN-major);
-//   - warps 0..3, lane = row: running maximum (a whole number in base 2, so
-//     rescaling is exact), P = 2^(s - m + 14) as hi and lo, sum;
-//   - warps 4..11, lane = row: O of each tile leaves tensor memory and is added
-//     to f32 registers with the tile's exponent and the row's rescaling, which
-//     keeps the long sum in rounded f32 adds.
+//   - warps 0..7, lane = row, two warps for a row: each takes half of the keys
+//     for the running maximum (a whole number in base 2, so rescaling is
+//     exact; the halves meet in shared memory), P = 2^(s - m + 14) as hi and lo
+//     and the sum, and half of the columns of the tile before's O, which it
+//     adds to f32 registers with that tile's exponent and the row's rescaling:
+//     the long sum is made of rounded f32 adds.
 // An infinity or NaN of K or V would reach every row through 0 * inf, so it is
 // replaced by 0 and its key marked; rows that see the key turn to NaN.
 // Every wait is bounded; one that gives up raises bit 8 of the error word.
-constexpr uint32_t kTcRows = 128, kTcKeys = 64, kTcSlots = 3, kTcRing = 8, kTcCorr = 4;
-// eight warpgroups; registers per thread 64 at launch (512 over the eight), then
-// 88 softmax + 2 x 88 output + 4 x 56 converters + 24 issuer = 512
-constexpr uint32_t kTcThreads = 32 * 32;
+constexpr uint32_t kTcRows = 128, kTcKeys = 64, kTcSlots = 2, kTcRing = 8;
+// seven warpgroups; registers per thread 72 at launch (504 over the seven), then
+// 2 x 128 rows + 4 x 56 converters + 24 issuer = 504
+constexpr uint32_t kTcThreads = 32 * 28;
 constexpr uint32_t kConvThreads = 256, kConvWarps = kConvThreads / 32;
 constexpr unsigned kErrTreeWait = 256u;
 constexpr float kPShift = 14.f;
@@ -256,7 +261,9 @@ struct TcTree {
     static constexpr uint32_t chunks = HD < 64 ? 1 : HD / 64;   // 128-byte columns of a tile
     static constexpr uint32_t half = chunks * kTcKeys * 128;    // bytes of a tile's hi or lo
     static constexpr uint32_t slot = 2 * half;
-    static constexpr size_t smem = 1024 + 2ull * kTcSlots * slot + 8192;
+    static constexpr uint32_t raw = kTcKeys / 2 * HD * 4;       // bytes of half a tile in f32
+    static constexpr size_t smem = 1024 + 2ull * kTcSlots * slot + 4ull * raw + 8192;
+    static_assert(kTcRows * HD * 4 <= kTcSlots * slot, "q and the output pass through the slots");
     static constexpr uint32_t pv_n = HD < 64 ? 64 : HD;         // columns past HD are never read
     // tensor-memory columns; P (hi 32, lo 32) takes the place of its S
     static constexpr uint32_t q_hi = 0, q_lo = 64, s0 = 128, o0 = 256;
@@ -266,13 +273,15 @@ struct TcTree {
 
 struct TcShared {
     uint64_t k_full[kTcSlots], k_empty[kTcSlots], v_full[kTcSlots], v_empty[kTcSlots];
-    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, ml_full, done;
+    uint64_t raw_full[2][2], raw_empty[2][2];  // [K, V][half]
+    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, done;
     float k_scale[kTcRing], v_scale[kTcRing];
     unsigned long long k_bad[kTcRing], v_bad[kTcRing];
     uint32_t wmax[2][2][kConvWarps];
     uint32_t tmem;
-    float corr[kTcCorr][kTcRows];
-    float2 ml[kTcRows];
+    float part_max[2][2][kTcRows];  // [tile % 2][half]
+    float part_sum[2][kTcRows];
+    uint32_t q_max[kTcRows];
 };
 static_assert(sizeof(TcShared) <= 8192, "shared-memory tail");
 
@@ -333,15 +342,6 @@ __device__ __forceinline__ float max_abs_nan(float a, float b) {
     asm("{\n .reg .f32 t;\n abs.f32 t, %2;\n max.NaN.f32 %0, %1, t;\n}" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// A streaming load, if `go`, that stays where it is written (a plain one may
-// sink to its use).
-__device__ __forceinline__ void load_stream(float4& v, const float* p, bool go) {
-    asm volatile(
-        "{\n .reg .pred q;\n setp.ne.u32 q, %5, 0;\n @q ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];\n}"
-        : "+f"(v.x), "+f"(v.y), "+f"(v.z), "+f"(v.w)
-        : "l"(p), "r"((uint32_t)go));
-}
-
 // Bits of the 64 keys from key0 that row token t sees.
 __device__ __forceinline__ unsigned long long tc_seen(const uint32_t* mask, uint32_t n_past, uint32_t n_tokens,
                                                    uint32_t t, uint32_t key0) {
@@ -361,73 +361,102 @@ __device__ __forceinline__ unsigned long long tc_seen(const uint32_t* mask, uint
     return m;
 }
 
-// One converter group: tiles t0 .. t0 + nt - 1 of `src` into `slots`.
+// One lane: tiles t0 .. t0 + nt - 1 of `src` (rows below n) into the two raw halves.
 template <int HD>
-__device__ __forceinline__ bool tc_convert(const float* src, uint32_t n, uint32_t t0, uint32_t nt, int group, int tid,
-                                           uint8_t* slots, uint64_t* full, uint64_t* empty, float* scales,
-                                           unsigned long long* bads, uint32_t (*wmax)[kConvWarps]) {
+__device__ __forceinline__ bool tc_copy(const float* src, uint32_t n, uint32_t t0, uint32_t nt, uint8_t* raw,
+                                        uint64_t* full, uint64_t* empty) {
     using C = TcTree<HD>;
-    constexpr int N = (int)kTcKeys * HD / 4 / kConvThreads;  // float4s of a thread
+    bool ok = true;
+    uint32_t last[2] = {0, 0};
+    for (uint32_t i = 0; ok && i < 2 * nt; ++i) {
+        const uint32_t t = i >> 1, h = i & 1, row = (t0 + t) * kTcKeys + h * (kTcKeys / 2);
+        ok = t == 0 || mbar_wait(&empty[h], (t - 1) & 1);
+        if (!ok) break;
+        const uint32_t rows = row < n ? min(n - row, kTcKeys / 2) : 0;
+        if (rows) {
+            mbar_arrive_expect_tx(&full[h], rows * HD * 4);
+            bulk_g2s(raw + h * C::raw, src + (size_t)row * HD, rows * HD * 4, &full[h]);
+        } else {
+            mbar_arrive(&full[h]);
+        }
+        last[h] = t + 1;
+    }
+    // no copy may still be landing when the CTA exits
+    for (uint32_t h = 0; h < 2; ++h)
+        if (last[h]) ok = mbar_wait(&full[h], (last[h] - 1) & 1) && ok;
+    return ok;
+}
+
+// One converter group: tiles t0 .. t0 + nt - 1 from the raw halves into `slots`.
+template <int HD, int GROUP>
+__device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt, int tid, uint8_t* smem, TcShared& sh) {
+    using C = TcTree<HD>;
+    constexpr int N = (int)kTcKeys * HD / 4 / kConvThreads;  // float4s of a thread, N / 2 from each half
     constexpr uint32_t W = HD / 4, STEP = kConvThreads / W;  // float4s of a row; rows between two units
     const uint32_t c4 = tid % W, row0 = tid / W;
-    const float* p = src + (size_t)(t0 * kTcKeys + row0) * HD + 4 * c4;
-    // rows left from this thread's first row of the tile; a row past the last
-    // keeps the tile before's values, which are finite and get the weight 0
-    int64_t left = (int64_t)n - t0 * kTcKeys - row0;
+    const float4* src = reinterpret_cast<const float4*>(smem + 2 * kTcSlots * C::slot + GROUP * 2 * C::raw) + tid;
+    uint8_t* slots = smem + GROUP * kTcSlots * C::slot;
+    uint64_t* full = GROUP ? sh.v_full : sh.k_full;
+    uint64_t* empty = GROUP ? sh.v_empty : sh.k_empty;
+    unsigned long long* bads = GROUP ? sh.v_bad : sh.k_bad;
+    auto& wmax = sh.wmax[GROUP];
     float4 x[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        load_stream(x[i], p + (size_t)i * STEP * HD, (int)(i * STEP) < left);
-    }
     // (STEP is a multiple of 8: the swizzle is the same for all units)
     const uint32_t dst0 =
         (c4 >> 4) * (kTcKeys * 128) + (c4 & 1) * 8 + row0 * 128 + ((((c4 & 15) >> 1) ^ (row0 & 7)) << 4);
     const int lane = tid & 31, cw = tid >> 5;
     for (uint32_t t = 0; t < nt; ++t) {
         const uint32_t slot = t % kTcSlots, use = t / kTcSlots, ring = t % kTcRing;
+        const uint32_t left = n - (t0 + t) * kTcKeys;  // rows from the tile's first to the last
+        bool stuck = false;
         float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            m = max_abs_nan(max_abs_nan(max_abs_nan(max_abs_nan(m, x[i].x), x[i].y), x[i].z), x[i].w);
+        for (int h = 0; h < 2; ++h) {
+            stuck = stuck || !mbar_wait(&sh.raw_full[GROUP][h], t & 1);
+#pragma unroll
+            for (int i = h * N / 2; i < (h + 1) * N / 2; ++i) {
+                x[i] = src[i * kConvThreads];
+                if (left < kTcKeys && row0 + i * STEP >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                m = max_abs_nan(max_abs_nan(max_abs_nan(max_abs_nan(m, x[i].x), x[i].y), x[i].z), x[i].w);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.raw_empty[GROUP][h]);
+        }
         const uint32_t mw = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
         if (lane == 0) wmax[t & 1][cw] = mw;
         if (tid == 0) bads[ring] = 0;
-        const bool stuck = use > 0 && !mbar_wait(&empty[slot], (use - 1) & 1);
-        if (conv_any(1 + group, stuck)) return false;
+        // (V's slots hold q until it is in tensor memory)
+        if (use > 0) stuck = stuck || !mbar_wait(&empty[slot], (use - 1) & 1);
+        else if (GROUP == 1 && t == 0) stuck = stuck || !mbar_wait(&sh.q_full, 0);
+        if (conv_any(1 + GROUP, stuck)) return false;
         uint32_t mx = 0;
 #pragma unroll
         for (int w = 0; w < (int)kConvWarps; ++w) mx = max(mx, wmax[t & 1][w]);
         if (mx >= 0x7F800000u) {  // the same for the whole group: clean the tile
             m = 0.f;
+            uint32_t hurt = 0;  // this thread's units that held any
+            auto clean = [&](float& v, int i) {
+                if (!(fabsf(v) < INFINITY)) {
+                    v = 0.f;
+                    hurt |= 1u << i;
+                }
+                m = fmaxf(m, fabsf(v));
+            };
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                bool any = false;
-                auto clean = [&](float& v) {
-                    if ((__float_as_uint(v) & 0x7FFFFFFFu) >= 0x7F800000u) {
-                        v = 0.f;
-                        any = true;
-                    }
-                    m = fmaxf(m, fabsf(v));
-                };
-                clean(x[i].x), clean(x[i].y), clean(x[i].z), clean(x[i].w);
-                if (any) atomicOr(&bads[ring], 1ull << (row0 + i * STEP));
-            }
+            for (int i = 0; i < N; ++i) clean(x[i].x, i), clean(x[i].y, i), clean(x[i].z, i), clean(x[i].w, i);
+            for (; hurt; hurt &= hurt - 1) atomicOr(&bads[ring], 1ull << (row0 + (__ffs(hurt) - 1) * STEP));
             const uint32_t m2 = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-            conv_any(1 + group, false);  // wmax has been read by all
+            conv_any(1 + GROUP, false);  // wmax has been read by all
             if (lane == 0) wmax[t & 1][cw] = m2;
-            conv_any(1 + group, false);
+            conv_any(1 + GROUP, false);
             mx = 0;
 #pragma unroll
             for (int w = 0; w < (int)kConvWarps; ++w) mx = max(mx, wmax[t & 1][w]);
         }
         float mult, inv;
         tc_scale(mx, mult, inv);
-        if (tid == 0) scales[ring] = inv;
+        if (tid == 0) (GROUP ? sh.v_scale : sh.k_scale)[ring] = inv;
         uint8_t* dst = slots + slot * C::slot + dst0;
-        p += (size_t)kTcKeys * HD;
-        left -= kTcKeys;
-        const int lim = t + 1 < nt ? (int)(left < (int64_t)kTcKeys ? left : (int64_t)kTcKeys) : 0;
         const float2 mult2 = make_float2(mult, mult);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -436,7 +465,6 @@ __device__ __forceinline__ bool tc_convert(const float* src, uint32_t n, uint32_
             split_f16(mul2(make_float2(x[i].z, x[i].w), mult2), hi.y, lo.y);
             *reinterpret_cast<uint2*>(dst + i * STEP * 128) = hi;
             *reinterpret_cast<uint2*>(dst + i * STEP * 128 + C::half) = lo;
-            load_stream(x[i], p + (size_t)i * STEP * HD, (int)(i * STEP) < lim);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -452,7 +480,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* ks = smem;
     uint8_t* vs = smem + kTcSlots * C::slot;
-    TcShared& sh = *reinterpret_cast<TcShared*>(vs + kTcSlots * C::slot);
+    uint8_t* raw = vs + kTcSlots * C::slot;  // K's two halves, then V's
+    TcShared& sh = *reinterpret_cast<TcShared*>(raw + 4 * C::raw);
     const TreeArgs& a = p.a;
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t r0 = blockIdx.x * kTcRows, split = blockIdx.y, g = blockIdx.z;
@@ -466,18 +495,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
             mbar_init(&sh.v_full[i], kConvWarps);
             mbar_init(&sh.v_empty[i], 1);
         }
+        for (uint32_t i = 0; i < 4; ++i) {
+            mbar_init(&sh.raw_full[i >> 1][i & 1], 1);
+            mbar_init(&sh.raw_empty[i >> 1][i & 1], kConvWarps);
+        }
         for (uint32_t b = 0; b < 2; ++b) {
             mbar_init(&sh.s_full[b], 2);   // the MMA's commit and the issuing thread
-            mbar_init(&sh.p_full[b], 4);
+            mbar_init(&sh.p_full[b], 8);
             mbar_init(&sh.o_full[b], 2);
             mbar_init(&sh.o_empty[b], 8);
         }
-        mbar_init(&sh.q_full, 4);
-        mbar_init(&sh.ml_full, 4);
+        mbar_init(&sh.q_full, 8);
         mbar_init(&sh.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 28) {
+    if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                      "r"(512u)
                      : "memory");
@@ -489,107 +521,157 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
     const uint32_t tm = __shfl_sync(0xffffffffu, sh.tmem, 0);
     bool ok = true;
 
-    if (warp < 4) {
-        // ---- softmax: lane = row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
-        const uint32_t rl = threadIdx.x, r = r0 + rl;
-        const uint32_t lanes = tm + ((warp * 32u) << 16);
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        constexpr int OC = HD / 2, SC = (int)kTcKeys / 2;  // this thread's columns of O and of S
+        const uint32_t quad = warp & 3, half = warp >> 2;
+        const uint32_t rl = quad * 32 + lane, r = r0 + rl;
+        const uint32_t lanes = tm + ((quad * 32u) << 16);
         const bool valid = r < p.R;
         const uint32_t tok = valid ? r / p.G : 0;
-        const float4* q = reinterpret_cast<const float4*>(a.q + (size_t)tok * a.q_stride +
-                                                          ((size_t)g * p.G + (valid ? r % p.G : 0)) * HD);
-        // largest magnitude of each row: the warp reads a row at a time
-        uint32_t mb = 0;
-        constexpr int QL = HD / 32;
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) {
-            const uint32_t ri = min(r0 + warp * 32 + i, p.R - 1);
-            const float* qi = a.q + (size_t)(ri / p.G) * a.q_stride + ((size_t)g * p.G + ri % p.G) * HD + lane * QL;
-            float x[QL];
-            if constexpr (QL == 4) *reinterpret_cast<float4*>(x) = __ldg(reinterpret_cast<const float4*>(qi));
-            else if constexpr (QL == 2) *reinterpret_cast<float2*>(x) = __ldg(reinterpret_cast<const float2*>(qi));
-            else x[0] = __ldg(qi);
-            uint32_t m = 0;
-#pragma unroll
-            for (int j = 0; j < QL; ++j) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-            m = __reduce_max_sync(0xffffffffu, m);
-            if (lane == i) mb = m;
-        }
-        float mult, qinv;
-        tc_scale(mb, mult, qinv);
-        const float2 mult2 = make_float2(mult, mult);
+        {
+            // q: the eight warps read 16 rows each, and their largest magnitudes,
+            // into V's slots; then each row is scaled and split by its two threads
+            constexpr int QL = HD / 32;
+            float* stage = reinterpret_cast<float*>(vs);
+            uint32_t tt = (r0 + warp * 16) / p.G, hh = (r0 + warp * 16) % p.G;
 #pragma unroll 1
-        for (int i = 0; i < HD / 32; ++i) {
-            float4 x[8];
+            for (uint32_t b = warp * 16; b < warp * 16 + 16; b += 8) {
+                alignas(16) float x[8][QL];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = valid ? __ldg(q + 8 * i + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = 0; i < 8; ++i) {
+                    const float* qi = a.q + (size_t)tt * a.q_stride + ((size_t)g * p.G + hh) * HD + lane * QL;
 #pragma unroll
-            for (int j = 0; j < 8; j += 4) {
+                    for (int j = 0; j < QL; ++j) x[i][j] = 0.f;
+                    if (r0 + b + i < p.R) {
+                        if constexpr (QL == 4) *reinterpret_cast<float4*>(x[i]) = __ldg(reinterpret_cast<const float4*>(qi));
+                        else if constexpr (QL == 2) *reinterpret_cast<float2*>(x[i]) = __ldg(reinterpret_cast<const float2*>(qi));
+                        else x[i][0] = __ldg(qi);
+                    }
+                    if (++hh == p.G) hh = 0, ++tt;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int j = 0; j < QL; ++j) m = max(m, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+                    // (16-byte units of a row permuted by the row: no bank conflicts either way)
+                    float* at = stage + (b + i) * HD + (((lane * QL >> 2) ^ (i & 7)) << 2) + (lane * QL & 3);
+                    if constexpr (QL == 4) *reinterpret_cast<float4*>(at) = *reinterpret_cast<const float4*>(x[i]);
+                    else if constexpr (QL == 2) *reinterpret_cast<float2*>(at) = *reinterpret_cast<const float2*>(x[i]);
+                    else *at = x[i][0];
+                    m = __reduce_max_sync(0xffffffffu, m);
+                    if (lane == 0) sh.q_max[b + i] = m;
+                }
+            }
+        }
+        asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
+        float qinv;
+        {
+            const float4* src = reinterpret_cast<const float4*>(vs) + rl * (HD / 4);
+            float mult;
+            tc_scale(sh.q_max[rl], mult, qinv);
+            const float2 mult2 = make_float2(mult, mult);
+#pragma unroll
+            for (int i = 0; i < HD / 8; i += 4) {
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    split_f16(mul2(make_float2(x[j + u].x, x[j + u].y), mult2), hi[2 * u], lo[2 * u]);
-                    split_f16(mul2(make_float2(x[j + u].z, x[j + u].w), mult2), hi[2 * u + 1], lo[2 * u + 1]);
+                    const float4 x = src[(half * (HD / 8) + i + u) ^ (rl & 7)];
+                    split_f16(mul2(make_float2(x.x, x.y), mult2), hi[2 * u], lo[2 * u]);
+                    split_f16(mul2(make_float2(x.z, x.w), mult2), hi[2 * u + 1], lo[2 * u + 1]);
                 }
-                tmem_st8(lanes + C::q_hi + 16 * i + 2 * j, hi);
-                tmem_st8(lanes + C::q_lo + 16 * i + 2 * j, lo);
+                tmem_st8(lanes + C::q_hi + half * (HD / 4) + 2 * i, hi);
+                tmem_st8(lanes + C::q_lo + half * (HD / 4) + 2 * i, lo);
             }
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full);
-        float m = -INFINITY, l = 0.f;
-        float* sc = p.scores && valid ? p.scores + ((size_t)g * p.R + r) * p.sc_stride : nullptr;
+
+        float2 o[OC / 2];
+#pragma unroll
+        for (int i = 0; i < OC / 2; ++i) o[i] = make_float2(0.f, 0.f);
+        float m = -INFINITY, l = 0.f, corr = 1.f;
+        float* sc = p.scores && valid ? p.scores + ((size_t)g * p.R + r) * p.sc_stride + half * SC : nullptr;
+        // o = o * corr + O of tile t
+        auto take_output = [&](uint32_t t) {
+            const uint32_t b = t & 1;
+            ok = ok && mbar_wait(&sh.o_full[b], (t >> 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            const float scale = sh.v_scale[t % kTcRing] * 0x1p-14f;
+            const float2 corr2 = make_float2(corr, corr), scale2 = make_float2(scale, scale);
+#pragma unroll
+            for (int c = 0; c < OC; c += 16) {
+                uint32_t x[16];
+                tmem_ld16(lanes + C::o0 + b * 128 + half * OC + c, x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    o[c / 2 + i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2,
+                                        mul2(o[c / 2 + i], corr2));
+            }
+            const unsigned long long bad = sh.v_bad[t % kTcRing];
+            if (bad && valid && (bad & tc_seen(a.mask, a.n_past, a.n_tokens, tok, (t0 + t) * kTcKeys))) {
+#pragma unroll
+                for (int i = 0; i < OC / 2; ++i)
+                    o[i] = make_float2(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.o_empty[b]);
+        };
+        // a wait that gave up leaves the loop running (without waits) to its
+        // end, since the two warps of a row meet at a barrier in it
         for (uint32_t t = 0; t < nt; ++t) {
             const uint32_t b = t & 1, key0 = (t0 + t) * kTcKeys, ring = t % kTcRing;
-            ok = mbar_wait(&sh.s_full[b], (t >> 1) & 1);
+            ok = ok && mbar_wait(&sh.s_full[b], (t >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
             tc_fence_after();
             const uint32_t sp = lanes + C::s0 + b * kTcKeys;
-            float s[kTcKeys];
+            float s[SC];
             {
                 uint32_t x[32];
-                tmem_ld32(sp, x);
+                tmem_ld32(sp + half * SC, x);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(x[i]);
-                tmem_ld32(sp + 32, x);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) s[32 + i] = __uint_as_float(x[i]);
+                for (int i = 0; i < SC; ++i) s[i] = __uint_as_float(x[i]);
             }
             // (never 0: an unseen key's -inf times it stays -inf)
             const float raw = fmaxf(qinv * sh.k_scale[ring], 0x1p-120f);
             const unsigned long long bad = sh.k_bad[ring];
             if (key0 + kTcKeys > a.n_past || bad) {
-                const unsigned long long seen = tc_seen(a.mask, a.n_past, a.n_tokens, tok, key0);
+                const uint32_t seen = (uint32_t)(tc_seen(a.mask, a.n_past, a.n_tokens, tok, key0) >> (half * SC));
+                const uint32_t hurt = (uint32_t)(bad >> (half * SC));
 #pragma unroll
-                for (int i = 0; i < (int)kTcKeys; ++i) {
+                for (int i = 0; i < SC; ++i) {
                     if (!((seen >> i) & 1)) s[i] = -INFINITY;
-                    else if ((bad >> i) & 1) s[i] = __uint_as_float(0x7FC00000u);
+                    else if ((hurt >> i) & 1) s[i] = __uint_as_float(0x7FC00000u);
                 }
             }
             if (sc) {
 #pragma unroll
-                for (int i = 0; i < (int)kTcKeys; i += 4)
+                for (int i = 0; i < SC; i += 4)
                     *reinterpret_cast<float4*>(sc + key0 + i) =
                         make_float4(s[i] * raw, s[i + 1] * raw, s[i + 2] * raw, s[i + 3] * raw);
             }
             float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 4; i < (int)kTcKeys; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            for (int i = 4; i < SC; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            sh.part_max[b][half][rl] = top;
+            asm volatile("barrier.cta.sync %0, 64;" ::"r"(4 + quad) : "memory");
+            top = fmaxf(top, sh.part_max[b][half ^ 1][rl]);
             const float ct = raw * p.c;
             const float mn = fmaxf(m, top == -INFINITY ? -INFINITY : ceilf(top * ct));
             const float ref = mn == -INFINITY ? 0.f : mn;
-            const float corr = ex2_approx(m - ref);
-            sh.corr[t % kTcCorr][rl] = corr;
+            const float corr_t = ex2_approx(m - ref);
             m = mn;
             const float off = kPShift - ref;
             float2 sum = make_float2(0.f, 0.f);
             const float2 ct2 = make_float2(ct, ct), off2 = make_float2(off, off);
 #pragma unroll
-            for (int i = 0; i < (int)kTcKeys; i += 16) {
+            for (int i = 0; i < SC; i += 16) {
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -599,85 +681,56 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
                     sum = add2(sum, e);
                     split_f16(e, hi[j], lo[j]);
                 }
-                tmem_st8(sp + i / 2, hi);
-                tmem_st8(sp + 32 + i / 2, lo);
+                tmem_st8(sp + half * (SC / 2) + i / 2, hi);
+                tmem_st8(sp + 32 + half * (SC / 2) + i / 2, lo);
             }
-            l = fmaf(l, corr, sum.x + sum.y);
+            l = fmaf(l, corr_t, sum.x + sum.y);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.p_full[b]);
+            if (t) take_output(t - 1);
+            corr = corr_t;
         }
-        sh.ml[rl] = make_float2(m, l * 0x1p-14f);
+        take_output(nt - 1);
+        sh.part_sum[half][rl] = l;
+        asm volatile("barrier.cta.sync %0, 64;" ::"r"(4 + quad) : "memory");
+        l = (l + sh.part_sum[half ^ 1][rl]) * 0x1p-14f;
+        const size_t row = (size_t)g * p.R + r;
+        float f = 1.f;
+        if (p.n_split > 1) {
+            if (half == 0 && valid) p.part_ml[(size_t)split * a.n_kv * p.R + row] = make_float2(m, l);
+        } else {
+            f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+            if (half == 0 && valid && p.scores) p.stats[row] = make_float2(m == -INFINITY ? 0.f : m, f);
+        }
+        // rows leave through K's slots (every MMA has completed), so that the
+        // stores run along rows
+        constexpr int OL = OC / 4, OX = OL < 8 ? OL - 1 : 7;  // float4s of half a row; their permutation
+        float4* stage = reinterpret_cast<float4*>(ks) + warp * 32 * OL;
+#pragma unroll
+        for (int i = 0; i < OC; i += 4)
+            stage[lane * OL + ((i / 4) ^ (lane & OX))] =
+                make_float4(o[i / 2].x * f, o[i / 2].y * f, o[i / 2 + 1].x * f, o[i / 2 + 1].y * f);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.ml_full);
-    } else if (warp < 12) {
-        // ---- output: lane = row, warps 4..7 the first half of the columns, 8..11 the second
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
-        constexpr int OC = HD / 2;
-        float2 o[OC / 2];
-#pragma unroll
-        for (int i = 0; i < OC / 2; ++i) o[i] = make_float2(0.f, 0.f);
-        const uint32_t rl = (warp & 3) * 32 + lane, r = r0 + rl, col = warp < 8 ? 0 : OC;
-        const uint32_t src = tm + (((warp & 3) * 32u) << 16) + C::o0 + col;
-        for (uint32_t t = 0; t < nt; ++t) {
-            const uint32_t b = t & 1;
-            ok = mbar_wait(&sh.o_full[b], (t >> 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            const float corr = sh.corr[t % kTcCorr][rl], scale = sh.v_scale[t % kTcRing] * 0x1p-14f;
-            const float2 corr2 = make_float2(corr, corr), scale2 = make_float2(scale, scale);
-#pragma unroll
-            for (int c = 0; c < OC; c += 16) {
-                uint32_t x[16];
-                tmem_ld16(src + b * 128 + c, x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    o[c / 2 + i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2,
-                                        mul2(o[c / 2 + i], corr2));
-            }
-            const unsigned long long bad = sh.v_bad[t % kTcRing];
-            if (bad && r < p.R && (bad & tc_seen(a.mask, a.n_past, a.n_tokens, r / p.G, (t0 + t) * kTcKeys))) {
-#pragma unroll
-                for (int i = 0; i < OC / 2; ++i)
-                    o[i] = make_float2(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.o_empty[b]);
+#pragma unroll 4
+        for (int i = lane; i < 32 * OL; i += 32) {
+            const uint32_t ro = r0 + quad * 32 + i / OL, c = half * OC + i % OL * 4;
+            if (ro >= p.R) break;
+            float* dst = p.n_split > 1
+                             ? p.part_o + ((size_t)split * a.n_kv * p.R + (size_t)g * p.R + ro) * HD + c
+                             : a.out + (size_t)(ro / p.G) * a.out_stride + ((size_t)g * p.G + ro % p.G) * HD + c;
+            *reinterpret_cast<float4*>(dst) = stage[i / OL * OL + ((i % OL) ^ (i / OL & OX))];
         }
-        ok = mbar_wait(&sh.ml_full, 0) && ok;
-        if (r < p.R) {
-            const float2 ml = sh.ml[rl];
-            const size_t row = (size_t)g * p.R + r;
-            float* dst;
-            float f = 1.f;
-            if (p.n_split > 1) {
-                const size_t slot = (size_t)split * a.n_kv * p.R + row;
-                dst = p.part_o + slot * HD + col;
-                if (col == 0) p.part_ml[slot] = ml;
-            } else {
-                f = ml.y > 0.f ? 1.f / ml.y : (ml.y == 0.f ? 0.f : ml.y);
-                dst = a.out + (size_t)(r / p.G) * a.out_stride + ((size_t)g * p.G + r % p.G) * HD + col;
-                if (col == 0 && p.scores) p.stats[row] = make_float2(ml.x == -INFINITY ? 0.f : ml.x, f);
-            }
-#pragma unroll
-            for (int i = 0; i < OC; i += 4)
-                *reinterpret_cast<float4*>(dst + i) =
-                    make_float4(o[i / 2].x * f, o[i / 2].y * f, o[i / 2 + 1].x * f, o[i / 2 + 1].y * f);
-        }
-    } else if (warp < 20) {
+    } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        ok = tc_convert<HD>(a.kcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, 0, (int)threadIdx.x - 384, ks,
-                            sh.k_full, sh.k_empty, sh.k_scale, sh.k_bad, sh.wmax[0]);
-    } else if (warp < 28) {
+        ok = tc_convert<HD, 0>(p.n, t0, nt, (int)threadIdx.x - 256, smem, sh);
+    } else if (warp < 24) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        ok = tc_convert<HD>(a.vcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, 1, (int)threadIdx.x - 640, vs,
-                            sh.v_full, sh.v_empty, sh.v_scale, sh.v_bad, sh.wmax[1]);
+        ok = tc_convert<HD, 1>(p.n, t0, nt, (int)threadIdx.x - 512, smem, sh);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
-        if (warp == 28) {
+        if (warp == 24) {
             // ---- MMA issuer: the whole warp walks the loop, one lane issues
             uint32_t leader;
             asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
@@ -738,13 +791,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
             if (leader) mma_commit(&sh.done);
             __syncwarp();
             ok = mbar_wait(&sh.done, 0) && ok;
+        } else if (lane == 0 && warp == 25) {
+            ok = tc_copy<HD>(a.kcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, raw, sh.raw_full[0], sh.raw_empty[0]);
+        } else if (lane == 0 && warp == 26) {
+            ok = tc_copy<HD>(a.vcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, raw + 2 * C::raw, sh.raw_full[1],
+                             sh.raw_empty[1]);
         }
     }
     if (!ok) atomicOr(p.err, kErrTreeWait);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 28) {
+    if (warp == 24) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u) : "memory");
     }
