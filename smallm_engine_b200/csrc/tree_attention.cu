@@ -314,12 +314,14 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
           "l"(reinterpret_cast<const uint64_t&>(c)));
     return r;
 }
+// hi = x rounded to f16, lo = (x - hi) rounded to f16, of two values.
 __device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __float22half2_rn(x);
-    const float2 f = __half22float2(h);
-    const __half2 l = __float22half2_rn(fma2(f, make_float2(-1.f, -1.f), x));
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
+    asm("{\n .reg .f16 a, b;\n .reg .f32 c, d;\n"
+        " cvt.rn.f16x2.f32 %0, %3, %2;\n mov.b32 {a, b}, %0;\n"
+        " sub.rn.f32.f16 c, a, %2;\n sub.rn.f32.f16 d, b, %3;\n"
+        " neg.f32 c, c;\n neg.f32 d, d;\n cvt.rn.f16x2.f32 %1, d, c;\n}"
+        : "=&r"(hi), "=r"(lo)
+        : "f"(x.x), "f"(x.y));
 }
 // Barrier of the 256 threads of converter group `id`; true where any says so.
 __device__ __forceinline__ bool conv_any(int id, bool v) {
@@ -416,7 +418,14 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
 #pragma unroll
             for (int i = h * N / 2; i < (h + 1) * N / 2; ++i) {
                 x[i] = src[i * kConvThreads];
-                if (left < kTcKeys && row0 + i * STEP >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            if (left < kTcKeys) {
+#pragma unroll
+                for (int i = h * N / 2; i < (h + 1) * N / 2; ++i)
+                    if (row0 + i * STEP >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int i = h * N / 2; i < (h + 1) * N / 2; ++i) {
                 m = max_abs_nan(max_abs_nan(max_abs_nan(max_abs_nan(m, x[i].x), x[i].y), x[i].z), x[i].w);
             }
             __syncwarp();
@@ -429,9 +438,7 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
         if (use > 0) stuck = stuck || !mbar_wait(&empty[slot], (use - 1) & 1);
         else if (GROUP == 1 && t == 0) stuck = stuck || !mbar_wait(&sh.q_full, 0);
         if (conv_any(1 + GROUP, stuck)) return false;
-        uint32_t mx = 0;
-#pragma unroll
-        for (int w = 0; w < (int)kConvWarps; ++w) mx = max(mx, wmax[t & 1][w]);
+        uint32_t mx = __reduce_max_sync(0xffffffffu, wmax[t & 1][lane % kConvWarps]);
         if (mx >= 0x7F800000u) {  // the same for the whole group: clean the tile
             m = 0.f;
             uint32_t hurt = 0;  // this thread's units that held any
@@ -449,9 +456,7 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
             conv_any(1 + GROUP, false);  // wmax has been read by all
             if (lane == 0) wmax[t & 1][cw] = m2;
             conv_any(1 + GROUP, false);
-            mx = 0;
-#pragma unroll
-            for (int w = 0; w < (int)kConvWarps; ++w) mx = max(mx, wmax[t & 1][w]);
+            mx = __reduce_max_sync(0xffffffffu, wmax[t & 1][lane % kConvWarps]);
         }
         float mult, inv;
         tc_scale(mx, mult, inv);
@@ -488,6 +493,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
     const uint32_t tiles = (p.n + kTcKeys - 1) / kTcKeys;
     const uint32_t t0 = split * p.tiles_per_split, nt = min(tiles, t0 + p.tiles_per_split) - t0;
 
+    const uint32_t quads = min(4u, (p.R - r0 + 31) / 32);  // warps' row quarters that hold rows
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kTcSlots; ++i) {
             mbar_init(&sh.k_full[i], kConvWarps);
@@ -501,11 +507,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
         }
         for (uint32_t b = 0; b < 2; ++b) {
             mbar_init(&sh.s_full[b], 2);   // the MMA's commit and the issuing thread
-            mbar_init(&sh.p_full[b], 8);
+            mbar_init(&sh.p_full[b], 2 * quads);
             mbar_init(&sh.o_full[b], 2);
-            mbar_init(&sh.o_empty[b], 8);
+            mbar_init(&sh.o_empty[b], 2 * quads);
         }
-        mbar_init(&sh.q_full, 8);
+        mbar_init(&sh.q_full, 2 * quads);
         mbar_init(&sh.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -566,6 +572,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
             }
         }
         asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
+        // a quarter without rows is done: what the products hold in its lanes is not read
+        if (quad < quads) {
         float qinv;
         {
             const float4* src = reinterpret_cast<const float4*>(vs) + rl * (HD / 4);
@@ -602,7 +610,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             const float scale = sh.v_scale[t % kTcRing] * 0x1p-14f;
-            const float2 corr2 = make_float2(corr, corr), scale2 = make_float2(scale, scale);
+            if (__any_sync(0xffffffffu, corr != 1.f)) {
+                const float2 corr2 = make_float2(corr, corr);
+#pragma unroll
+                for (int i = 0; i < OC / 2; ++i) o[i] = mul2(o[i], corr2);
+            }
+            const float2 scale2 = make_float2(scale, scale);
 #pragma unroll
             for (int c = 0; c < OC; c += 16) {
                 uint32_t x[16];
@@ -610,7 +623,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     o[c / 2 + i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2,
-                                        mul2(o[c / 2 + i], corr2));
+                                        o[c / 2 + i]);
             }
             const unsigned long long bad = sh.v_bad[t % kTcRing];
             if (bad && valid && (bad & tc_seen(a.mask, a.n_past, a.n_tokens, tok, (t0 + t) * kTcKeys))) {
@@ -721,6 +734,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
                              ? p.part_o + ((size_t)split * a.n_kv * p.R + (size_t)g * p.R + ro) * HD + c
                              : a.out + (size_t)(ro / p.G) * a.out_stride + ((size_t)g * p.G + ro % p.G) * HD + c;
             *reinterpret_cast<float4*>(dst) = stage[i / OL * OL + ((i % OL) ^ (i / OL & OX))];
+        }
         }
     } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
