@@ -14,12 +14,15 @@
 // latency: one read of the totals and four cluster barriers.
 //
 // move: row dst + i of K and V (and the totals) becomes row rows[i], for a
-// strictly ascending list with rows[i] >= dst + i.  In place: a cluster owns a
-// slice of columns of one head and walks the list in waves, all of a wave's
-// loads (in registers) before any of its stores, by a cluster barrier.  A later
-// wave's source rows[j], j >= i, is at least dst + j, so no store of an
-// earlier wave can have overwritten it, and its loads are in flight before
-// the wave's barrier.  Bound by the bytes moved.
+// strictly ascending list with rows[i] >= dst + i.  In place: a cluster owns
+// one head's K or V and walks the list in waves, all of a wave's rows read
+// before any is written, by a cluster barrier.  A later wave's source rows[j],
+// j >= i, is at least dst + j, so no store of an earlier wave can have
+// overwritten it, and its reads run while the wave before is written.
+//   - up to a wave of one CTA (an accepted path): rows pass through registers;
+//   - longer lists: rows arrive in two shared-memory buffers by a bulk copy
+//     each, and leave, being neighbours now, by one bulk copy of the buffer.
+//     Bound by the bytes moved (registers instead of bulk copies: %MOVE_REG%).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -94,12 +97,15 @@ __global__ void __launch_bounds__(kSelThreads, 1)
         if (2u * tid < bins) {
             own = *reinterpret_cast<const uint2*>(&hist[top]);
             sum = own;
-            for (uint32_t r = 1; r < C; ++r) {
-                const uint32_t peer = cr + r < C ? cr + r : cr + r - C;
-                const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[top], peer));
-                sum.x += v.x;
-                sum.y += v.y;
-            }
+            // all peers' reads in flight at once
+#pragma unroll
+            for (uint32_t r = 1; r < kSelMaxCluster; ++r)
+                if (r < C) {
+                    const uint32_t peer = cr + r < C ? cr + r : cr + r - C;
+                    const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[top], peer));
+                    sum.x += v.x;
+                    sum.y += v.y;
+                }
         }
         // inclusive scan of the pairs from the top: keys in this pair's bins or above
         uint32_t incl = sum.x + sum.y, iown = own.x + own.y;
@@ -114,10 +120,8 @@ __global__ void __launch_bounds__(kSelThreads, 1)
         }
         __syncthreads();
         uint32_t before = incl - sum.x - sum.y, obefore = iown - own.x - own.y;
-        for (int v = 0; v < warp; ++v) {
-            before += sh.warp[v];
-            obefore += sh.warp_eq[v];
-        }
+        before += __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp[lane] : 0u);
+        obefore += __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_eq[lane] : 0u);
         // the bin where the count from the top reaches `want`
         if (before < want && want <= before + sum.x + sum.y) {
             const bool up = want <= before + sum.y;  // the higher bin of the pair
@@ -137,12 +141,15 @@ __global__ void __launch_bounds__(kSelThreads, 1)
     }
     if (C > 1) cluster.sync();
     else __syncthreads();
+    // keys of the ranges before this one (lane r: CTA r)
     uint32_t gt0 = 0, eq0 = 0;
-    for (uint32_t r = 0; r < cr; ++r) {
-        const SelShared* o = cluster.map_shared_rank(&sh, r);
-        gt0 += o->gt;
-        eq0 += o->eq;
+    if ((uint32_t)lane < cr) {
+        const SelShared* o = cluster.map_shared_rank(&sh, lane);
+        gt0 = o->gt;
+        eq0 = o->eq;
     }
+    gt0 = __reduce_add_sync(0xffffffffu, gt0);
+    eq0 = __reduce_add_sync(0xffffffffu, eq0);
     // each warp owns a contiguous run of the range
     const uint32_t run = (len + kSelThreads - 1) / kSelThreads * 32;
     const uint32_t wb = min(len, warp * run), we = min(len, wb + run);
@@ -157,10 +164,8 @@ __global__ void __launch_bounds__(kSelThreads, 1)
         sh.warp_eq[warp] = ce;
     }
     __syncthreads();
-    for (int v = 0; v < warp; ++v) {
-        gt0 += sh.warp[v];
-        eq0 += sh.warp_eq[v];
-    }
+    gt0 += __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp[lane] : 0u);
+    eq0 += __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_eq[lane] : 0u);
     const uint32_t lt = (1u << lane) - 1u;
     for (uint32_t i = wb + lane; i - lane < we; i += 32) {
         const uint32_t key = i < we ? key_of(i) : 0u;
@@ -176,9 +181,9 @@ __global__ void __launch_bounds__(kSelThreads, 1)
 
 constexpr int kMoveThreads = 512;
 constexpr int kMoveUnroll = 8;
-constexpr uint32_t kMoveWave = kMoveThreads * kMoveUnroll;  // vectors of a CTA per wave
-constexpr uint32_t kMoveMaxCluster = 8;
-constexpr unsigned kErrMoveList = 128u;
+constexpr uint32_t kMoveWave = kMoveThreads * kMoveUnroll;  // vectors of a CTA per wave in registers
+constexpr uint32_t kMoveMaxCluster = 16;
+constexpr unsigned kErrMoveList = 128u, kErrMoveWait = 512u;
 
 struct MoveArgs {
     const uint32_t* rows;
@@ -186,79 +191,145 @@ struct MoveArgs {
     unsigned int* err;
 };
 
-// Source row of entry i, or UINT32_MAX where there is nothing to do; an entry
-// that breaks the list's rules raises bit 7 of the error word.
+// Source row of entry i (< n_rows); dst + i, no move, where the entry breaks the
+// list's rules, which raises bit 7 of the error word.
 __device__ __forceinline__ uint32_t move_source(const MoveArgs& a, uint32_t i) {
-    if (i >= a.n_rows) return 0xFFFFFFFFu;
     const uint32_t src = __ldg(a.rows + i);
     const bool ok = src < a.max_ctx && src >= a.dst + i && (i == 0 || __ldg(a.rows + i - 1) < src);
     if (!ok) atomicOr(a.err, kErrMoveList);
-    return ok && src != a.dst + i ? src : 0xFFFFFFFFu;
+    return ok ? src : a.dst + i;
 }
 
-// base[(dst + i) * pitch + c] = base[rows[i] * pitch + c] for c < width
-// (vectors of type V); the cluster's CTAs take consecutive parts of a wave.
+// base[(dst + i) * width + c] = base[rows[i] * width + c] for c < width (vectors
+// of type V), by a cluster of C CTAs that take consecutive parts of a wave.
 template <typename V>
-__device__ __forceinline__ void move_rows(V* base, uint32_t pitch, uint32_t width, const MoveArgs& a, uint32_t C,
-                                          uint32_t cr) {
-    const uint32_t wave = kMoveWave * C / width;  // rows per wave (width divides kMoveWave)
-    const uint32_t c = threadIdx.x % width, r0 = (cr * kMoveWave + threadIdx.x) / width;
-    constexpr uint32_t kStep = kMoveThreads;
-    uint32_t src[kMoveUnroll];
-    V v[kMoveUnroll];
-    auto sources = [&](uint32_t first) {
-#pragma unroll
-        for (int u = 0; u < kMoveUnroll; ++u) src[u] = move_source(a, first + r0 + u * (kStep / width));
-    };
-    sources(0);
+__device__ __forceinline__ void move_rows(V* base, uint32_t width, const MoveArgs& a, uint32_t C, uint32_t cr) {
+    const uint32_t wave = kMoveWave * C / width;  // rows per wave (width divides kMoveThreads)
+    const uint32_t c = threadIdx.x % width, r0 = (cr * kMoveWave + threadIdx.x) / width, step = kMoveThreads / width;
     for (uint32_t first = 0; first < a.n_rows; first += wave) {
+        V v[kMoveUnroll];
         uint32_t go = 0;
 #pragma unroll
-        for (int u = 0; u < kMoveUnroll; ++u)
-            if (src[u] != 0xFFFFFFFFu) {
-                v[u] = base[(size_t)src[u] * pitch + c];
-                go |= 1u << u;
-            }
-        if (first + wave < a.n_rows) sources(first + wave);
+        for (int u = 0; u < kMoveUnroll; ++u) {
+            const uint32_t i = first + r0 + u * step;
+            if (i >= a.n_rows) continue;
+            const uint32_t src = move_source(a, i);
+            if (src == a.dst + i) continue;
+            v[u] = base[(size_t)src * width + c];
+            go |= 1u << u;
+        }
         if (C > 1) cg::this_cluster().sync();
         else __syncthreads();
 #pragma unroll
         for (int u = 0; u < kMoveUnroll; ++u)
-            if (go >> u & 1)
-                base[(size_t)(a.dst + first + r0 + u * (kStep / width)) * pitch + c] = v[u];
+            if (go >> u & 1) base[(size_t)(a.dst + first + r0 + u * step) * width + c] = v[u];
     }
 }
 
-// grid.x: (slice of columns) x cluster, grid.y: head, grid.z: K, V, totals
+// grid.y: head, grid.z: K, V, totals; a list of at most kMoveWave vectors, one CTA each
 __global__ void __launch_bounds__(kMoveThreads, 1)
-    smallm_cache_move_kernel(float* kc, float* vc, float* totals, uint32_t hd, uint32_t slice, MoveArgs a,
-                             uint32_t list_stride) {
-    cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t C = cluster.num_blocks(), cr = cluster.block_rank(), part = blockIdx.x / C;
+    smallm_cache_move_short_kernel(float* kc, float* vc, float* totals, uint32_t hd, MoveArgs a, uint32_t list_stride) {
     a.rows += (size_t)blockIdx.y * list_stride;
     if (blockIdx.z == 2) {
-        if (part == 0) move_rows<float>(totals + (size_t)blockIdx.y * a.max_ctx, 1, 1, a, C, cr);
-        return;
+        move_rows<float>(totals + (size_t)blockIdx.y * a.max_ctx, 1, a, 1, 0);
+    } else {
+        float* base = (blockIdx.z ? vc : kc) + (size_t)blockIdx.y * a.max_ctx * hd;
+        move_rows<float4>(reinterpret_cast<float4*>(base), hd / 4, a, 1, 0);
     }
-    float4* base = reinterpret_cast<float4*>((blockIdx.z ? vc : kc) + (size_t)blockIdx.y * a.max_ctx * hd) +
-                   part * slice;
-    move_rows<float4>(base, hd / 4, slice, a, C, cr);
+}
+
+// The totals of a longer list: a cluster per head.
+__global__ void __launch_bounds__(kMoveThreads)
+    smallm_cache_move_totals_kernel(float* totals, MoveArgs a, uint32_t list_stride) {
+    pdl_launch_dependents();  // K and V do not wait for the totals
+    cg::cluster_group cluster = cg::this_cluster();
+    a.rows += (size_t)blockIdx.y * list_stride;
+    move_rows<float>(totals + (size_t)blockIdx.y * a.max_ctx, 1, a, cluster.num_blocks(), cluster.block_rank());
+}
+
+constexpr uint32_t kMoveBuf = 96 * 1024;  // bytes of one of a CTA's two buffers
+
+// grid.x: the cluster's CTAs, grid.y: head, grid.z: K, V
+__global__ void __launch_bounds__(kMoveThreads, 1)
+    smallm_cache_move_kernel(float* kc, float* vc, uint32_t hd, MoveArgs a, uint32_t list_stride) {
+    extern __shared__ __align__(128) uint8_t buf[];
+    __shared__ __align__(8) uint64_t full[2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t C = cluster.num_blocks(), cr = cluster.block_rank();
+    const int tid = threadIdx.x;
+    a.rows += (size_t)blockIdx.y * list_stride;
+    if (tid == 0) {
+        mbar_init(&full[0], 1);
+        mbar_init(&full[1], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    float* base = (blockIdx.z ? vc : kc) + (size_t)blockIdx.y * a.max_ctx * hd;
+    const uint32_t row = hd * 4, per = kMoveBuf / row;  // bytes of a row; rows of a CTA per wave
+    const uint32_t waves = (a.n_rows + per * C - 1) / (per * C);
+    // this CTA's entries of wave w
+    auto range = [&](uint32_t w, uint32_t& first, uint32_t& count) {
+        first = min(a.n_rows, (w * C + cr) * per);
+        count = min(a.n_rows - first, per);
+    };
+    auto fetch = [&](uint32_t w) {
+        uint32_t first, count;
+        range(w, first, count);
+        uint64_t* bar = &full[w & 1];
+        if (tid == 0) {
+            if (count) mbar_arrive_expect_tx(bar, count * row);
+            else mbar_arrive(bar);
+        }
+        for (uint32_t i = tid; i < count; i += kMoveThreads)
+            bulk_g2s(buf + (w & 1) * kMoveBuf + i * row, base + (size_t)move_source(a, first + i) * hd, row, bar);
+    };
+    fetch(0);
+    bool ok = true;
+    for (uint32_t w = 0; w < waves; ++w) {
+        if (w + 1 < waves) {
+            // the other buffer's rows have left
+            if (w && tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncthreads();
+            fetch(w + 1);
+        }
+        // (a second wait after one that gave up: no copy lands in a CTA that has left)
+        ok = (mbar_wait(&full[w & 1], w >> 1 & 1) || (mbar_wait(&full[w & 1], w >> 1 & 1), false)) && ok;
+        ok = !__syncthreads_or(!ok);
+        if (C > 1) cluster.sync();  // every row of the wave has been read
+        else __syncthreads();
+        uint32_t first, count;
+        range(w, first, count);
+        if (ok && count && tid == 0) {
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                             base + (size_t)(a.dst + first) * hd),
+                         "r"(smem_u32(buf + (w & 1) * kMoveBuf)), "r"(count * row)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+    }
+    if (tid == 0) {
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (!ok) atomicOr(a.err, kErrMoveWait);
+    }
+    pdl_wait();  // this kernel ends after the totals' (where there is one before it)
 }
 
 void launch_cluster(const void* fn, dim3 grid, uint32_t threads, size_t smem, uint32_t C, cudaStream_t stream,
-                    void** args) {
+                    void** args, bool pdl = false) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = C;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = pdl ? 2 : 1;
     SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
 }
 
@@ -293,17 +364,29 @@ void launch_cache_move(float* kcache, float* vcache, float* weights, uint32_t n_
     if ((reinterpret_cast<uintptr_t>(kcache) | reinterpret_cast<uintptr_t>(vcache)) & 15u)
         throw Error(SMALLM_ERR_INVALID, "cache_move: kcache and vcache must be 16-byte aligned");
     if (!n_kv || !n_rows) return;
-    // CTAs of a cluster: no more than the rows fill a wave of; then slices of
-    // columns (16 floats, two 32-byte sectors, at least) until the SMs are used
-    const uint32_t sms = (uint32_t)device_sm_count();
-    uint32_t C = 1, slices = 1;
-    while (C < kMoveMaxCluster && (uint64_t)n_rows * hd / 4 > (uint64_t)C * kMoveWave && n_kv * 2 * C * 2 <= sms) C *= 2;
-    while (hd / slices > 16 && n_kv * 2 * C * slices * 2 <= sms && n_rows > 64) slices *= 2;
     MoveArgs a{rows, n_rows, dst, max_ctx, device_error_flag()};
-    uint32_t slice = hd / 4 / slices, stride = per_head ? n_rows : 0;
-    void* args[] = {&kcache, &vcache, &weights, &hd, &slice, &a, &stride};
-    launch_cluster((const void*)smallm_cache_move_kernel, dim3(slices * C, n_kv, weights ? 3 : 2), kMoveThreads, 0, C,
-                   stream, args);
+    uint32_t stride = per_head ? n_rows : 0;
+    if ((uint64_t)n_rows * hd / 4 <= kMoveWave) {
+        void* args[] = {&kcache, &vcache, &weights, &hd, &a, &stride};
+        launch_kernel_ex((const void*)smallm_cache_move_short_kernel, dim3(1, n_kv, weights ? 3 : 2),
+                         dim3(kMoveThreads), 0, stream, false, args);
+        return;
+    }
+    if (weights) {
+        uint32_t C = 1;
+        while (C < 8 && n_rows > C * kMoveWave) C *= 2;
+        void* args[] = {&weights, &a, &stride};
+        launch_cluster((const void*)smallm_cache_move_totals_kernel, dim3(C, n_kv), kMoveThreads, 0, C, stream, args);
+    }
+    // CTAs of a cluster: a buffer each at least, one CTA per SM in all
+    const uint32_t sms = (uint32_t)device_sm_count();
+    uint32_t C = 1;
+    while (C < kMoveMaxCluster && (uint64_t)n_rows * hd * 4 > (uint64_t)C * kMoveBuf && n_kv * 2 * C * 2 <= sms) C *= 2;
+    const void* fn = (const void*)smallm_cache_move_kernel;
+    set_smem_limit_once(fn, (int)(2 * kMoveBuf));
+    if (C > 8) SM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    void* args[] = {&kcache, &vcache, &hd, &a, &stride};
+    launch_cluster(fn, dim3(C, n_kv, 2), kMoveThreads, 2 * kMoveBuf, C, stream, args, weights != nullptr);
 }
 
 }  // namespace smallm

@@ -874,19 +874,37 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
     if (c == 0 && p.scores) p.stats[row] = make_float2(ref, inv);
 }
 
-// weights[g][k] += sum_r 2^(s c - mc_r) / sum_r, one thread per (KV head, key):
-// rows in order, so the total does not depend on the launch.
-__global__ void __launch_bounds__(256) smallm_tree_weights_kernel(const TreeParams p) {
-    const uint32_t key = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y;
-    if (key >= p.n) return;
-    float acc = 0.f;
-    const float* s = p.scores + (size_t)g * p.R * p.sc_stride + key;
-#pragma unroll 4
-    for (uint32_t r = 0; r < p.R; ++r) {
-        const float2 st = p.stats[(size_t)g * p.R + r];
-        acc = fmaf(exp2f(fmaf(s[(size_t)r * p.sc_stride], p.c, -st.x)), st.y, acc);
+// weights[g][k] += sum_r 2^(s c - mc_r) / sum_r.  A CTA per (128 keys, KV head);
+// a lane has four keys, warp w the rows w, w + 8, ...; the warps' sums meet in
+// shared memory in their order, so the total does not depend on the launch.
+constexpr int kWeightKeys = 128, kWeightWarps = 8;
+__global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(const TreeParams p) {
+    __shared__ float4 part[kWeightWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t key = blockIdx.x * kWeightKeys + 4 * lane, g = blockIdx.y;
+    pdl_wait();
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (key < p.sc_stride) {
+        const float* s = p.scores + (size_t)g * p.R * p.sc_stride + key;
+#pragma unroll 8
+        for (uint32_t r = warp; r < p.R; r += kWeightWarps) {
+            const float2 st = p.stats[(size_t)g * p.R + r];
+            const float4 v = *reinterpret_cast<const float4*>(s + (size_t)r * p.sc_stride);
+            acc.x = fmaf(exp2f(fmaf(v.x, p.c, -st.x)), st.y, acc.x);
+            acc.y = fmaf(exp2f(fmaf(v.y, p.c, -st.x)), st.y, acc.y);
+            acc.z = fmaf(exp2f(fmaf(v.z, p.c, -st.x)), st.y, acc.z);
+            acc.w = fmaf(exp2f(fmaf(v.w, p.c, -st.x)), st.y, acc.w);
+        }
     }
-    p.a.weights[(size_t)g * p.a.max_ctx + key] += acc;
+    part[warp][lane] = acc;
+    __syncthreads();
+    // (the scores behind the last key are not written: those sums are dropped here)
+    const uint32_t k = blockIdx.x * kWeightKeys + threadIdx.x;
+    if (threadIdx.x >= kWeightKeys || k >= p.n) return;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWeightWarps; ++w) sum += reinterpret_cast<const float*>(part[w])[threadIdx.x];
+    p.a.weights[(size_t)g * p.a.max_ctx + k] += sum;
 }
 
 #ifndef SMALLM_TREE_TC_ROWS
@@ -958,8 +976,11 @@ void launch_tree(const TreeParams& p, bool tc, cudaStream_t stream) {
                          stream, true, args);
     }
     if (p.a.weights) {
-        smallm_tree_weights_kernel<<<dim3((p.n + 255) / 256, p.a.n_kv), 256, 0, stream>>>(p);
-        SM_CUDA(cudaGetLastError());
+        TreeParams pp = p;
+        void* args[] = {&pp};
+        launch_kernel_ex((const void*)smallm_tree_weights_kernel,
+                         dim3((p.n + kWeightKeys - 1) / kWeightKeys, p.a.n_kv), dim3(32 * kWeightWarps), 0, stream, true,
+                         args);
     }
 }
 
