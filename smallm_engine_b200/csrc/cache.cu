@@ -15,18 +15,18 @@
 // totals and five cluster barriers.
 //
 // move: row dst + i of K and V (and the totals) becomes row rows[i], for a
-// strictly ascending list with rows[i] >= dst + i.  In place: a cluster owns
-// one head's K or V and walks the list in waves, all of a wave's rows read
-// before any is written, by a cluster barrier.  A later wave's source rows[j],
-// j >= i, is at least dst + j, so no store of an earlier wave can have
-// overwritten it, and its reads run while the wave before is written.
-//   - up to a wave of one CTA (an accepted path): rows pass through registers;
-//   - longer lists: rows arrive in shared memory by bulk copies, one for each
-//     run of neighbours, and leave, being neighbours now, by one bulk copy of a
-//     buffer.  One warp per CTA, four buffers of 16 KB, three of them on their
-//     way in while the barrier of the wave before is waited for.  Bound by the
-//     bytes moved.  8 heads x 16384 of 32768 rows of 128: %MOVE_US%; two buffers
-//     of 48 KB and 512 threads 88 us, through registers 166 us.
+// strictly ascending list with rows[i] >= dst + i.  In place: a cluster owns a
+// slice of columns of one head's K or V and walks the list in waves, a part of
+// a wave for each CTA, its rows in registers between load and store.  A store
+// may only overwrite rows that have been read.  Row dst + j is read by entries
+// <= j alone, so a CTA may store its part of a wave once the others have loaded
+// every wave whose first source lies below the part's end; each tells the
+// others how many waves it has loaded.  The distance rows[i] - (dst + i) never
+// shrinks along the list, so beyond the first few waves of an eviction that
+// has long been the case and nobody waits.  Bound by the bytes moved.
+// 8 heads x 16384 of 32768 rows of 128: %MOVE_US%; with a cluster barrier for
+// each wave 166 us, and rows by bulk copies through shared memory, whatever the
+// buffers, 88 us at best: copies of a row or two are too small for them.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kSelThreads, 2)
 constexpr int kMoveThreads = 512;
 constexpr int kMoveUnroll = 8;
 constexpr uint32_t kMoveWave = kMoveThreads * kMoveUnroll;  // vectors of a CTA per wave in registers
-constexpr uint32_t kMoveMaxCluster = 16;
+constexpr uint32_t kMoveMaxCluster = 8;
 constexpr unsigned kErrMoveList = 128u, kErrMoveWait = 512u;
 
 struct MoveArgs {
@@ -213,29 +213,25 @@ __device__ __forceinline__ uint32_t move_source(const MoveArgs& a, uint32_t i) {
 }
 
 // base[(dst + i) * width + c] = base[rows[i] * width + c] for c < width (vectors
-// of type V), by a cluster of C CTAs that take consecutive parts of a wave.
+// of type V) of a list that fits one wave of a CTA.
 template <typename V>
-__device__ __forceinline__ void move_rows(V* base, uint32_t width, const MoveArgs& a, uint32_t C, uint32_t cr) {
-    const uint32_t wave = kMoveWave * C / width;  // rows per wave (width divides kMoveThreads)
-    const uint32_t c = threadIdx.x % width, r0 = (cr * kMoveWave + threadIdx.x) / width, step = kMoveThreads / width;
-    for (uint32_t first = 0; first < a.n_rows; first += wave) {
-        V v[kMoveUnroll];
-        uint32_t go = 0;
+__device__ __forceinline__ void move_rows(V* base, uint32_t width, const MoveArgs& a) {
+    const uint32_t c = threadIdx.x % width, r0 = threadIdx.x / width, step = kMoveThreads / width;
+    V v[kMoveUnroll];
+    uint32_t go = 0;
 #pragma unroll
-        for (int u = 0; u < kMoveUnroll; ++u) {
-            const uint32_t i = first + r0 + u * step;
-            if (i >= a.n_rows) continue;
-            const uint32_t src = move_source(a, i);
-            if (src == a.dst + i) continue;
-            v[u] = base[(size_t)src * width + c];
-            go |= 1u << u;
-        }
-        if (C > 1) cg::this_cluster().sync();
-        else __syncthreads();
-#pragma unroll
-        for (int u = 0; u < kMoveUnroll; ++u)
-            if (go >> u & 1) base[(size_t)(a.dst + first + r0 + u * step) * width + c] = v[u];
+    for (int u = 0; u < kMoveUnroll; ++u) {
+        const uint32_t i = r0 + u * step;
+        if (i >= a.n_rows) continue;
+        const uint32_t src = move_source(a, i);
+        if (src == a.dst + i) continue;
+        v[u] = base[(size_t)src * width + c];
+        go |= 1u << u;
     }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u)
+        if (go >> u & 1) base[(size_t)(a.dst + r0 + u * step) * width + c] = v[u];
 }
 
 // grid.y: head, grid.z: K, V, totals; a list of at most kMoveWave vectors, one CTA each
@@ -243,133 +239,134 @@ __global__ void __launch_bounds__(kMoveThreads, 1)
     smallm_cache_move_short_kernel(float* kc, float* vc, float* totals, uint32_t hd, MoveArgs a, uint32_t list_stride) {
     a.rows += (size_t)blockIdx.y * list_stride;
     if (blockIdx.z == 2) {
-        move_rows<float>(totals + (size_t)blockIdx.y * a.max_ctx, 1, a, 1, 0);
+        move_rows<float>(totals + (size_t)blockIdx.y * a.max_ctx, 1, a);
     } else {
         float* base = (blockIdx.z ? vc : kc) + (size_t)blockIdx.y * a.max_ctx * hd;
-        move_rows<float4>(reinterpret_cast<float4*>(base), hd / 4, a, 1, 0);
+        move_rows<float4>(reinterpret_cast<float4*>(base), hd / 4, a);
     }
 }
 
-// The totals of a longer list: a cluster per head.
-__global__ void __launch_bounds__(kMoveThreads)
-    smallm_cache_move_totals_kernel(float* totals, MoveArgs a, uint32_t list_stride) {
-    pdl_launch_dependents();  // K and V do not wait for the totals
-    cg::cluster_group cluster = cg::this_cluster();
-    a.rows += (size_t)blockIdx.y * list_stride;
-    move_rows<float>(totals + (size_t)blockIdx.y * a.max_ctx, 1, a, cluster.num_blocks(), cluster.block_rank());
+constexpr uint32_t kMoveTotals = kMoveWave / 4 / kMoveThreads;  // rows of a thread in a wave of the narrowest slice
+constexpr uint32_t kMoveStarts = 2048;  // waves whose first sources are kept at hand
+
+__device__ __forceinline__ uint32_t ld_acquire_cluster(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.acquire.cluster.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+    return v;
+}
+// *p of CTA `rank` = v
+__device__ __forceinline__ void st_release_cluster(const uint32_t* p, uint32_t rank, uint32_t v) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("st.release.cluster.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 
-constexpr uint32_t kMoveBuf = 16 * 1024;  // bytes of one of a CTA's buffers
-constexpr uint32_t kMoveBufs = 4;         // (three CTAs fit an SM)
-
-// grid.x: the cluster's CTAs (one warp each), grid.y: head, grid.z: K, V
-__global__ void __launch_bounds__(32) smallm_cache_move_kernel(float* kc, float* vc, uint32_t hd, MoveArgs a,
-                                                             uint32_t list_stride) {
-    extern __shared__ __align__(128) uint8_t buf[];
-    __shared__ __align__(8) uint64_t full[kMoveBufs];
+// grid.x: (slice of columns) x cluster, grid.y: head, grid.z: K, V; `slice`
+// float4s of a row.  The first slice of K takes the totals along.
+__global__ void __launch_bounds__(kMoveThreads, 2)
+    smallm_cache_move_kernel(float* kc, float* vc, float* totals, uint32_t hd, uint32_t slice, MoveArgs a,
+                             uint32_t list_stride) {
+    __shared__ uint32_t start[kMoveStarts];
+    __shared__ uint32_t loaded[kMoveMaxCluster];  // waves that each CTA has loaded
+    __shared__ uint32_t stuck;
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t C = cluster.num_blocks(), cr = cluster.block_rank(), lane = threadIdx.x;
+    const uint32_t C = cluster.num_blocks(), cr = cluster.block_rank(), tid = threadIdx.x;
     a.rows += (size_t)blockIdx.y * list_stride;
-    if (lane == 0) {
-        for (uint32_t b = 0; b < kMoveBufs; ++b) mbar_init(&full[b], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncwarp();
-    float* base = (blockIdx.z ? vc : kc) + (size_t)blockIdx.y * a.max_ctx * hd;
-    const uint32_t row = hd * 4, per = kMoveBuf / row;  // bytes of a row; rows of a CTA per wave (32, 64 or 128)
-    const uint32_t waves = (a.n_rows + per * C - 1) / (per * C);
-    // this CTA's entries of wave w
-    auto range = [&](uint32_t w, uint32_t& first, uint32_t& count) {
-        first = min(a.n_rows, (w * C + cr) * per);
-        count = min(a.n_rows - first, per);
-    };
-    uint32_t src[4];  // the lane's entries of the wave that is fetched next
+    const uint32_t per = kMoveWave / slice, wave = per * C;  // rows of a CTA and of the cluster in a wave
+    const uint32_t waves = (a.n_rows + wave - 1) / wave;
+    for (uint32_t w = tid; w < min(waves, kMoveStarts); w += kMoveThreads) start[w] = __ldg(a.rows + w * wave);
+    if (tid < kMoveMaxCluster) loaded[tid] = 0;
+    if (tid == 0) stuck = 0;
+    float4* base = reinterpret_cast<float4*>((blockIdx.z ? vc : kc) + (size_t)blockIdx.y * a.max_ctx * hd) +
+                   blockIdx.x / C * slice + tid % slice;
+    const uint32_t pitch = hd / 4, step = kMoveThreads / slice, own = tid / slice;
+    totals = totals && blockIdx.z == 0 && blockIdx.x < C ? totals + (size_t)blockIdx.y * a.max_ctx : nullptr;
+    uint32_t src[kMoveUnroll];  // the next wave's source rows
     auto sources = [&](uint32_t w) {
-        uint32_t first, count;
-        range(w, first, count);
+        const uint32_t first = w * wave + cr * per;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (32 * j + lane < count) src[j] = move_source(a, first + 32 * j + lane);
-    };
-    auto fetch = [&](uint32_t w) {
-        uint32_t first, count;
-        range(w, first, count);
-        uint64_t* bar = &full[w % kMoveBufs];
-        if (lane == 0) {
-            if (count) mbar_arrive_expect_tx(bar, count * row);
-            else mbar_arrive(bar);
+        for (int u = 0; u < kMoveUnroll; ++u) {
+            const uint32_t i = first + own + u * step;
+            src[u] = i < a.n_rows ? move_source(a, i) : a.dst + i;
         }
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (32 * j >= count) break;
-            // neighbours travel in one copy
-            const bool in = 32 * j + lane < count;
-            const uint32_t left = __shfl_up_sync(0xffffffffu, src[j], 1);
-            const uint32_t heads = __ballot_sync(0xffffffffu, in && (lane == 0 || src[j] != left + 1));
-            if (!(heads >> lane & 1)) continue;
-            const uint32_t more = heads & ~((2u << lane) - 1u);  // the next run's first lane
-            const uint32_t len = min(more ? __ffs(more) - 1 - lane : 32u - lane, count - 32 * j - lane);
-            bulk_g2s(buf + (w % kMoveBufs) * kMoveBuf + (32 * j + lane) * row, base + (size_t)src[j] * hd, len * row, bar);
-        }
-        __syncwarp();
     };
-    for (uint32_t w = 0; w < min(waves, kMoveBufs - 1); ++w) {
-        sources(w);
-        fetch(w);
-    }
-    if (kMoveBufs - 1 < waves) sources(kMoveBufs - 1);
-    bool ok = true;
+    sources(0);
+    cluster.sync();
+    uint32_t need = 0;  // the last wave with a source below this part's end
     for (uint32_t w = 0; w < waves; ++w) {
-        // (a second wait after one that gave up: no copy lands in a CTA that has left)
-        uint64_t* bar = &full[w % kMoveBufs];
-        const uint32_t parity = w / kMoveBufs & 1;
-        ok = (mbar_wait(bar, parity) || (mbar_wait(bar, parity), false)) && ok;
-        ok = __all_sync(0xffffffffu, ok);
-        cluster_arrive_release();  // this CTA's rows of the wave have been read
-        const uint32_t next = w + kMoveBufs - 1;
-        if (next < waves) {
-            // the buffer's rows of wave w - 1 have left
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
-            fetch(next);
-            if (next + 1 < waves) sources(next + 1);
+        const uint32_t first = w * wave + cr * per;
+        float4 v[kMoveUnroll];
+        uint32_t go = 0, seen = 0;
+#pragma unroll
+        for (int u = 0; u < kMoveUnroll; ++u) {
+            if (src[u] == a.dst + first + own + u * step) continue;
+            v[u] = base[(size_t)src[u] * pitch];
+            go |= 1u << u;
         }
-        cluster_wait();  // everybody's have
-        uint32_t first, count;
-        range(w, first, count);
-        if (ok && count && lane == 0) {
-            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
-                             base + (size_t)(a.dst + first) * hd),
-                         "r"(smem_u32(buf + (w % kMoveBufs) * kMoveBuf)), "r"(count * row)
-                         : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        float total[kMoveTotals] = {};
+        if (totals) {
+#pragma unroll
+            for (int u = 0; u < (int)kMoveTotals; ++u) {
+                const uint32_t j = tid + u * kMoveThreads;
+                if (j < per && first + j < a.n_rows) {
+                    total[u] = totals[move_source(a, first + j)];
+                    seen |= __float_as_uint(total[u]);
+                }
+            }
         }
-        __syncwarp();
+        if (w + 1 < waves) sources(w + 1);
+#pragma unroll
+        for (int u = 0; u < kMoveUnroll; ++u)
+            if (go >> u & 1)
+                seen |= __float_as_uint(v[u].x) | __float_as_uint(v[u].y) | __float_as_uint(v[u].z) | __float_as_uint(v[u].w);
+        // every thread's loads have returned (their values are in `seen`)
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.u32 p, %0, 0;\n barrier.cta.red.or.pred q, 0, p;\n}" ::"r"(seen) : "memory");
+        if (tid < 32) {
+            if (tid < C) st_release_cluster(&loaded[cr], tid, w + 1);
+            const uint32_t end = a.dst + min(a.n_rows, first + per);
+            while (need < w && (need + 1 >= kMoveStarts || start[need + 1] < end)) ++need;
+            const long long t0 = clock64();
+            for (;;) {
+                const bool behind = tid < C && ld_acquire_cluster(&loaded[tid]) <= need;
+                if (!__any_sync(0xffffffffu, behind)) break;
+                if (__any_sync(0xffffffffu, clock64() - t0 > (1ll << 31))) {
+                    if (tid == 0) stuck = 1;
+                    break;
+                }
+            }
+        }
+        __syncthreads();
+        if (stuck) continue;
+#pragma unroll
+        for (int u = 0; u < kMoveUnroll; ++u)
+            if (go >> u & 1) base[(size_t)(a.dst + first + own + u * step) * pitch] = v[u];
+        if (totals) {
+#pragma unroll
+            for (int u = 0; u < (int)kMoveTotals; ++u) {
+                const uint32_t j = tid + u * kMoveThreads;
+                if (j < per && first + j < a.n_rows) totals[a.dst + first + j] = total[u];
+            }
+        }
     }
-    if (lane == 0) {
-        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        if (!ok) atomicOr(a.err, kErrMoveWait);
-    }
-    pdl_wait();  // this kernel ends after the totals' (where there is one before it)
+    if (tid == 0 && stuck) atomicOr(a.err, kErrMoveWait);
+    cluster.sync();  // peers may still write here
 }
 
 void launch_cluster(const void* fn, dim3 grid, uint32_t threads, size_t smem, uint32_t C, cudaStream_t stream,
-                    void** args, bool pdl = false) {
+                    void** args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
+    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = C;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 2 : 1;
+    cfg.numAttrs = 1;
     SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
 }
 
@@ -441,22 +438,18 @@ void launch_cache_move(float* kcache, float* vcache, float* weights, uint32_t n_
                          dim3(kMoveThreads), 0, stream, false, args);
         return;
     }
-    if (weights) {
-        uint32_t C = 1;
-        while (C < 8 && n_rows > C * kMoveWave) C *= 2;
-        void* args[] = {&weights, &a, &stride};
-        launch_cluster((const void*)smallm_cache_move_totals_kernel, dim3(C, n_kv), kMoveThreads, 0, C, stream, args);
-    }
-    // CTAs of a cluster: a buffer each at least, two CTAs per SM in all, and no
-    // cluster left waiting for another to end
+    // CTAs of a cluster: a wave's part each at least; then slices of columns (64
+    // bytes at least) until there are two CTAs per SM; no cluster left waiting
+    // for another to end
     const uint32_t sms = (uint32_t)device_sm_count();
     const void* fn = (const void*)smallm_cache_move_kernel;
-    set_smem_limit_once(fn, (int)(kMoveBufs * kMoveBuf));
-    uint32_t C = 1;
-    while (C < kMoveMaxCluster && (uint64_t)n_rows * hd * 4 > (uint64_t)C * kMoveBuf && n_kv * 2 * C <= 2 * sms) C *= 2;
-    while (C > 1 && clusters_at_once(fn, C, 32, kMoveBufs * kMoveBuf) < 2 * n_kv) C /= 2;
-    void* args[] = {&kcache, &vcache, &hd, &a, &stride};
-    launch_cluster(fn, dim3(C, n_kv, 2), 32, kMoveBufs * kMoveBuf, C, stream, args, weights != nullptr);
+    uint32_t C = 1, slices = 1;
+    while (C < kMoveMaxCluster && (uint64_t)n_rows * hd / 4 > (uint64_t)C * kMoveWave && n_kv * 4 * C <= 2 * sms) C *= 2;
+    while (hd / slices > 16 && n_kv * 4 * C * slices <= 2 * sms) slices *= 2;
+    while (C > 1 && clusters_at_once(fn, C, kMoveThreads, 0) < 2 * n_kv * slices) C /= 2;
+    uint32_t slice = hd / 4 / slices;
+    void* args[] = {&kcache, &vcache, &weights, &hd, &slice, &a, &stride};
+    launch_cluster(fn, dim3(slices * C, n_kv, 2), kMoveThreads, 0, C, stream, args);
 }
 
 }  // namespace smallm
