@@ -10,7 +10,7 @@
 // summed over the cluster's shared memory, then the bin that holds the rank.
 // (Digits of 11, 11 and 10 bits save a barrier, but then every CTA reads 8 KB
 // from each of 15 others for each digit: 37 us for 8 x 131072 keys where this
-// takes %SEL_US%.)  Every larger key is kept, and of the equal ones the first few
+// takes 27 us.)  Every larger key is kept, and of the equal ones the first few
 // in row order; rows come out ascending.  Bound by latency: one read of the
 // totals and five cluster barriers.
 //
@@ -24,9 +24,10 @@
 // others how many waves it has loaded.  The distance rows[i] - (dst + i) never
 // shrinks along the list, so beyond the first few waves of an eviction that
 // has long been the case and nobody waits.  Bound by the bytes moved.
-// 8 heads x 16384 of 32768 rows of 128: %MOVE_US%; with a cluster barrier for
-// each wave 166 us, and rows by bulk copies through shared memory, whatever the
-// buffers, 88 us at best: copies of a row or two are too small for them.
+// 8 heads x 16384 of 32768 rows of 128: 65 us (77 us without the streaming
+// hints); with a cluster barrier for each wave 166 us, and rows by bulk copies
+// through shared memory, whatever the buffers, 88 us at best: copies of a row
+// or two are too small for them.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2)
 #pragma unroll
         for (int u = 0; u < kMoveUnroll; ++u) {
             if (src[u] == a.dst + first + own + u * step) continue;
-            v[u] = base[(size_t)src[u] * pitch];
+            v[u] = __ldcs(&base[(size_t)src[u] * pitch]);
             go |= 1u << u;
         }
         float total[kMoveTotals] = {};
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2)
         if (stuck) continue;
 #pragma unroll
         for (int u = 0; u < kMoveUnroll; ++u)
-            if (go >> u & 1) base[(size_t)(a.dst + first + own + u * step) * pitch] = v[u];
+            if (go >> u & 1) __stcs(&base[(size_t)(a.dst + first + own + u * step) * pitch], v[u]);
         if (totals) {
 #pragma unroll
             for (int u = 0; u < (int)kMoveTotals; ++u) {

@@ -10,8 +10,8 @@
 // -inf, has no distribution, and its log probabilities and entropy are NaN.
 //
 // Bound by the one read of the logits.  A cluster of 1 to 16 CTAs owns a row
-// (more CTAs when there are few rows), each a contiguous range of it, 16
-// elements of a thread at a time with the next 16 already in flight:
+// (more CTAs when there are few rows), each a contiguous range of it in chunks
+// of 16 KB that arrive in two shared-memory stages by bulk copies:
 //   - (m, S0, S1) run per thread; a larger maximum m' rescales them,
 //     S1' = e^(m - m') (S1 + (m - m') S0);
 //   - alternatives are 64-bit keys (value, then lower id), unique in a row.  A
@@ -37,7 +37,9 @@ namespace cg = cooperative_groups;
 constexpr int kLpThreads = 256;
 constexpr int kLpVec = 4;                          // float4s of a thread per chunk
 constexpr uint32_t kLpChunk = kLpThreads * kLpVec;  // float4s of a CTA per chunk
+constexpr uint32_t kLpStages = 2;
 constexpr uint32_t kLpMaxCluster = 16;
+constexpr unsigned kErrLpWait = 1024u;
 constexpr uint32_t kLpGroups = kLpThreads / 2;
 constexpr uint32_t kLpCut = 128;  // collected keys that make a cut worth its barriers
 constexpr uint32_t kLpKeys = kLogprobMaxTop * 2 * kLpVec * 4 + kLpCut + kLogprobMaxTop;
@@ -46,6 +48,8 @@ static_assert(kLpGroups >= kLogprobMaxTop && kLpKeys >= kLpMaxCluster * kLogprob
 typedef unsigned long long u64;
 
 struct LpShared {
+    alignas(128) float4 stage[kLpStages][kLpChunk];
+    uint64_t full[kLpStages];
     u64 keys[kLpKeys];          // collected
     u64 best[kLogprobMaxTop];   // ranked
     u64 group[kLpGroups];
@@ -70,10 +74,35 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// e^d of d <= 0; 0 below -200.
-__device__ __forceinline__ float exp_neg(float d) {
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float ex2(float t) {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+    return r;
+}
+// e^d of d <= 0; 0 below -200.
+__device__ __forceinline__ float exp_neg(float d) { return ex2(d * kLog2e); }
+// a + b, a * b and a * b + c of two values at once.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+          "l"(reinterpret_cast<const uint64_t&>(c)));
     return r;
 }
 // (m, s0, s1) joined with another range's.
@@ -107,8 +136,10 @@ __device__ void lp_cut(LpShared& sh, uint32_t want) {
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(kLpThreads, 4) smallm_logprobs_kernel(const LogprobArgs a, uint32_t per_cta) {
-    __shared__ LpShared sh;
+__global__ void __launch_bounds__(kLpThreads, 4)
+    smallm_logprobs_kernel(const LogprobArgs a, uint32_t per_cta, unsigned int* err) {
+    extern __shared__ __align__(128) uint8_t lp_smem[];
+    LpShared& sh = *reinterpret_cast<LpShared*>(lp_smem);
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -117,35 +148,52 @@ __global__ void __launch_bounds__(kLpThreads, 4) smallm_logprobs_kernel(const Lo
     const uint32_t mis = (uint32_t)(reinterpret_cast<uintptr_t>(x) >> 2) & 3u;
     const uint32_t nq = (uint32_t)(((uint64_t)a.vocab + mis + 3) / 4);
     const uint32_t qb = min(nq, rank * per_cta), qe = min(nq, qb + per_cta);
-    auto load = [&](uint32_t q, float (&v)[4]) {
-        const uint32_t i = 4 * q - mis;  // wraps below the row's start
-        if (q < qe && i < a.vocab && i + 3 < a.vocab) {
-            *reinterpret_cast<float4*>(v) = __ldcs(reinterpret_cast<const float4*>(x - mis) + q);
+    // whole float4s of the row arrive by bulk copies; its ragged ends are read directly
+    const uint32_t whole_b = mis ? 1 : 0, whole_e = (uint32_t)(((uint64_t)a.vocab + mis) / 4);
+    auto whole = [&](uint32_t q0, uint32_t& b, uint32_t& e) {  // ... of the chunk from q0
+        b = max(q0, whole_b);
+        e = max(b, min(min(q0 + kLpChunk, qe), whole_e));
+    };
+    auto fetch = [&](uint32_t q0) {  // one thread
+        uint32_t b, e;
+        whole(q0, b, e);
+        const uint32_t s = (q0 - qb) / kLpChunk % kLpStages;
+        if (e > b) {
+            mbar_arrive_expect_tx(&sh.full[s], (e - b) * 16);
+            bulk_g2s(&sh.stage[s][b - q0], x - mis + 4ull * b, (e - b) * 16, &sh.full[s]);
         } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = q < qe && i + c < a.vocab ? x[i + c] : -INFINITY;
+            mbar_arrive(&sh.full[s]);
         }
     };
     if (tid == 0) {
+        for (uint32_t s = 0; s < kLpStages; ++s) mbar_init(&sh.full[s], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (uint32_t s = 0; s < kLpStages; ++s)
+            if (qb + s * kLpChunk < qe) fetch(qb + s * kLpChunk);
         sh.floor = 0;
         sh.count = 0;
         sh.n_best = 0;
     }
     float m = -INFINITY, s0 = 0.f, s1 = 0.f;
-    bool bad = false;
-    float next[kLpVec][4];
-#pragma unroll
-    for (int u = 0; u < kLpVec; ++u) load(qb + u * kLpThreads + tid, next[u]);
+    bool bad = false, ok = true;
     __syncthreads();
-    for (uint32_t q0 = qb; q0 < qe; q0 += kLpChunk) {
+    for (uint32_t q0 = qb, n = 0; q0 < qe; q0 += kLpChunk, ++n) {
+        const uint32_t s = n % kLpStages, parity = n / kLpStages & 1;
+        // (a second wait after one that gave up: no copy lands in a CTA that has left)
+        ok = (mbar_wait(&sh.full[s], parity) || (mbar_wait(&sh.full[s], parity), false)) && ok;
+        uint32_t wb, we;
+        whole(q0, wb, we);
         float v[kLpVec][4];
 #pragma unroll
-        for (int u = 0; u < kLpVec; ++u)
+        for (int u = 0; u < kLpVec; ++u) {
+            const uint32_t q = q0 + u * kLpThreads + tid;
+            if (q >= wb && q < we) {
+                *reinterpret_cast<float4*>(v[u]) = sh.stage[s][q - q0];
+            } else {
+                const uint32_t i = 4 * q - mis;  // wraps below the row's start
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[u][c] = next[u][c];
-        if (q0 + kLpChunk < qe) {
-#pragma unroll
-            for (int u = 0; u < kLpVec; ++u) load(q0 + kLpChunk + u * kLpThreads + tid, next[u]);
+                for (int c = 0; c < 4; ++c) v[u][c] = q < qe && i + c < a.vocab ? x[i + c] : -INFINITY;
+            }
         }
         float xm = v[0][0];
 #pragma unroll
@@ -160,18 +208,29 @@ __global__ void __launch_bounds__(kLpThreads, 4) smallm_logprobs_kernel(const Lo
             m = xm;
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        float c0 = 0.f, c1 = 0.f;
+        // (S1 in units of log2 until the end)
+        float2 c0 = make_float2(0.f, 0.f), c1 = c0;
+        const float2 less = make_float2(-ref, -ref), scale = make_float2(kLog2e, kLog2e);
 #pragma unroll
         for (int u = 0; u < kLpVec; ++u)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float d = fmaxf(v[u][c] - ref, -200.f), e = exp_neg(d);
-                c0 += e;
-                c1 = fmaf(e, d, c1);
+            for (int c = 0; c < 4; c += 2) {
+                float2 t = mul2(add2(make_float2(v[u][c], v[u][c + 1]), less), scale);
+                t.x = fmaxf(t.x, -300.f);
+                t.y = fmaxf(t.y, -300.f);
+                const float2 e = make_float2(ex2(t.x), ex2(t.y));
+                c0 = add2(c0, e);
+                c1 = fma2(e, t, c1);
             }
-        s0 += c0;
-        s1 += c1;
-        if (!a.n_top) continue;
+        s0 += c0.x + c0.y;
+        s1 += (c1.x + c1.y) * (1.f / kLog2e);
+        // the stage is free once every thread has its elements
+        const bool more = tid == 0 && q0 + kLpStages * kLpChunk < qe;
+        if (!a.n_top) {
+            __syncthreads();
+            if (more) fetch(q0 + kLpStages * kLpChunk);
+            continue;
+        }
         // ids of this thread's elements: first of float4 u, or past vocab
         auto id_of = [&](int u, int c) { return 4 * (q0 + u * kLpThreads + tid) - mis + c; };
         auto in_row = [&](int u, int c) {
@@ -180,6 +239,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) smallm_logprobs_kernel(const Lo
         u64 floor = sh.floor;
         const bool over = !(xm < INFINITY) || float_order_key(xm + 0.f) >= (uint32_t)(floor >> 32);
         const int n_over = __syncthreads_count(over);
+        if (more) fetch(q0 + kLpStages * kLpChunk);
         if (!n_over) continue;
         if (n_over > kLpThreads / 2) {
             u64 k = 0;
@@ -245,12 +305,21 @@ __global__ void __launch_bounds__(kLpThreads, 4) smallm_logprobs_kernel(const Lo
     if (C > 1) {
         cluster.sync();
         if (rank == 0) {
-            // own ranked keys stay at the front of keys; the others' follow
+            // own ranked keys stay at the front of keys; the others' follow, unless
+            // some range alone has n_top larger ones
             const uint32_t top = a.n_top;
+            u64 floor = (uint32_t)lane < C ? cluster.map_shared_rank(&sh, lane)->floor : 0ull;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) {
+                const u64 y = __shfl_xor_sync(0xffffffffu, floor, o);
+                floor = y > floor ? y : floor;
+            }
+            floor = __shfl_sync(0xffffffffu, floor, 0);
             for (uint32_t i = tid; i < (C - 1) * top; i += kLpThreads) {
                 const uint32_t r = 1 + i / top, j = i % top;
                 const LpShared* o = cluster.map_shared_rank(&sh, r);
-                if (j < o->n_best) sh.keys[atomicAdd(&sh.count, 1u)] = o->best[j];
+                const u64 k = j < o->n_best ? o->best[j] : 0ull;
+                if (k >= floor && k) sh.keys[atomicAdd(&sh.count, 1u)] = k;
             }
             if (tid == 0) {
                 for (uint32_t r = 1; r < C; ++r) {
@@ -266,10 +335,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) smallm_logprobs_kernel(const Lo
             if (top) lp_cut(sh, top);
         }
         cluster.sync();
-        if (rank) return;
+        if (rank) {
+            if (!ok) atomicOr(err, kErrLpWait);
+            return;
+        }
     } else {
         __syncthreads();
     }
+    if (!ok) atomicOr(err, kErrLpWait);
     const float nan = __int_as_float(0x7FC00000);
     const float M = sh.m, ls = sh.bad || M == -INFINITY ? nan : logf(sh.s0);
     if (tid == 0) {
@@ -302,9 +375,11 @@ void launch_logprobs(const LogprobArgs& a, cudaStream_t stream) {
     while (C < kLpMaxCluster && a.n_rows * C < 2 * sms && nq > C * kLpChunk) C *= 2;
     const void* fn = (const void*)smallm_logprobs_kernel;
     if (C > 8) SM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    set_smem_limit_once(fn, (int)sizeof(LpShared));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.n_rows * C);
     cfg.blockDim = dim3(kLpThreads);
+    cfg.dynamicSmemBytes = sizeof(LpShared);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -315,7 +390,8 @@ void launch_logprobs(const LogprobArgs& a, cudaStream_t stream) {
     cfg.numAttrs = 1;
     LogprobArgs aa = a;
     uint32_t per_cta = (nq + C - 1) / C;
-    void* args[] = {&aa, &per_cta};
+    unsigned int* err = device_error_flag();
+    void* args[] = {&aa, &per_cta, &err};
     SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
 }
 
