@@ -123,6 +123,7 @@ __device__ void lp_cut(LpShared& sh, uint32_t want) {
     for (uint32_t i = threadIdx.x; i < c; i += kLpThreads) {
         const u64 k = sh.keys[i];
         uint32_t rank = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < c; ++j) rank += sh.keys[j] > k;
         if (rank < want) sh.best[rank] = k;
     }
@@ -174,6 +175,9 @@ __global__ void __launch_bounds__(kLpThreads, 4)
         sh.count = 0;
         sh.n_best = 0;
     }
+    // (on its way before it is needed)
+    const uint32_t token = a.tokens && rank == 0 && tid == 0 ? a.tokens[row] : a.vocab;
+    const float given = token < a.vocab ? x[token] : 0.f;
     float m = -INFINITY, s0 = 0.f, s1 = 0.f;
     bool bad = false, ok = true;
     __syncthreads();
@@ -181,15 +185,14 @@ __global__ void __launch_bounds__(kLpThreads, 4)
         const uint32_t s = n % kLpStages, parity = n / kLpStages & 1;
         // (a second wait after one that gave up: no copy lands in a CTA that has left)
         ok = (mbar_wait(&sh.full[s], parity) || (mbar_wait(&sh.full[s], parity), false)) && ok;
-        uint32_t wb, we;
-        whole(q0, wb, we);
         float v[kLpVec][4];
 #pragma unroll
-        for (int u = 0; u < kLpVec; ++u) {
-            const uint32_t q = q0 + u * kLpThreads + tid;
-            if (q >= wb && q < we) {
-                *reinterpret_cast<float4*>(v[u]) = sh.stage[s][q - q0];
-            } else {
+        for (int u = 0; u < kLpVec; ++u) *reinterpret_cast<float4*>(v[u]) = sh.stage[s][u * kLpThreads + tid];
+        if (q0 < whole_b || q0 + kLpChunk > min(qe, whole_e)) {  // the row's ends
+#pragma unroll
+            for (int u = 0; u < kLpVec; ++u) {
+                const uint32_t q = q0 + u * kLpThreads + tid;
+                if (q >= whole_b && q < min(qe, whole_e)) continue;
                 const uint32_t i = 4 * q - mis;  // wraps below the row's start
 #pragma unroll
                 for (int c = 0; c < 4; ++c) v[u][c] = q < qe && i + c < a.vocab ? x[i + c] : -INFINITY;
@@ -255,31 +258,34 @@ __global__ void __launch_bounds__(kLpThreads, 4)
             k = other > k ? other : k;
             if (!(tid & 1)) sh.group[tid >> 1] = k;
             __syncthreads();
-            if (tid < (int)kLpGroups) {
-                const u64 mine = sh.group[tid];
-                uint32_t larger = 0;
-                const ulonglong2* gk = reinterpret_cast<const ulonglong2*>(sh.group);
+            // two threads for a group, half of the other groups each
+            const u64 mine = sh.group[tid >> 1];
+            uint32_t larger = 0;
+            const ulonglong2* gk = reinterpret_cast<const ulonglong2*>(sh.group) + (tid & 1) * (kLpGroups / 4);
 #pragma unroll 8
-                for (uint32_t j = 0; j < kLpGroups / 2; ++j) {
-                    const ulonglong2 y = gk[j];
-                    larger += (y.x > mine) + (y.y > mine);
-                }
-                if (mine && larger == a.n_top - 1 && mine - 1 > sh.floor) sh.floor = mine - 1;
+            for (uint32_t j = 0; j < kLpGroups / 4; ++j) {
+                const ulonglong2 y = gk[j];
+                larger += (y.x > mine) + (y.y > mine);
             }
+            larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+            if (!(tid & 1) && mine && larger == a.n_top - 1 && mine - 1 > sh.floor) sh.floor = mine - 1;
             __syncthreads();
             floor = sh.floor;
         }
         if (over) {
+            const float least = alt_value(floor);  // NaN (everything may count) where there is no floor yet
 #pragma unroll
             for (int u = 0; u < kLpVec; ++u)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
+                    if (v[u][c] < least) continue;
                     const u64 k = alt_key(v[u][c], id_of(u, c));
                     if (k > floor && in_row(u, c)) sh.keys[atomicAdd(&sh.count, 1u)] = k;
                 }
         }
         __syncthreads();
-        if (sh.count > kLpCut) lp_cut(sh, a.n_top);
+        // (a cut soon after the first chunks, while the floor still rises fast)
+        if (sh.count > min(kLpCut, a.n_top + max(4u, a.n_top / 2))) lp_cut(sh, a.n_top);
     }
     if (a.n_top) lp_cut(sh, a.n_top);
     // this CTA's (m, s0, s1)
@@ -321,15 +327,26 @@ __global__ void __launch_bounds__(kLpThreads, 4)
                 const u64 k = j < o->n_best ? o->best[j] : 0ull;
                 if (k >= floor && k) sh.keys[atomicAdd(&sh.count, 1u)] = k;
             }
-            if (tid == 0) {
-                for (uint32_t r = 1; r < C; ++r) {
-                    const LpShared* o = cluster.map_shared_rank(&sh, r);
-                    join(m, s0, s1, o->m, o->s0, o->s1);
-                    sh.bad |= o->bad;
+            if (warp == 0) {  // lane r: CTA r
+                const LpShared* o = cluster.map_shared_rank(&sh, (uint32_t)lane < C ? lane : 0);
+                m = o->m;
+                s0 = o->s0;
+                s1 = o->s1;
+                bad = (uint32_t)lane < C && o->bad;
+                if ((uint32_t)lane >= C) m = -INFINITY, s0 = s1 = 0.f;
+#pragma unroll
+                for (int d = 8; d > 0; d >>= 1) {
+                    const float om = __shfl_xor_sync(0xffffffffu, m, d), o0 = __shfl_xor_sync(0xffffffffu, s0, d),
+                                o1 = __shfl_xor_sync(0xffffffffu, s1, d);
+                    join(m, s0, s1, om, o0, o1);
                 }
-                sh.m = m;
-                sh.s0 = s0;
-                sh.s1 = s1;
+                bad = __any_sync(0xffffffffu, bad);
+                if (lane == 0) {
+                    sh.m = m;
+                    sh.s0 = s0;
+                    sh.s1 = s1;
+                    sh.bad = bad;
+                }
             }
             __syncthreads();
             if (top) lp_cut(sh, top);
@@ -347,10 +364,7 @@ __global__ void __launch_bounds__(kLpThreads, 4)
     const float M = sh.m, ls = sh.bad || M == -INFINITY ? nan : logf(sh.s0);
     if (tid == 0) {
         if (a.entropy) a.entropy[row] = ls - sh.s1 / sh.s0;
-        if (a.tokens) {
-            const uint32_t t = a.tokens[row];
-            a.logprob[row] = t < a.vocab ? (x[t] - M) - ls : nan;
-        }
+        if (a.tokens) a.logprob[row] = token < a.vocab ? (given - M) - ls : nan;
     }
     for (uint32_t i = tid; i < a.n_top; i += kLpThreads) {
         const u64 k = sh.best[i];
