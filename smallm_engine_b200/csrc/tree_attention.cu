@@ -27,11 +27,6 @@
 namespace smallm {
 namespace {
 
-constexpr uint32_t kTile = 32;       // keys per warp tile: one lane per key in the softmax
-constexpr int kVecRows = 8;          // rows per CTA
-constexpr int kVecWarps = 8;
-constexpr int kVecThreads = 32 * kVecWarps;
-
 struct TreeParams {
     TreeArgs a;
     uint32_t G, R, n, words;
@@ -45,186 +40,14 @@ struct TreeParams {
     unsigned int* err;   // the device error word
 };
 
-__device__ __forceinline__ bool tree_sees(const TreeParams& p, uint32_t t, uint32_t key) {
-    if (key < p.a.n_past) return true;
-    const uint32_t u = key - p.a.n_past;
-    if (u >= p.a.n_tokens) return false;
-    if (!p.a.mask) return u <= t;
-    return (p.a.mask[(size_t)t * p.words + (u >> 5)] >> (u & 31)) & 1u;
-}
-
-// Sum v[i] over the 8 lanes of a group; lane l8 of the group gets the sum of
-// row l8 (a reduce-scatter: 7 shuffles instead of 24).
-__device__ __forceinline__ float group_reduce8(float (&v)[8], int l8) {
-#pragma unroll
-    for (int w = 4; w >= 1; w >>= 1) {
-        const bool up = (l8 & w) != 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (i < w) {
-                const float keep = up ? v[i + w] : v[i];
-                const float send = up ? v[i] : v[i + w];
-                v[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
-            }
-        }
-    }
-    return v[0];
-}
-
-// Vector path: f32 FMAs, each warp runs its own online softmax over tiles of
-// 32 keys for the CTA's 8 rows; the warps' states are joined at the end.
-template <int HD>
-__global__ void __launch_bounds__(kVecThreads, 2) smallm_tree_vec_kernel(const TreeParams p) {
-    constexpr int DV = HD / 32;  // K float4s of a lane (8 lanes per key); V floats of a lane (32 lanes per key)
-    __shared__ __align__(16) float qs[kVecRows][HD];
-    __shared__ __align__(16) float ps[kVecWarps][kTile][kVecRows];
-    __shared__ __align__(16) float os[kVecWarps][kVecRows][HD];
-    __shared__ float wm[kVecWarps][kVecRows], wl[kVecWarps][kVecRows];
-    const TreeArgs& a = p.a;
-    const uint32_t split = blockIdx.x, g = blockIdx.y, r0 = blockIdx.z * kVecRows;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l8 = lane & 7, kl = lane >> 3;
-    for (int i = tid; i < kVecRows * HD; i += kVecThreads) {
-        const uint32_t r = r0 + i / HD;
-        qs[i / HD][i % HD] =
-            r < p.R ? a.q[(size_t)(r / p.G) * a.q_stride + ((size_t)g * p.G + r % p.G) * HD + i % HD] : 0.f;
-    }
-    __syncthreads();
-    float m[kVecRows], l[kVecRows], o[kVecRows][DV];
-#pragma unroll
-    for (int r = 0; r < kVecRows; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.f;
-#pragma unroll
-        for (int e = 0; e < DV; ++e) o[r][e] = 0.f;
-    }
-    const float* kb = a.kcache + (size_t)g * a.max_ctx * HD;
-    const float* vb = a.vcache + (size_t)g * a.max_ctx * HD;
-    const uint32_t tiles = (p.n + kTile - 1) / kTile;
-    const uint32_t t_end = min(tiles, (split + 1) * p.tiles_per_split);
-    for (uint32_t tile = split * p.tiles_per_split + warp; tile < t_end; tile += kVecWarps) {
-        const uint32_t base = tile * kTile;
-        // scores: 4 keys at a time, 8 lanes per key
-#pragma unroll 2
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t key = base + 4 * j + kl;
-            float4 kv[DV];
-#pragma unroll
-            for (int e = 0; e < DV; ++e)
-                kv[e] = key < p.n ? __ldg(reinterpret_cast<const float4*>(kb + (size_t)key * HD) + l8 + 8 * e)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-            float s[kVecRows];
-#pragma unroll
-            for (int r = 0; r < kVecRows; ++r) {
-                s[r] = 0.f;
-#pragma unroll
-                for (int e = 0; e < DV; ++e) {
-                    const float4 q4 = reinterpret_cast<const float4*>(qs[r])[l8 + 8 * e];
-                    s[r] = fmaf(q4.x, kv[e].x, s[r]);
-                    s[r] = fmaf(q4.y, kv[e].y, s[r]);
-                    s[r] = fmaf(q4.z, kv[e].z, s[r]);
-                    s[r] = fmaf(q4.w, kv[e].w, s[r]);
-                }
-            }
-            ps[warp][4 * j + kl][l8] = group_reduce8(s, l8);
-        }
-        __syncwarp();
-        // online softmax: lane = key
-        const uint32_t key = base + lane;
-        const bool mixed = base + kTile > a.n_past;  // the tile holds drafted rows or the end
-        float s[kVecRows];
-        *reinterpret_cast<float4*>(&s[0]) = *reinterpret_cast<const float4*>(&ps[warp][lane][0]);
-        *reinterpret_cast<float4*>(&s[4]) = *reinterpret_cast<const float4*>(&ps[warp][lane][4]);
-#pragma unroll
-        for (int r = 0; r < kVecRows; ++r) {
-            if (mixed && (r0 + r >= p.R || !tree_sees(p, (r0 + r) / p.G, key))) s[r] = -INFINITY;
-            if (p.scores && r0 + r < p.R && key < p.n)
-                p.scores[((size_t)g * p.R + r0 + r) * p.sc_stride + key] = s[r];
-            const float mt = warp_max(s[r]) * p.c;
-            const float mn = fmaxf(m[r], mt);
-            const float ref = mn == -INFINITY ? 0.f : mn;
-            const float e = exp2f(fmaf(s[r], p.c, -ref));
-            const float cf = exp2f(m[r] - ref);
-            m[r] = mn;
-            l[r] = fmaf(l[r], cf, e);
-            s[r] = e;
-#pragma unroll
-            for (int d = 0; d < DV; ++d) o[r][d] *= cf;
-        }
-        *reinterpret_cast<float4*>(&ps[warp][lane][0]) = *reinterpret_cast<const float4*>(&s[0]);
-        *reinterpret_cast<float4*>(&ps[warp][lane][4]) = *reinterpret_cast<const float4*>(&s[4]);
-        __syncwarp();
-        // o += p V: lane owns DV consecutive head dimensions
-#pragma unroll 4
-        for (int k = 0; k < (int)kTile; ++k) {
-            float v[DV];
-            const bool in = base + k < p.n;
-            const float* vr = vb + (size_t)(base + k) * HD + lane * DV;
-            if constexpr (DV == 4) {
-                const float4 x = in ? __ldg(reinterpret_cast<const float4*>(vr)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-            } else if constexpr (DV == 2) {
-                const float2 x = in ? __ldg(reinterpret_cast<const float2*>(vr)) : make_float2(0.f, 0.f);
-                v[0] = x.x, v[1] = x.y;
-            } else {
-                v[0] = in ? __ldg(vr) : 0.f;
-            }
-            float e[kVecRows];
-            *reinterpret_cast<float4*>(&e[0]) = *reinterpret_cast<const float4*>(&ps[warp][k][0]);
-            *reinterpret_cast<float4*>(&e[4]) = *reinterpret_cast<const float4*>(&ps[warp][k][4]);
-#pragma unroll
-            for (int r = 0; r < kVecRows; ++r)
-#pragma unroll
-                for (int d = 0; d < DV; ++d)
-                    // an unseen row may hold anything: 0 * inf must not reach o
-                    if (!mixed || e[r] != 0.f) o[r][d] = fmaf(e[r], v[d], o[r][d]);
-        }
-        __syncwarp();
-    }
-    // join the warps
-#pragma unroll
-    for (int r = 0; r < kVecRows; ++r) {
-        const float lt = warp_sum(l[r]);
-        if (lane == 0) {
-            wm[warp][r] = m[r];
-            wl[warp][r] = lt;
-        }
-#pragma unroll
-        for (int d = 0; d < DV; ++d) os[warp][r][lane * DV + d] = o[r][d];
-    }
-    __syncthreads();
-    for (int i = tid; i < kVecRows * HD; i += kVecThreads) {
-        const int rr = i / HD, d = i % HD;
-        const uint32_t r = r0 + rr;
-        if (r >= p.R) continue;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kVecWarps; ++w) M = fmaxf(M, wm[w][rr]);
-        const float ref = M == -INFINITY ? 0.f : M;
-        float L = 0.f, O = 0.f;
-#pragma unroll
-        for (int w = 0; w < kVecWarps; ++w) {
-            const float f = exp2f(wm[w][rr] - ref);
-            L = fmaf(f, wl[w][rr], L);
-            O = fmaf(f, os[w][rr][d], O);
-        }
-        const size_t row = (size_t)g * p.R + r;
-        if (p.n_split > 1) {
-            const size_t slot = (size_t)split * a.n_kv * p.R + row;
-            p.part_o[slot * HD + d] = O;
-            if (d == 0) p.part_ml[slot] = make_float2(M, L);
-        } else {
-            const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-            a.out[(size_t)(r / p.G) * a.out_stride + ((size_t)g * p.G + r % p.G) * HD + d] = O * inv;
-            if (d == 0 && p.scores) p.stats[row] = make_float2(ref, inv);
-        }
-    }
-}
-
-// ---- tensor-core path --------------------------------------------------------
+// ---- the kernel ----------------------------------------------------------------
 //
-// From about a dozen rows the vector path is bound by its FMAs (R / 2 flop per
-// byte of K and V), so blocks of 128 rows go to tcgen05, one CTA per SM, tiles
-// of 64 keys.  f32 operands enter as two f16 halves, x 2^e = hi + lo with |lo|
+// R rows need R / 2 flop per byte of K and V, more than the f32 units give from
+// a dozen rows on, so blocks of 128 rows go to tcgen05, one CTA per SM, tiles of
+// 64 keys.  (With fewer rows it is the copies that bound the kernel, and a form
+// in f32 FMAs, two CTAs per SM, was slower for one token of 32 heads at 128:
+// 55 us against 36 us over 16384 rows, 12 us against 10 us over 128.)  f32
+// operands enter as two f16 halves, x 2^e = hi + lo with |lo|
 // at most half a unit of hi: 22 bits, and three products (hi hi + hi lo +
 // lo hi) leave out 2^-24 of the operands' size.  e brings the largest
 // magnitude of the tile (K, V) or row (q) to [2^14, 2^15), so an element loses
@@ -232,8 +55,7 @@ __global__ void __launch_bounds__(kVecThreads, 2) smallm_tree_vec_kernel(const T
 //   - warps 25 (K) and 26 (V) copy f32 rows with bulk copies, half a tile at a
 //     time, into two halves each: 64 KB in flight while the tile before is
 //     converted.  (Loads through registers took the load/store unit twice as
-//     long as these copies and the reads of them, and 135 us where this form
-//     takes %TC_US% for 64 tokens x 32 heads over 32683 rows.)
+//     long as these copies and the reads of them.)
 //   - warps 8..15 (K) and 16..23 (V) convert: a group takes a tile into
 //     registers, finds its exponent and writes hi and lo in the MMA's swizzled
 //     layout, two slots for each of K and V;
@@ -372,7 +194,7 @@ __device__ __forceinline__ bool tc_copy(const float* src, uint32_t n, uint32_t t
     uint32_t last[2] = {0, 0};
     for (uint32_t i = 0; ok && i < 2 * nt; ++i) {
         const uint32_t t = i >> 1, h = i & 1, row = (t0 + t) * kTcKeys + h * (kTcKeys / 2);
-        ok = t == 0 || mbar_wait(&empty[h], (t - 1) & 1);
+        ok = t == 0 || mbar_wait_soon(&empty[h], (t - 1) & 1);
         if (!ok) break;
         const uint32_t rows = row < n ? min(n - row, kTcKeys / 2) : 0;
         if (rows) {
@@ -385,7 +207,7 @@ __device__ __forceinline__ bool tc_copy(const float* src, uint32_t n, uint32_t t
     }
     // no copy may still be landing when the CTA exits
     for (uint32_t h = 0; h < 2; ++h)
-        if (last[h]) ok = mbar_wait(&full[h], (last[h] - 1) & 1) && ok;
+        if (last[h]) ok = mbar_wait_soon(&full[h], (last[h] - 1) & 1) && ok;
     return ok;
 }
 
@@ -414,7 +236,7 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
         float m = 0.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            stuck = stuck || !mbar_wait(&sh.raw_full[GROUP][h], t & 1);
+            stuck = stuck || !mbar_wait_soon(&sh.raw_full[GROUP][h], t & 1);
 #pragma unroll
             for (int i = h * N / 2; i < (h + 1) * N / 2; ++i) {
                 x[i] = src[i * kConvThreads];
@@ -435,8 +257,8 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
         if (lane == 0) wmax[t & 1][cw] = mw;
         if (tid == 0) bads[ring] = 0;
         // (V's slots hold q until it is in tensor memory)
-        if (use > 0) stuck = stuck || !mbar_wait(&empty[slot], (use - 1) & 1);
-        else if (GROUP == 1 && t == 0) stuck = stuck || !mbar_wait(&sh.q_full, 0);
+        if (use > 0) stuck = stuck || !mbar_wait_soon(&empty[slot], (use - 1) & 1);
+        else if (GROUP == 1 && t == 0) stuck = stuck || !mbar_wait_soon(&sh.q_full, 0);
         if (conv_any(1 + GROUP, stuck)) return false;
         uint32_t mx = __reduce_max_sync(0xffffffffu, wmax[t & 1][lane % kConvWarps]);
         if (mx >= 0x7F800000u) {  // the same for the whole group: clean the tile
@@ -479,7 +301,7 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const TreeParams p) {
+__global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreeParams p) {
     using C = TcTree<HD>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -606,7 +428,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
         // o = o * corr + O of tile t
         auto take_output = [&](uint32_t t) {
             const uint32_t b = t & 1;
-            ok = ok && mbar_wait(&sh.o_full[b], (t >> 1) & 1);
+            ok = ok && mbar_wait_soon(&sh.o_full[b], (t >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             const float scale = sh.v_scale[t % kTcRing] * 0x1p-14f;
@@ -616,12 +438,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
                 for (int i = 0; i < OC / 2; ++i) o[i] = mul2(o[i], corr2);
             }
             const float2 scale2 = make_float2(scale, scale);
+            constexpr int OW = OC < 32 ? 16 : 32;
 #pragma unroll
-            for (int c = 0; c < OC; c += 16) {
-                uint32_t x[16];
-                tmem_ld16(lanes + C::o0 + b * 128 + half * OC + c, x);
+            for (int c = 0; c < OC; c += OW) {
+                uint32_t x[OW];
+                if constexpr (OW == 32) tmem_ld32(lanes + C::o0 + b * 128 + half * OC + c, x);
+                else tmem_ld16(lanes + C::o0 + b * 128 + half * OC + c, x);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < OW / 2; ++i)
                     o[c / 2 + i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2,
                                         o[c / 2 + i]);
             }
@@ -639,7 +463,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
         // end, since the two warps of a row meet at a barrier in it
         for (uint32_t t = 0; t < nt; ++t) {
             const uint32_t b = t & 1, key0 = (t0 + t) * kTcKeys, ring = t % kTcRing;
-            ok = ok && mbar_wait(&sh.s_full[b], (t >> 1) & 1);
+            ok = ok && mbar_wait_soon(&sh.s_full[b], (t >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             const uint32_t sp = lanes + C::s0 + b * kTcKeys;
@@ -748,7 +572,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
             // ---- MMA issuer: the whole warp walks the loop, one lane issues
             uint32_t leader;
             asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
-            auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+            auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_soon(bar, parity)); };
             ok = wait(&sh.q_full, 0);
             tc_fence_after();
             auto scores = [&](uint32_t t) -> bool {
@@ -804,7 +628,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_tc_kernel(const Tre
             // tensor memory is freed only after every MMA has completed
             if (leader) mma_commit(&sh.done);
             __syncwarp();
-            ok = mbar_wait(&sh.done, 0) && ok;
+            ok = mbar_wait_soon(&sh.done, 0) && ok;
         } else if (lane == 0 && warp == 25) {
             ok = tc_copy<HD>(a.kcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, raw, sh.raw_full[0], sh.raw_empty[0]);
         } else if (lane == 0 && warp == 26) {
@@ -907,15 +731,10 @@ __global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(
     p.a.weights[(size_t)g * p.a.max_ctx + k] += sum;
 }
 
-#ifndef SMALLM_TREE_TC_ROWS
-#define SMALLM_TREE_TC_ROWS 9u
-#endif
-
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // Split of the keys and the workspace's layout, from sizes alone.
 struct TreePlan {
-    bool tc;
     uint32_t n_split, tiles_per_split, sc_stride;
     size_t off_ml, off_scores, off_stats, bytes;
 };
@@ -923,14 +742,9 @@ struct TreePlan {
 TreePlan tree_plan(uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t n_past, uint32_t n_tokens, bool weights) {
     TreePlan t{};
     const uint32_t R = n_tokens * (n_heads / n_kv), n = n_past + n_tokens;
-    t.tc = R >= SMALLM_TREE_TC_ROWS;
-    const uint32_t keys = t.tc ? kTcKeys : kTile, rows_cta = t.tc ? kTcRows : kVecRows;
-    const uint32_t blocks = n_kv * ((R + rows_cta - 1) / rows_cta), tiles = (n + keys - 1) / keys;
-    // one CTA per SM in all on the tensor path, else two; no split below a
-    // tile for each warp of a vector CTA
-    const uint32_t want = std::max(1u, (t.tc ? 1 : 2) * (uint32_t)device_sm_count() / blocks);
-    const uint32_t most = t.tc ? tiles : (tiles + kVecWarps - 1) / kVecWarps;
-    t.n_split = std::min(want, most);
+    const uint32_t blocks = n_kv * ((R + kTcRows - 1) / kTcRows), tiles = (n + kTcKeys - 1) / kTcKeys;
+    // one CTA per SM in all; two tiles cost a CTA less than the joining kernel
+    t.n_split = tiles <= 2 ? 1 : std::min(std::max(1u, (uint32_t)device_sm_count() / blocks), tiles);
     t.tiles_per_split = (tiles + t.n_split - 1) / t.n_split;
     t.n_split = (tiles + t.tiles_per_split - 1) / t.tiles_per_split;
     const size_t rows = (size_t)n_kv * R;
@@ -959,15 +773,10 @@ void tree_check_shape(uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t n_p
 }
 
 template <int HD>
-void launch_tree(const TreeParams& p, bool tc, cudaStream_t stream) {
-    if (tc) {
-        set_smem_limit_once((const void*)smallm_tree_tc_kernel<HD>, (int)TcTree<HD>::smem);
-        const dim3 grid((p.R + kTcRows - 1) / kTcRows, p.n_split, p.a.n_kv);
-        smallm_tree_tc_kernel<HD><<<grid, kTcThreads, TcTree<HD>::smem, stream>>>(p);
-    } else {
-        const dim3 grid(p.n_split, p.a.n_kv, (p.R + kVecRows - 1) / kVecRows);
-        smallm_tree_vec_kernel<HD><<<grid, kVecThreads, 0, stream>>>(p);
-    }
+void launch_tree(const TreeParams& p, cudaStream_t stream) {
+    set_smem_limit_once((const void*)smallm_tree_kernel<HD>, (int)TcTree<HD>::smem);
+    const dim3 grid((p.R + kTcRows - 1) / kTcRows, p.n_split, p.a.n_kv);
+    smallm_tree_kernel<HD><<<grid, kTcThreads, TcTree<HD>::smem, stream>>>(p);
     SM_CUDA(cudaGetLastError());
     if (p.n_split > 1) {
         TreeParams pp = p;
@@ -1028,9 +837,9 @@ void launch_attention_tree(const TreeArgs& a, void* work, size_t work_bytes, cud
     p.part_ml = reinterpret_cast<float2*>(w + t.off_ml);
     p.scores = a.weights ? reinterpret_cast<float*>(w + t.off_scores) : nullptr;
     p.stats = a.weights ? reinterpret_cast<float2*>(w + t.off_stats) : nullptr;
-    if (a.hd == 32) launch_tree<32>(p, t.tc, stream);
-    else if (a.hd == 64) launch_tree<64>(p, t.tc, stream);
-    else launch_tree<128>(p, t.tc, stream);
+    if (a.hd == 32) launch_tree<32>(p, stream);
+    else if (a.hd == 64) launch_tree<64>(p, stream);
+    else launch_tree<128>(p, stream);
 }
 
 }  // namespace smallm
