@@ -31,11 +31,11 @@ struct TreeParams {
     TreeArgs a;
     uint32_t G, R, n, words;
     uint32_t n_split, tiles_per_split;
-    uint32_t sc_stride;  // floats between two rows of stored scores
+    uint32_t sc_rows;    // stored scores of a key: R, padded
     float c;             // log2(e) / sqrt(hd)
     float* part_o;       // [n_split][n_kv * R][hd]
     float2* part_ml;     // [n_split][n_kv * R] (mc, sum)
-    float* scores;       // [n_kv * R][sc_stride], raw q . K, -inf where unseen
+    float* scores;       // [n_kv][n][sc_rows], raw q . K, -inf where unseen
     float2* stats;       // [n_kv * R] (mc of the whole row, 1 / sum or 0)
     unsigned int* err;   // the device error word
 };
@@ -315,6 +315,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
     const uint32_t tiles = (p.n + kTcKeys - 1) / kTcKeys;
     const uint32_t t0 = split * p.tiles_per_split, nt = min(tiles, t0 + p.tiles_per_split) - t0;
 
+    pdl_launch_dependents();  // the joining kernel's launch overlaps this one
     const uint32_t quads = min(4u, (p.R - r0 + 31) / 32);  // warps' row quarters that hold rows
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kTcSlots; ++i) {
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
 #pragma unroll
         for (int i = 0; i < OC / 2; ++i) o[i] = make_float2(0.f, 0.f);
         float m = -INFINITY, l = 0.f, corr = 1.f;
-        float* sc = p.scores && valid ? p.scores + ((size_t)g * p.R + r) * p.sc_stride + half * SC : nullptr;
+        float* sc = p.scores && valid ? p.scores + ((size_t)g * p.n + half * SC) * p.sc_rows + r : nullptr;
         // o = o * corr + O of tile t
         auto take_output = [&](uint32_t t) {
             const uint32_t b = t & 1;
@@ -486,12 +487,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                     else if ((hurt >> i) & 1) s[i] = __uint_as_float(0x7FC00000u);
                 }
             }
-            if (sc) {
-#pragma unroll
-                for (int i = 0; i < SC; i += 4)
-                    *reinterpret_cast<float4*>(sc + key0 + i) =
-                        make_float4(s[i] * raw, s[i + 1] * raw, s[i + 2] * raw, s[i + 3] * raw);
-            }
             float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
             for (int i = 4; i < SC; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
@@ -526,6 +521,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.p_full[b]);
+            if (sc) {  // the lanes' rows are neighbours
+                float* at = sc + (size_t)key0 * p.sc_rows;
+                const uint32_t left = p.n - key0 - min(p.n - key0, half * (uint32_t)SC);
+                if (left >= SC) {
+#pragma unroll
+                    for (int i = 0; i < SC; ++i) at[i * p.sc_rows] = s[i] * raw;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < SC; ++i)
+                        if (i < left) at[i * p.sc_rows] = s[i] * raw;
+                }
+            }
             if (t) take_output(t - 1);
             corr = corr_t;
         }
@@ -698,44 +705,52 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
     if (c == 0 && p.scores) p.stats[row] = make_float2(ref, inv);
 }
 
-// weights[g][k] += sum_r 2^(s c - mc_r) / sum_r.  A CTA per (128 keys, KV head);
-// a lane has four keys, warp w the rows w, w + 8, ...; the warps' sums meet in
-// shared memory in their order, so the total does not depend on the launch.
-constexpr int kWeightKeys = 128, kWeightWarps = 8;
+// weights[g][k] += sum_r 2^(s c - mc_r) / sum_r.  L lanes (a power of two, the
+// stored rows of a key up to 32) have the rows of a key, each lane 16 keys at a
+// time; the lanes' sums meet in a fixed order, so the total does not depend on
+// the launch.
+constexpr int kWeightKeys = 16, kWeightWarps = 8;
+template <int L>
 __global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(const TreeParams p) {
-    __shared__ float4 part[kWeightWarps][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t key = blockIdx.x * kWeightKeys + 4 * lane, g = blockIdx.y;
+    constexpr uint32_t KW = 32 / L;  // keys side by side in a warp
+    const uint32_t lane = threadIdx.x & 31, g = blockIdx.y;
+    const uint32_t key = (blockIdx.x * kWeightWarps + (threadIdx.x >> 5)) * kWeightKeys * KW + lane / L;
     pdl_wait();
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (key < p.sc_stride) {
-        const float* s = p.scores + (size_t)g * p.R * p.sc_stride + key;
-#pragma unroll 8
-        for (uint32_t r = warp; r < p.R; r += kWeightWarps) {
-            const float2 st = p.stats[(size_t)g * p.R + r];
-            const float4 v = *reinterpret_cast<const float4*>(s + (size_t)r * p.sc_stride);
-            acc.x = fmaf(exp2f(fmaf(v.x, p.c, -st.x)), st.y, acc.x);
-            acc.y = fmaf(exp2f(fmaf(v.y, p.c, -st.x)), st.y, acc.y);
-            acc.z = fmaf(exp2f(fmaf(v.z, p.c, -st.x)), st.y, acc.z);
-            acc.w = fmaf(exp2f(fmaf(v.w, p.c, -st.x)), st.y, acc.w);
-        }
-    }
-    part[warp][lane] = acc;
-    __syncthreads();
-    // (the scores behind the last key are not written: those sums are dropped here)
-    const uint32_t k = blockIdx.x * kWeightKeys + threadIdx.x;
-    if (threadIdx.x >= kWeightKeys || k >= p.n) return;
-    float sum = 0.f;
+    float acc[kWeightKeys];
 #pragma unroll
-    for (int w = 0; w < kWeightWarps; ++w) sum += reinterpret_cast<const float*>(part[w])[threadIdx.x];
-    p.a.weights[(size_t)g * p.a.max_ctx + k] += sum;
+    for (int k = 0; k < kWeightKeys; ++k) acc[k] = 0.f;
+    // (loads without conditions, so that all are in flight: past the last key
+    // they read it again and the sum is dropped)
+    float* w = p.a.weights + (size_t)g * p.a.max_ctx;
+    const float* s = p.scores + (size_t)g * p.n * p.sc_rows;
+    float old[kWeightKeys];
+#pragma unroll
+    for (int k = 0; k < kWeightKeys; ++k) old[k] = w[min(key + k * KW, p.n - 1)];
+    for (uint32_t r = lane % L; r < p.R; r += L) {
+        const float2 st = p.stats[(size_t)g * p.R + r];
+        float v[kWeightKeys];
+#pragma unroll
+        for (int k = 0; k < kWeightKeys; ++k) v[k] = __ldg(s + (size_t)min(key + k * KW, p.n - 1) * p.sc_rows + r);
+#pragma unroll
+        for (int k = 0; k < kWeightKeys; ++k) acc[k] = fmaf(exp2f(fmaf(v[k], p.c, -st.x)), st.y, acc[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kWeightKeys; ++k) {
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], o);
+    }
+    if (lane % L == 0) {
+#pragma unroll
+        for (int k = 0; k < kWeightKeys; ++k)
+            if (key + k * KW < p.n) w[key + k * KW] = old[k] + acc[k];
+    }
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // Split of the keys and the workspace's layout, from sizes alone.
 struct TreePlan {
-    uint32_t n_split, tiles_per_split, sc_stride;
+    uint32_t n_split, tiles_per_split, sc_rows;
     size_t off_ml, off_scores, off_stats, bytes;
 };
 
@@ -752,8 +767,10 @@ TreePlan tree_plan(uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t n_past
     t.off_ml = at;
     if (t.n_split > 1) at += align256(8 * rows * t.n_split);
     t.off_scores = at;
-    t.sc_stride = (n + 63) / 64 * 64;
-    if (weights) at += align256(4 * rows * t.sc_stride);
+    t.sc_rows = 1;
+    while (t.sc_rows < std::min(R, 32u)) t.sc_rows *= 2;
+    if (R > 32) t.sc_rows = (R + 31) / 32 * 32;
+    if (weights) at += align256(4 * (size_t)n_kv * n * t.sc_rows);
     t.off_stats = at;
     if (weights) at += align256(8 * rows);
     t.bytes = at;
@@ -787,9 +804,14 @@ void launch_tree(const TreeParams& p, cudaStream_t stream) {
     if (p.a.weights) {
         TreeParams pp = p;
         void* args[] = {&pp};
-        launch_kernel_ex((const void*)smallm_tree_weights_kernel,
-                         dim3((p.n + kWeightKeys - 1) / kWeightKeys, p.a.n_kv), dim3(32 * kWeightWarps), 0, stream, true,
-                         args);
+        const uint32_t lanes = std::min(32u, p.sc_rows), keys = kWeightWarps * kWeightKeys * (32 / lanes);
+        const void* fn = lanes == 32   ? (const void*)smallm_tree_weights_kernel<32>
+                         : lanes == 16 ? (const void*)smallm_tree_weights_kernel<16>
+                         : lanes == 8  ? (const void*)smallm_tree_weights_kernel<8>
+                         : lanes == 4  ? (const void*)smallm_tree_weights_kernel<4>
+                         : lanes == 2  ? (const void*)smallm_tree_weights_kernel<2>
+                                       : (const void*)smallm_tree_weights_kernel<1>;
+        launch_kernel_ex(fn, dim3((p.n + keys - 1) / keys, p.a.n_kv), dim3(32 * kWeightWarps), 0, stream, true, args);
     }
 }
 
@@ -829,7 +851,7 @@ void launch_attention_tree(const TreeArgs& a, void* work, size_t work_bytes, cud
     p.words = (a.n_tokens + 31) / 32;
     p.n_split = t.n_split;
     p.tiles_per_split = t.tiles_per_split;
-    p.sc_stride = t.sc_stride;
+    p.sc_rows = t.sc_rows;
     p.c = (float)(1.4426950408889634 / sqrt((double)a.hd));
     p.err = device_error_flag();
     uint8_t* w = static_cast<uint8_t*>(work);
