@@ -185,17 +185,19 @@ __device__ __forceinline__ unsigned long long tc_seen(const uint32_t* mask, uint
     return m;
 }
 
-// One lane: tiles t0 .. t0 + nt - 1 of `src` (rows below n) into the two raw halves.
+// One lane: tiles from .. to - 1 of a CTA's tiles t0 .. (rows of `src` below n)
+// into the two raw halves.
 template <int HD>
-__device__ __forceinline__ bool tc_copy(const float* src, uint32_t n, uint32_t t0, uint32_t nt, uint8_t* raw,
-                                        uint64_t* full, uint64_t* empty) {
+__device__ __forceinline__ bool tc_copy(const float* src, uint32_t n, uint32_t t0, uint32_t from, uint32_t to,
+                                        uint8_t* raw, uint64_t* full, uint64_t* empty) {
     using C = TcTree<HD>;
-    bool ok = true;
-    uint32_t last[2] = {0, 0};
-    for (uint32_t i = 0; ok && i < 2 * nt; ++i) {
+    for (uint32_t i = 2 * from; i < 2 * to; ++i) {
         const uint32_t t = i >> 1, h = i & 1, row = (t0 + t) * kTcKeys + h * (kTcKeys / 2);
-        ok = t == 0 || mbar_wait_soon(&empty[h], (t - 1) & 1);
-        if (!ok) break;
+        if (t && !mbar_wait_soon(&empty[h], (t - 1) & 1)) {
+            // no copy may still be landing when the CTA exits
+            for (uint32_t j = 0; j < 2; ++j) mbar_wait(&full[j], (t - (j >= h)) & 1);
+            return false;
+        }
         const uint32_t rows = row < n ? min(n - row, kTcKeys / 2) : 0;
         if (rows) {
             mbar_arrive_expect_tx(&full[h], rows * HD * 4);
@@ -203,12 +205,8 @@ __device__ __forceinline__ bool tc_copy(const float* src, uint32_t n, uint32_t t
         } else {
             mbar_arrive(&full[h]);
         }
-        last[h] = t + 1;
     }
-    // no copy may still be landing when the CTA exits
-    for (uint32_t h = 0; h < 2; ++h)
-        if (last[h]) ok = mbar_wait_soon(&full[h], (last[h] - 1) & 1) && ok;
-    return ok;
+    return true;
 }
 
 // One converter group: tiles t0 .. t0 + nt - 1 from the raw halves into `slots`.
@@ -324,10 +322,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             mbar_init(&sh.v_full[i], kConvWarps);
             mbar_init(&sh.v_empty[i], 1);
         }
-        for (uint32_t i = 0; i < 4; ++i) {
-            mbar_init(&sh.raw_full[i >> 1][i & 1], 1);
-            mbar_init(&sh.raw_empty[i >> 1][i & 1], kConvWarps);
-        }
         for (uint32_t b = 0; b < 2; ++b) {
             mbar_init(&sh.s_full[b], 2);   // the MMA's commit and the issuing thread
             mbar_init(&sh.p_full[b], 2 * quads);
@@ -337,6 +331,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         mbar_init(&sh.q_full, 2 * quads);
         mbar_init(&sh.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // the first tile's rows are on their way while the CTA is set up
+    // (copying warps: 25 K, 26 V)
+    if (warp - 25 < 2 && lane == 0) {
+        const uint32_t op = warp - 25;
+        const float* rows_src = (op ? a.vcache : a.kcache) + (size_t)g * a.max_ctx * HD;
+        for (uint32_t h = 0; h < 2; ++h) {
+            mbar_init(&sh.raw_full[op][h], 1);
+            mbar_init(&sh.raw_empty[op][h], kConvWarps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tc_copy<HD>(rows_src, p.n, t0, 0, 1, raw + op * 2 * C::raw, sh.raw_full[op], sh.raw_empty[op]);
     }
     if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
@@ -361,11 +367,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         {
             // q: the eight warps read 16 rows each, and their largest magnitudes,
             // into V's slots; then each row is scaled and split by its two threads
+            // (rows past the last stay as they are: nothing of them is written)
             constexpr int QL = HD / 32;
             float* stage = reinterpret_cast<float*>(vs);
             uint32_t tt = (r0 + warp * 16) / p.G, hh = (r0 + warp * 16) % p.G;
 #pragma unroll 1
-            for (uint32_t b = warp * 16; b < warp * 16 + 16; b += 8) {
+            for (uint32_t b = warp * 16; b < warp * 16 + 16 && r0 + b < p.R; b += 8) {
                 alignas(16) float x[8][QL];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -636,11 +643,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             if (leader) mma_commit(&sh.done);
             __syncwarp();
             ok = mbar_wait_soon(&sh.done, 0) && ok;
-        } else if (lane == 0 && warp == 25) {
-            ok = tc_copy<HD>(a.kcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, raw, sh.raw_full[0], sh.raw_empty[0]);
-        } else if (lane == 0 && warp == 26) {
-            ok = tc_copy<HD>(a.vcache + (size_t)g * a.max_ctx * HD, p.n, t0, nt, raw + 2 * C::raw, sh.raw_full[1],
-                             sh.raw_empty[1]);
+        } else if (warp < 27 && lane == 0) {
+            const uint32_t op = warp - 25;
+            const float* rows_src = (op ? a.vcache : a.kcache) + (size_t)g * a.max_ctx * HD;
+            ok = tc_copy<HD>(rows_src, p.n, t0, 1, nt, raw + op * 2 * C::raw, sh.raw_full[op], sh.raw_empty[op]);
+            for (uint32_t h = 0; ok && h < 2; ++h) ok = mbar_wait_soon(&sh.raw_full[op][h], (nt - 1) & 1);
         }
     }
     if (!ok) atomicOr(p.err, kErrTreeWait);
