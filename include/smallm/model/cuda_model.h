@@ -110,6 +110,23 @@ public:
         return ids;
     }
 
+    // Beyond the reference's Model: log probabilities under the last step's
+    // logits, computed on the device: of `token`, the distribution's entropy,
+    // and the n_top (at most 64) most likely tokens, largest first.
+    struct Logprobs {
+        float logprob = 0.f, entropy = 0.f;
+        std::vector<uint32_t> top_ids;
+        std::vector<float> top_logprobs;
+    };
+    Logprobs logprobs(uint32_t token, uint32_t n_top = 0) {
+        Logprobs r;
+        r.top_ids.resize(n_top);
+        r.top_logprobs.resize(n_top);
+        check(smallm_model_logprobs(m_, token, &r.logprob, &r.entropy, n_top, r.top_ids.data(),
+                                    r.top_logprobs.data()));
+        return r;
+    }
+
     smallm_model* handle() const { return m_; }
 
 private:

@@ -397,6 +397,15 @@ int smallm_model_prefill(smallm_model* m, const uint32_t* tokens, uint32_t n, ui
 int smallm_model_sample(smallm_model* m, uint32_t kind, uint32_t k, float p, float temperature, float u,
                         uint32_t* token);
 
+/* Log probabilities under the last step's logits, computed on the device
+ * (smallm_logprobs): of `token` into *logprob (NULL: not wanted, token
+ * ignored), the distribution's entropy into *entropy (may be NULL) and the
+ * n_top most likely tokens into top_ids / top_logprobs (host, n_top <= 64 and
+ * <= vocab; 0: both may be NULL).  Under tensor parallelism every rank calls
+ * it (the vocabulary shards are gathered first). */
+int smallm_model_logprobs(smallm_model* m, uint32_t token, float* logprob, float* entropy, uint32_t n_top,
+                          uint32_t* top_ids, float* top_logprobs);
+
 /* Device address of the last step's logits (f32[vocab] on this rank's
  * device; this rank's vocabulary shard under tensor parallelism), valid
  * until the next step is enqueued. */

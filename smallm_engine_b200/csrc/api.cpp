@@ -490,6 +490,15 @@ int smallm_model_sample(smallm_model* m, uint32_t kind, uint32_t k, float p, flo
     });
 }
 
+int smallm_model_logprobs(smallm_model* m, uint32_t token, float* logprob, float* entropy, uint32_t n_top,
+                          uint32_t* top_ids, float* top_logprobs) {
+    return guard([&] {
+        need(m && (!n_top || (top_ids && top_logprobs)), "NULL argument");
+        set_dev(m->m.device);
+        m->m.logprobs(token, logprob, entropy, n_top, top_ids, top_logprobs);
+    });
+}
+
 int smallm_qmatrix_dequantize(smallm_ctx* ctx, const smallm_qmatrix* W, float* y_dev, void* stream) {
     return guard([&] {
         need(ctx && W && y_dev, "NULL argument");

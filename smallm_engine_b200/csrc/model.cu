@@ -788,6 +788,41 @@ uint32_t Model::sample(uint32_t kind, uint32_t k, float p, float temperature, fl
     return tok;
 }
 
+void Model::logprobs(uint32_t token, float* logprob, float* entropy, uint32_t n_top, uint32_t* top_ids,
+                     float* top_logprobs) {
+    if (logprob && token >= vocab) throw Error(SMALLM_ERR_INVALID, "token id out of range");
+    if (n_top > kLogprobMaxTop || n_top > vocab)
+        throw Error(SMALLM_ERR_RANGE, "logprobs: at most 64 alternatives, and no more than the vocabulary");
+    constexpr uint32_t kHead = 4;
+    if (!lp_scratch) lp_scratch = static_cast<uint32_t*>(dalloc(4 * (kHead + 2 * kLogprobMaxTop)));
+    if (tp_size > 1)
+        nccl_check(ncclAllGather(logits_local, logits, vocab_l, ncclFloat32, comm, stream), "ncclAllGather");
+    LogprobArgs a{};
+    a.logits = logits;
+    a.n_rows = 1;
+    a.vocab = a.stride = vocab;
+    float* out = reinterpret_cast<float*>(lp_scratch);
+    if (logprob) {
+        SM_CUDA(cudaMemcpyAsync(lp_scratch, &token, 4, cudaMemcpyHostToDevice, stream));
+        a.tokens = lp_scratch;
+        a.logprob = out + 1;
+    }
+    a.entropy = out + 2;
+    a.n_top = n_top;
+    a.top_ids = lp_scratch + kHead;
+    a.top_logprobs = out + kHead + n_top;
+    launch_logprobs(a, stream);
+    uint32_t host[kHead + 2 * kLogprobMaxTop];
+    SM_CUDA(cudaMemcpyAsync(host, lp_scratch, 4 * (kHead + 2 * n_top), cudaMemcpyDeviceToHost, stream));
+    SM_CUDA(cudaStreamSynchronize(stream));
+    if (logprob) std::memcpy(logprob, host + 1, 4);
+    if (entropy) std::memcpy(entropy, host + 2, 4);
+    if (n_top) {
+        std::memcpy(top_ids, host + kHead, 4 * n_top);
+        std::memcpy(top_logprobs, host + kHead + n_top, 4 * n_top);
+    }
+}
+
 void Model::decode_ids(uint32_t* out, uint32_t n) {
     if (n > pending_steps) throw Error(1, "fewer decode steps were run than ids requested");
     SM_CUDA(cudaMemcpyAsync(out, ids, 4ull * n, cudaMemcpyDeviceToHost, stream));

@@ -40,6 +40,16 @@ class ModelConfig:
     step_launches: int = 0
 
 
+@dataclass
+class TokenLogprobs:
+    """A token's log probability in the distribution it was taken from, that
+    distribution's entropy and its most likely tokens (id, log probability)."""
+    token: int | None
+    logprob: float | None
+    entropy: float
+    top: list[tuple[int, float]]
+
+
 class CudaModel:
     def __init__(self, path, device: int = 0, max_ctx: int = 0, tp_rank: int = 0, tp_size: int = 1,
                  nccl_id: bytes | None = None):
@@ -114,6 +124,19 @@ class CudaModel:
         check(lib().smallm_model_prefill(self.h, toks.ctypes.data, toks.size, int(start_pos),
                                          out.ctypes.data if want_logits else None, ctypes.byref(am), 0))
         return out, int(am.value)
+
+    def logprobs(self, token: int | None = None, top: int = 0) -> "TokenLogprobs":
+        """Log probabilities under the last step's logits
+        (smallm_model_logprobs): of `token` (None: not wanted), the
+        distribution's entropy and the `top` (at most 64) most likely tokens."""
+        lp, ent = ctypes.c_float(), ctypes.c_float()
+        ids = np.empty(top, dtype=np.uint32)
+        lps = np.empty(top, dtype=np.float32)
+        check(lib().smallm_model_logprobs(self.h, 0 if token is None else int(token),
+                                          None if token is None else ctypes.byref(lp), ctypes.byref(ent), int(top),
+                                          ids.ctypes.data, lps.ctypes.data))
+        return TokenLogprobs(None if token is None else int(token), None if token is None else lp.value, ent.value,
+                             [(int(i), float(p)) for i, p in zip(ids, lps)])
 
     def logits_device_ptr(self) -> int:
         return lib().smallm_model_logits_device(self.h) or 0
@@ -271,8 +294,13 @@ class Generator:
     this backend): prefix reuse against the previous call, one forward per
     new prompt token, then sample / forward until max_new or EOS."""
 
-    def __init__(self, model: CudaModel, sampler, eos_id: int = -1, batched_prefill: bool = True):
+    def __init__(self, model: CudaModel, sampler, eos_id: int = -1, batched_prefill: bool = True,
+                 logprobs: int | None = None):
         self.model, self.sampler, self.eos = model, sampler, eos_id
+        # not None: self.logprobs holds a TokenLogprobs with this many
+        # alternatives for each token that generate() returned
+        self.n_logprobs = logprobs
+        self.logprobs: list[TokenLogprobs] = []
         # the prompt in one pass per layer (smallm_model_prefill) instead of
         # one forward per token; single GPU only
         self.batched_prefill = batched_prefill and model.config().n_layers > 0
@@ -309,6 +337,7 @@ class Generator:
                 self.stats.prefill_tokens += 1
         self.stats.prefill_ms = (time.perf_counter() - t0) * 1e3
         out: list[int] = []
+        self.logprobs = []
         generated = list(tokens)
         t0 = time.perf_counter()
         for _ in range(max_new_tokens):
@@ -317,6 +346,8 @@ class Generator:
                 break
             out.append(nxt)
             generated.append(nxt)
+            if self.n_logprobs is not None:
+                self.logprobs.append(self.model.logprobs(nxt, self.n_logprobs))
             logits = self.model.forward(nxt, pos, want_logits=not on_device)
             pos += 1
             self.stats.generated_tokens += 1
