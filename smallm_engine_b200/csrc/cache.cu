@@ -10,7 +10,7 @@
 // summed over the cluster's shared memory, then the bin that holds the rank.
 // (Digits of 11, 11 and 10 bits save a barrier, but then every CTA reads 8 KB
 // from each of 15 others for each digit: 37 us for 8 x 131072 keys where this
-// takes 27 us.)  Every larger key is kept, and of the equal ones the first few
+// takes 23 us.)  Every larger key is kept, and of the equal ones the first few
 // in row order; rows come out ascending.  Bound by latency: one read of the
 // totals and five cluster barriers.
 //
@@ -92,19 +92,19 @@ __global__ void __launch_bounds__(kSelThreads, 2)
         const uint32_t bins = pass == 0 ? 512u : (pass == 3 ? 128u : 256u);
         const uint32_t high = pass == 0 ? 0u : ~(bins * (1u << shift) - 1u);
         uint32_t* hist = sh.hist[pass];
-        for (uint32_t i = tid; i - lane < len; i += kSelThreads) {
-            const uint32_t key = i < len ? key_of(i) : 0u;
-            const bool in = i < len && (key & high) == prefix;
-            const uint32_t bin = key >> shift & (bins - 1);
-            const uint32_t act = __ballot_sync(0xffffffffu, in);
-            if (!act) continue;
-            // a warp whose keys share a bin (like totals) counts once
-            const uint32_t lead = __shfl_sync(0xffffffffu, bin, __ffs(act) - 1);
-            if (__all_sync(0xffffffffu, !in || bin == lead)) {
-                if (lane == 0) atomicAdd(&hist[lead], __popc(act));
-            } else if (in) {
-                atomicAdd(&hist[bin], 1u);
+        // (four keys of a lane at a time; plain shared-memory adds, even where all
+        // keys share a bin: counting a warp's equal bins first cost more)
+        for (uint32_t i0 = tid; i0 - lane < len; i0 += 4 * kSelThreads) {
+            uint32_t bin[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t i = i0 + j * kSelThreads;
+                const uint32_t key = key_of(min(i, len - 1));
+                bin[j] = i < len && (key & high) == prefix ? key >> shift & (bins - 1) : kSelBins;
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (bin[j] != kSelBins) atomicAdd(&hist[bin[j]], 1u);
         }
         if (C > 1) cluster.sync();
         else __syncthreads();
@@ -114,14 +114,21 @@ __global__ void __launch_bounds__(kSelThreads, 2)
         if (4u * tid < bins) {
             own = *reinterpret_cast<const uint4*>(&hist[top]);
             sum = own;
-            // all peers' reads in flight at once
+            // the peers' reads in flight together (past the last one the loads
+            // repeat it and are dropped)
+            for (uint32_t r = 1; r < C; r += 5) {
+                uint4 v[5];
 #pragma unroll
-            for (uint32_t r = 1; r < kSelMaxCluster; ++r)
-                if (r < C) {
-                    const uint32_t peer = cr + r < C ? cr + r : cr + r - C;
-                    const uint4 v = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&hist[top], peer));
-                    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+                for (uint32_t j = 0; j < 5; ++j) {
+                    const uint32_t d = cr + min(r + j, C - 1), peer = d < C ? d : d - C;
+                    v[j] = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&hist[top], peer));
                 }
+#pragma unroll
+                for (uint32_t j = 0; j < 5; ++j) {
+                    const uint32_t on = r + j < C ? 0xFFFFFFFFu : 0u;
+                    sum.x += v[j].x & on, sum.y += v[j].y & on, sum.z += v[j].z & on, sum.w += v[j].w & on;
+                }
+            }
         }
         // inclusive scan from the top: keys in these bins or above, of the head and of this CTA
         const uint32_t all = sum.x + sum.y + sum.z + sum.w, mine = own.x + own.y + own.z + own.w;

@@ -42,6 +42,7 @@ constexpr uint32_t kLpMaxCluster = 16;
 constexpr unsigned kErrLpWait = 1024u;
 constexpr uint32_t kLpGroups = kLpThreads / 2;
 constexpr uint32_t kLpCut = 128;  // collected keys that make a cut worth its barriers
+constexpr uint32_t kLpLists = (kLpMaxCluster - 1) * kLogprobMaxTop / kLpThreads + 1;  // joined keys of a thread
 constexpr uint32_t kLpKeys = kLogprobMaxTop * 2 * kLpVec * 4 + kLpCut + kLogprobMaxTop;
 static_assert(kLpGroups >= kLogprobMaxTop && kLpKeys >= kLpMaxCluster * kLogprobMaxTop, "key buffer");
 
@@ -54,7 +55,7 @@ struct LpShared {
     u64 best[kLogprobMaxTop];   // ranked
     u64 group[kLpGroups];
     u64 floor;                  // only larger keys matter
-    uint32_t count, n_best;
+    uint32_t count;
     float m, s0, s1;
     uint32_t bad;
     float wm[kLpThreads / 32], w0[kLpThreads / 32], w1[kLpThreads / 32];
@@ -131,7 +132,7 @@ __device__ void lp_cut(LpShared& sh, uint32_t want) {
     const uint32_t n = min(c, want);
     if (threadIdx.x < n) sh.keys[threadIdx.x] = sh.best[threadIdx.x];
     if (threadIdx.x == 0) {
-        sh.count = sh.n_best = n;
+        sh.count = n;
         if (n == want && sh.best[n - 1] > sh.floor) sh.floor = sh.best[n - 1];
     }
     __syncthreads();
@@ -166,6 +167,7 @@ __global__ void __launch_bounds__(kLpThreads, 4)
             mbar_arrive(&sh.full[s]);
         }
     };
+    if (tid < (int)kLogprobMaxTop) sh.best[tid] = 0;
     if (tid == 0) {
         for (uint32_t s = 0; s < kLpStages; ++s) mbar_init(&sh.full[s], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -173,7 +175,6 @@ __global__ void __launch_bounds__(kLpThreads, 4)
             if (qb + s * kLpChunk < qe) fetch(qb + s * kLpChunk);
         sh.floor = 0;
         sh.count = 0;
-        sh.n_best = 0;
     }
     // (on its way before it is needed)
     const uint32_t token = a.tokens && rank == 0 && tid == 0 ? a.tokens[row] : a.vocab;
@@ -246,14 +247,24 @@ __global__ void __launch_bounds__(kLpThreads, 4)
         if (!n_over) continue;
         if (n_over > kLpThreads / 2) {
             u64 k = 0;
+            if (xm < INFINITY && xm > -INFINITY) {  // the first place of the maximum
+                uint32_t id = 0;
 #pragma unroll
-            for (int u = 0; u < kLpVec; ++u)
+                for (int u = kLpVec - 1; u >= 0; --u)
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (in_row(u, c)) {
-                        const u64 y = alt_key(v[u][c], id_of(u, c));
-                        k = y > k ? y : k;
-                    }
+                    for (int c = 3; c >= 0; --c)
+                        if (v[u][c] == xm) id = id_of(u, c);
+                k = alt_key(xm, id);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < kLpVec; ++u)
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c)
+                        if (in_row(u, c)) {
+                            const u64 y = alt_key(x[id_of(u, c)], id_of(u, c));
+                            k = y > k ? y : k;
+                        }
+            }
             const u64 other = __shfl_xor_sync(0xffffffffu, k, 1);
             k = other > k ? other : k;
             if (!(tid & 1)) sh.group[tid >> 1] = k;
@@ -311,22 +322,26 @@ __global__ void __launch_bounds__(kLpThreads, 4)
     if (C > 1) {
         cluster.sync();
         if (rank == 0) {
-            // own ranked keys stay at the front of keys; the others' follow, unless
-            // some range alone has n_top larger ones
-            const uint32_t top = a.n_top;
-            u64 floor = (uint32_t)lane < C ? cluster.map_shared_rank(&sh, lane)->floor : 0ull;
+            // Own ranked keys stay at the front of keys; the others' follow.  Where
+            // m ranges have d keys each at or above a key and m d >= n_top, smaller
+            // ones do not matter: the m-th largest of the ranges' d-th keys.
+            const uint32_t top = a.n_top, d = min(top, max((top + C - 1) / C, 5u)), need = (top + d - 1) / max(d, 1u);
+            u64 list[kLpLists];
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) {
-                const u64 y = __shfl_xor_sync(0xffffffffu, floor, o);
-                floor = y > floor ? y : floor;
+            for (int j = 0; j < (int)kLpLists; ++j) {
+                const uint32_t i = min(tid + j * kLpThreads, (C - 1) * top), r = i / max(top, 1u) + 1;
+                list[j] = *cluster.map_shared_rank(&sh.best[i % max(top, 1u)], min(r, C - 1));
             }
-            floor = __shfl_sync(0xffffffffu, floor, 0);
-            for (uint32_t i = tid; i < (C - 1) * top; i += kLpThreads) {
-                const uint32_t r = 1 + i / top, j = i % top;
-                const LpShared* o = cluster.map_shared_rank(&sh, r);
-                const u64 k = j < o->n_best ? o->best[j] : 0ull;
-                if (k >= floor && k) sh.keys[atomicAdd(&sh.count, 1u)] = k;
-            }
+            u64 least = (uint32_t)lane < C && top ? *cluster.map_shared_rank(&sh.best[d - 1], lane) : 0ull;
+            uint32_t larger = 0;
+#pragma unroll
+            for (int r = 0; r < (int)kLpMaxCluster; ++r) larger += __shfl_sync(0xffffffffu, least, r) > least;
+            const uint32_t at = __ballot_sync(0xffffffffu, (uint32_t)lane < C && least && larger == need - 1);
+            const u64 bound = at ? __shfl_sync(0xffffffffu, least, __ffs(at) - 1) : 0ull;
+#pragma unroll
+            for (int j = 0; j < (int)kLpLists; ++j)
+                if (tid + j * kLpThreads < (C - 1) * top && list[j] && list[j] >= bound)
+                    sh.keys[atomicAdd(&sh.count, 1u)] = list[j];
             if (warp == 0) {  // lane r: CTA r
                 const LpShared* o = cluster.map_shared_rank(&sh, (uint32_t)lane < C ? lane : 0);
                 m = o->m;
