@@ -31,11 +31,12 @@ struct TreeParams {
     TreeArgs a;
     uint32_t G, R, n, words;
     uint32_t n_split, tiles_per_split;
-    uint32_t sc_rows;    // stored scores of a key: R, padded
+    uint32_t sc_rows;    // stored scores of a key: R, padded; 0: they run along keys
+    uint32_t sc_keys;    // ... and of a row: n, padded
     float c;             // log2(e) / sqrt(hd)
     float* part_o;       // [n_split][n_kv * R][hd]
     float2* part_ml;     // [n_split][n_kv * R] (mc, sum)
-    float* scores;       // [n_kv][n][sc_rows], raw q . K, -inf where unseen
+    float* scores;       // [n_kv][n][sc_rows] or [n_kv][R][sc_keys], raw q . K, -inf where unseen
     float2* stats;       // [n_kv * R] (mc of the whole row, 1 / sum or 0)
     unsigned int* err;   // the device error word
 };
@@ -161,11 +162,18 @@ __device__ __forceinline__ float ex2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float max_abs_nan(float a, float b) {
+// The largest of three magnitudes, NaN if any is; of three values.
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     float r;
-    asm("{\n .reg .f32 t;\n abs.f32 t, %2;\n max.NaN.f32 %0, %1, t;\n}" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Bits of the 64 keys from key0 that row token t sees.
 __device__ __forceinline__ unsigned long long tc_seen(const uint32_t* mask, uint32_t n_past, uint32_t n_tokens,
                                                    uint32_t t, uint32_t key0) {
@@ -246,7 +254,7 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
             }
 #pragma unroll
             for (int i = h * N / 2; i < (h + 1) * N / 2; ++i) {
-                m = max_abs_nan(max_abs_nan(max_abs_nan(max_abs_nan(m, x[i].x), x[i].y), x[i].z), x[i].w);
+                m = max3_abs_nan(max3_abs_nan(m, x[i].x, x[i].y), x[i].z, x[i].w);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.raw_empty[GROUP][h]);
@@ -298,7 +306,9 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
     return true;
 }
 
-template <int HD>
+// SCORES: the scores are stored, for the totals, along the keys (1: few rows) or
+// along the rows (2).
+template <int HD, int SCORES>
 __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreeParams p) {
     using C = TcTree<HD>;
     extern __shared__ uint8_t smem_raw[];
@@ -432,7 +442,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
 #pragma unroll
         for (int i = 0; i < OC / 2; ++i) o[i] = make_float2(0.f, 0.f);
         float m = -INFINITY, l = 0.f, corr = 1.f;
-        float* sc = p.scores && valid ? p.scores + ((size_t)g * p.n + half * SC) * p.sc_rows + r : nullptr;
+        float* sc = nullptr;
+        if constexpr (SCORES == 1) sc = p.scores + ((size_t)g * p.R + r) * p.sc_keys + half * SC;
+        if constexpr (SCORES == 2) sc = p.scores + ((size_t)g * p.n + half * SC) * p.sc_rows + r;
         // o = o * corr + O of tile t
         auto take_output = [&](uint32_t t) {
             const uint32_t b = t & 1;
@@ -475,6 +487,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             const uint32_t sp = lanes + C::s0 + b * kTcKeys;
+            const float k_scale = sh.k_scale[ring];
+            const unsigned long long bad = sh.k_bad[ring];
             float s[SC];
             {
                 uint32_t x[32];
@@ -483,8 +497,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                 for (int i = 0; i < SC; ++i) s[i] = __uint_as_float(x[i]);
             }
             // (never 0: an unseen key's -inf times it stays -inf)
-            const float raw = fmaxf(qinv * sh.k_scale[ring], 0x1p-120f);
-            const unsigned long long bad = sh.k_bad[ring];
+            const float raw = fmaxf(qinv * k_scale, 0x1p-120f);
             if (key0 + kTcKeys > a.n_past || bad) {
                 const uint32_t seen = (uint32_t)(tc_seen(a.mask, a.n_past, a.n_tokens, tok, key0) >> (half * SC));
                 const uint32_t hurt = (uint32_t)(bad >> (half * SC));
@@ -492,6 +505,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                 for (int i = 0; i < SC; ++i) {
                     if (!((seen >> i) & 1)) s[i] = -INFINITY;
                     else if ((hurt >> i) & 1) s[i] = __uint_as_float(0x7FC00000u);
+                }
+            }
+            if (SCORES == 1 && valid) {
+#pragma unroll
+                for (int i = 0; i < SC; i += 4)
+                    *reinterpret_cast<float4*>(sc + key0 + i) =
+                        make_float4(s[i] * raw, s[i + 1] * raw, s[i + 2] * raw, s[i + 3] * raw);
+            }
+            if (SCORES == 2 && valid) {  // the lanes' rows are neighbours
+                float* at = sc + (size_t)key0 * p.sc_rows;
+                const uint32_t left = p.n - key0 - min(p.n - key0, half * (uint32_t)SC);
+                if (left >= SC) {
+#pragma unroll
+                    for (int i = 0; i < SC; ++i) at[i * p.sc_rows] = s[i] * raw;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < SC; ++i)
+                        if (i < left) at[i * p.sc_rows] = s[i] * raw;
                 }
             }
             float mx[4] = {s[0], s[1], s[2], s[3]};
@@ -528,18 +559,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.p_full[b]);
-            if (sc) {  // the lanes' rows are neighbours
-                float* at = sc + (size_t)key0 * p.sc_rows;
-                const uint32_t left = p.n - key0 - min(p.n - key0, half * (uint32_t)SC);
-                if (left >= SC) {
-#pragma unroll
-                    for (int i = 0; i < SC; ++i) at[i * p.sc_rows] = s[i] * raw;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < SC; ++i)
-                        if (i < left) at[i * p.sc_rows] = s[i] * raw;
-                }
-            }
             if (t) take_output(t - 1);
             corr = corr_t;
         }
@@ -553,7 +572,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             if (half == 0 && valid) p.part_ml[(size_t)split * a.n_kv * p.R + row] = make_float2(m, l);
         } else {
             f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-            if (half == 0 && valid && p.scores) p.stats[row] = make_float2(m == -INFINITY ? 0.f : m, f);
+            if (SCORES && half == 0 && valid) p.stats[row] = make_float2(m == -INFINITY ? 0.f : m, f);
         }
         // rows leave through K's slots (every MMA has completed), so that the
         // stores run along rows
@@ -712,16 +731,31 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
     if (c == 0 && p.scores) p.stats[row] = make_float2(ref, inv);
 }
 
-// weights[g][k] += sum_r 2^(s c - mc_r) / sum_r.  L lanes (a power of two, the
-// stored rows of a key up to 32) have the rows of a key, each lane 16 keys at a
-// time; the lanes' sums meet in a fixed order, so the total does not depend on
-// the launch.
+// weights[g][k] += sum_r 2^(s c - mc_r) / sum_r, in a fixed order, so that the
+// total does not depend on the launch.  Scores of up to kFewRows rows run along
+// the keys: a lane has a key and walks the rows.  More rows run along
+// themselves: the lanes of a warp have a key's rows, 16 keys at a time, and
+// their sums meet by shuffles.
 constexpr int kWeightKeys = 16, kWeightWarps = 8;
-template <int L>
+constexpr uint32_t kFewRows = 16;
+__global__ void __launch_bounds__(256) smallm_tree_weights_few_kernel(const TreeParams p) {
+    const uint32_t key = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y;
+    pdl_wait();
+    if (key >= p.n) return;
+    float* w = p.a.weights + (size_t)g * p.a.max_ctx + key;
+    const float* s = p.scores + (size_t)g * p.R * p.sc_keys + key;
+    const float old = *w;
+    float acc = 0.f;
+#pragma unroll 8
+    for (uint32_t r = 0; r < p.R; ++r) {
+        const float2 st = p.stats[(size_t)g * p.R + r];
+        acc = fmaf(exp2f(fmaf(__ldg(s + (size_t)r * p.sc_keys), p.c, -st.x)), st.y, acc);
+    }
+    *w = old + acc;
+}
 __global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(const TreeParams p) {
-    constexpr uint32_t KW = 32 / L;  // keys side by side in a warp
     const uint32_t lane = threadIdx.x & 31, g = blockIdx.y;
-    const uint32_t key = (blockIdx.x * kWeightWarps + (threadIdx.x >> 5)) * kWeightKeys * KW + lane / L;
+    const uint32_t key = (blockIdx.x * kWeightWarps + (threadIdx.x >> 5)) * kWeightKeys;
     pdl_wait();
     float acc[kWeightKeys];
 #pragma unroll
@@ -730,34 +764,29 @@ __global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(
     // they read it again and the sum is dropped)
     float* w = p.a.weights + (size_t)g * p.a.max_ctx;
     const float* s = p.scores + (size_t)g * p.n * p.sc_rows;
-    float old[kWeightKeys];
-#pragma unroll
-    for (int k = 0; k < kWeightKeys; ++k) old[k] = w[min(key + k * KW, p.n - 1)];
-    for (uint32_t r = lane % L; r < p.R; r += L) {
+    const float old = w[min(key + lane % kWeightKeys, p.n - 1)];
+    for (uint32_t r = lane; r < p.R; r += 32) {
         const float2 st = p.stats[(size_t)g * p.R + r];
         float v[kWeightKeys];
 #pragma unroll
-        for (int k = 0; k < kWeightKeys; ++k) v[k] = __ldg(s + (size_t)min(key + k * KW, p.n - 1) * p.sc_rows + r);
+        for (int k = 0; k < kWeightKeys; ++k) v[k] = __ldg(s + (size_t)min(key + k, p.n - 1) * p.sc_rows + r);
 #pragma unroll
         for (int k = 0; k < kWeightKeys; ++k) acc[k] = fmaf(exp2f(fmaf(v[k], p.c, -st.x)), st.y, acc[k]);
     }
+    float mine = 0.f;  // lane k: key k
 #pragma unroll
     for (int k = 0; k < kWeightKeys; ++k) {
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], o);
+        const float sum = warp_sum(acc[k]);
+        if (lane == (uint32_t)k) mine = sum;
     }
-    if (lane % L == 0) {
-#pragma unroll
-        for (int k = 0; k < kWeightKeys; ++k)
-            if (key + k * KW < p.n) w[key + k * KW] = old[k] + acc[k];
-    }
+    if (lane < kWeightKeys && key + lane < p.n) w[key + lane] = old + mine;
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // Split of the keys and the workspace's layout, from sizes alone.
 struct TreePlan {
-    uint32_t n_split, tiles_per_split, sc_rows;
+    uint32_t n_split, tiles_per_split, sc_rows, sc_keys;
     size_t off_ml, off_scores, off_stats, bytes;
 };
 
@@ -774,10 +803,9 @@ TreePlan tree_plan(uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t n_past
     t.off_ml = at;
     if (t.n_split > 1) at += align256(8 * rows * t.n_split);
     t.off_scores = at;
-    t.sc_rows = 1;
-    while (t.sc_rows < std::min(R, 32u)) t.sc_rows *= 2;
-    if (R > 32) t.sc_rows = (R + 31) / 32 * 32;
-    if (weights) at += align256(4 * (size_t)n_kv * n * t.sc_rows);
+    t.sc_rows = R > kFewRows ? (R + 31) / 32 * 32 : 0;
+    t.sc_keys = tiles * kTcKeys;
+    if (weights) at += align256(4 * (size_t)n_kv * (t.sc_rows ? (size_t)n * t.sc_rows : (size_t)R * t.sc_keys));
     t.off_stats = at;
     if (weights) at += align256(8 * rows);
     t.bytes = at;
@@ -798,27 +826,22 @@ void tree_check_shape(uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t n_p
 
 template <int HD>
 void launch_tree(const TreeParams& p, cudaStream_t stream) {
-    set_smem_limit_once((const void*)smallm_tree_kernel<HD>, (int)TcTree<HD>::smem);
+    const void* fn = !p.scores   ? (const void*)smallm_tree_kernel<HD, 0>
+                     : p.sc_rows ? (const void*)smallm_tree_kernel<HD, 2>
+                                 : (const void*)smallm_tree_kernel<HD, 1>;
+    set_smem_limit_once(fn, (int)TcTree<HD>::smem);
     const dim3 grid((p.R + kTcRows - 1) / kTcRows, p.n_split, p.a.n_kv);
-    smallm_tree_kernel<HD><<<grid, kTcThreads, TcTree<HD>::smem, stream>>>(p);
-    SM_CUDA(cudaGetLastError());
+    TreeParams pp = p;
+    void* args[] = {&pp};
+    launch_kernel_ex(fn, grid, dim3(kTcThreads), TcTree<HD>::smem, stream, false, args);
     if (p.n_split > 1) {
-        TreeParams pp = p;
-        void* args[] = {&pp};
         launch_kernel_ex((const void*)smallm_tree_merge_kernel<HD>, dim3(p.a.n_kv * p.R), dim3(kMergeThreads), 0,
                          stream, true, args);
     }
     if (p.a.weights) {
-        TreeParams pp = p;
-        void* args[] = {&pp};
-        const uint32_t lanes = std::min(32u, p.sc_rows), keys = kWeightWarps * kWeightKeys * (32 / lanes);
-        const void* fn = lanes == 32   ? (const void*)smallm_tree_weights_kernel<32>
-                         : lanes == 16 ? (const void*)smallm_tree_weights_kernel<16>
-                         : lanes == 8  ? (const void*)smallm_tree_weights_kernel<8>
-                         : lanes == 4  ? (const void*)smallm_tree_weights_kernel<4>
-                         : lanes == 2  ? (const void*)smallm_tree_weights_kernel<2>
-                                       : (const void*)smallm_tree_weights_kernel<1>;
-        launch_kernel_ex(fn, dim3((p.n + keys - 1) / keys, p.a.n_kv), dim3(32 * kWeightWarps), 0, stream, true, args);
+        const void* sum = p.sc_rows ? (const void*)smallm_tree_weights_kernel : (const void*)smallm_tree_weights_few_kernel;
+        const uint32_t keys = p.sc_rows ? kWeightWarps * kWeightKeys : 256;
+        launch_kernel_ex(sum, dim3((p.n + keys - 1) / keys, p.a.n_kv), dim3(256), 0, stream, true, args);
     }
 }
 
@@ -859,6 +882,7 @@ void launch_attention_tree(const TreeArgs& a, void* work, size_t work_bytes, cud
     p.n_split = t.n_split;
     p.tiles_per_split = t.tiles_per_split;
     p.sc_rows = t.sc_rows;
+    p.sc_keys = t.sc_keys;
     p.c = (float)(1.4426950408889634 / sqrt((double)a.hd));
     p.err = device_error_flag();
     uint8_t* w = static_cast<uint8_t*>(work);
