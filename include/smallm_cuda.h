@@ -167,7 +167,8 @@ int smallm_gemv_residual_sum(smallm_ctx* ctx, const smallm_qmatrix* W, const flo
  * kernels raise when they give up (0 = none): bit 0 a GEMV producer's stage
  * wait, bits 1-2 a GEMV or attention pipeline wait, bit 3 a residual part's
  * arrival flag, bit 5 the decode position changed during a step, bit 6 a wait
- * of the tensor-core GEMM, bit 7 a bad row list (smallm_cache_move).  Waits for
+ * of the tensor-core GEMM, bit 7 a bad row list (smallm_cache_move), bits 8-10
+ * a wait of smallm_attention_tree, smallm_cache_move or smallm_logprobs.  Waits for
  * the device; clear != 0 resets the word. */
 int smallm_ctx_device_errors(smallm_ctx* ctx, uint32_t* flags, int clear);
 

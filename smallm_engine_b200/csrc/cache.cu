@@ -12,7 +12,7 @@
 // from each of 15 others for each digit: 37 us for 8 x 131072 keys where this
 // takes 23 us.)  Every larger key is kept, and of the equal ones the first few
 // in row order; rows come out ascending.  Bound by latency: one read of the
-// totals and five cluster barriers.
+// totals, five cluster barriers and as many rounds of remote reads.
 //
 // move: row dst + i of K and V (and the totals) becomes row rows[i], for a
 // strictly ascending list with rows[i] >= dst + i.  In place: a cluster owns a
@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(kSelThreads, 2)
     const uint32_t b0 = min(m, cr * per_cta), len = min(m, b0 + per_cta) - b0;
     const float* w = weights + (size_t)head * stride + n_first + b0;
     uint32_t* out = rows + (size_t)head * n_keep;
+    pdl_wait();
     if (cr == 0) {
         for (uint32_t i = tid; i < n_first; i += kSelThreads) out[i] = i;
         for (uint32_t i = tid; i < n_last; i += kSelThreads) out[n_first + k + i] = n - n_last + i;
@@ -246,6 +247,7 @@ __device__ __forceinline__ void move_rows(V* base, uint32_t width, const MoveArg
 __global__ void __launch_bounds__(kMoveThreads, 1)
     smallm_cache_move_short_kernel(float* kc, float* vc, float* totals, uint32_t hd, MoveArgs a, uint32_t list_stride) {
     a.rows += (size_t)blockIdx.y * list_stride;
+    pdl_wait();
     if (blockIdx.z == 2) {
         move_rows<float>(totals + (size_t)blockIdx.y * a.max_ctx, 1, a);
     } else {
@@ -282,6 +284,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2)
     a.rows += (size_t)blockIdx.y * list_stride;
     const uint32_t per = kMoveWave / slice, wave = per * C;  // rows of a CTA and of the cluster in a wave
     const uint32_t waves = (a.n_rows + wave - 1) / wave;
+    pdl_wait();
     for (uint32_t w = tid; w < min(waves, kMoveStarts); w += kMoveThreads) start[w] = __ldg(a.rows + w * wave);
     if (tid < kMoveMaxCluster) loaded[tid] = 0;
     if (tid == 0) stuck = 0;
@@ -368,13 +371,15 @@ void launch_cluster(const void* fn, dim3 grid, uint32_t threads, size_t smem, ui
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = C;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
 }
 
@@ -443,7 +448,7 @@ void launch_cache_move(float* kcache, float* vcache, float* weights, uint32_t n_
     if ((uint64_t)n_rows * hd / 4 <= kMoveWave) {
         void* args[] = {&kcache, &vcache, &weights, &hd, &a, &stride};
         launch_kernel_ex((const void*)smallm_cache_move_short_kernel, dim3(1, n_kv, weights ? 3 : 2),
-                         dim3(kMoveThreads), 0, stream, false, args);
+                         dim3(kMoveThreads), 0, stream, true, args);
         return;
     }
     // CTAs of a cluster: a wave's part each at least; then slices of columns (64

