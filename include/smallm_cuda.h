@@ -168,8 +168,8 @@ int smallm_gemv_residual_sum(smallm_ctx* ctx, const smallm_qmatrix* W, const flo
  * wait, bits 1-2 a GEMV or attention pipeline wait, bit 3 a residual part's
  * arrival flag, bit 5 the decode position changed during a step, bit 6 a wait
  * of the tensor-core GEMM, bit 7 a bad row list (smallm_cache_move), bits 8-10
- * a wait of smallm_attention_tree, smallm_cache_move or smallm_logprobs.  Waits for
- * the device; clear != 0 resets the word. */
+ * a wait of smallm_attention_tree, smallm_cache_move or smallm_logprobs.
+ * Waits for the device; clear != 0 resets the word. */
 int smallm_ctx_device_errors(smallm_ctx* ctx, uint32_t* flags, int clear);
 
 /* Dequantize the matrix from its device layout into y_dev[rows * cols]
@@ -271,7 +271,7 @@ int smallm_attention_tree_workspace(smallm_ctx* ctx, uint32_t n_heads, uint32_t 
  * n_keep - n_first - n_last with the largest totals (equal totals: the lower
  * row; NaN counts as less than everything).  rows_dev [n_kv_heads][n_keep]
  * receives them in ascending order.  weights_dev is [n_kv_heads][max_ctx].
- * n_first + n_last <= n_keep <= n <= max_ctx. */
+ * n_first + n_last <= n_keep <= n <= max_ctx, n <= 2^30, n_kv_heads <= 65535. */
 int smallm_cache_select(smallm_ctx* ctx, const float* weights_dev, uint32_t n_kv_heads, uint32_t max_ctx, uint32_t n,
                         uint32_t n_keep, uint32_t n_first, uint32_t n_last, uint32_t* rows_dev, void* stream);
 
@@ -281,7 +281,9 @@ int smallm_cache_select(smallm_ctx* ctx, const float* weights_dev, uint32_t n_kv
  * tree), or with per_head != 0 [n_kv_heads][n_rows] (what smallm_cache_select
  * kept).  A list is strictly ascending with rows[i] >= dst + i.  weights_dev,
  * unless NULL, is [n_kv_heads][max_ctx] and moves along.  Keys keep the
- * rotary position they were stored with.
+ * rotary position they were stored with.  head_dim 32, 64 or 128; kcache_dev
+ * and vcache_dev are 16-byte aligned; dst + n_rows <= max_ctx, n_rows <= 2^30,
+ * n_kv_heads <= 65535.
  * An entry that breaks the rules, or names a row at max_ctx or above, raises
  * bit 7 of the device error word; nothing outside the caches is touched, but
  * the rows from dst on then hold unspecified rows of the cache. */
@@ -299,7 +301,8 @@ int smallm_cache_move(smallm_ctx* ctx, float* kcache_dev, float* vcache_dev, flo
  *                   (n_top <= 64 and <= vocab; 0: both may be NULL)
  * A logit of -inf has probability 0.  A row that holds NaN or +inf, or nothing
  * above -inf, has no distribution: its log probabilities and entropy are NaN,
- * and its alternatives are still ordered (NaN logits last). */
+ * and its alternatives are still ordered (NaN logits last).  vocab <= 2^30,
+ * n_rows <= 2^26. */
 int smallm_logprobs(smallm_ctx* ctx, const float* logits_dev, uint32_t n_rows, uint32_t vocab, uint32_t stride,
                     const uint32_t* tokens_dev, float* logprob_dev, float* entropy_dev, uint32_t n_top,
                     uint32_t* top_ids_dev, float* top_logprobs_dev, void* stream);

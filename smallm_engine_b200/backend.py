@@ -108,8 +108,8 @@ class CUDABackend:
         return out
 
     # ---- drafted tokens over a bounded cache ----
-    # Pointers are device addresses (int); stream None is the context's own.
-    # Sizes must fit the C types: they are checked by the library.
+    # Pointers are device addresses (int), sizes 32-bit; stream None is the
+    # context's own.
     def attention_tree_workspace(self, n_heads: int, n_kv_heads: int, head_dim: int, n_past: int, n_tokens: int,
                                  weights: bool = False) -> int:
         """Bytes of workspace one attention_tree call needs."""

@@ -50,6 +50,7 @@ constexpr int kSelPasses = 4;
 constexpr uint32_t kSelBins = 512;
 constexpr uint32_t kSelCached = 20480;  // keys of a CTA that fit shared memory
 constexpr uint32_t kSelMaxCluster = 16;
+constexpr uint32_t kCacheMaxRows = 1u << 30;  // keeps 32-bit row numbers from wrapping
 
 // Order-preserving key, NaN lowest, -0 equal to +0.
 __device__ __forceinline__ uint32_t total_key(float x) { return x == x ? float_order_key(x + 0.f) : 0u; }
@@ -204,7 +205,6 @@ constexpr int kMoveThreads = 512;
 constexpr int kMoveUnroll = 8;
 constexpr uint32_t kMoveWave = kMoveThreads * kMoveUnroll;  // vectors of a CTA per wave in registers
 constexpr uint32_t kMoveMaxCluster = 8;
-constexpr unsigned kErrMoveList = 128u, kErrMoveWait = 512u;
 
 struct MoveArgs {
     const uint32_t* rows;
@@ -419,6 +419,9 @@ void launch_cache_select(const float* weights, uint32_t n_kv, uint32_t max_ctx, 
     if (n_keep > n || (uint64_t)n_first + n_last > n_keep)
         throw Error(SMALLM_ERR_INVALID, "cache_select: needs n_first + n_last <= n_keep <= n");
     if (n_kv > 65535) throw Error(SMALLM_ERR_RANGE, "cache_select: at most 65535 KV heads");
+    if (n > kCacheMaxRows) throw Error(SMALLM_ERR_RANGE, "cache_select: at most 2^30 rows");
+    if ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(rows)) & 3u)
+        throw Error(SMALLM_ERR_INVALID, "cache_select: weights and rows must be 4-byte aligned");
     if (!n_kv || !n_keep) return;
     // CTAs per head: a couple of keys per thread at least, two CTAs per SM in
     // all, and no cluster left waiting for another to end
@@ -440,8 +443,11 @@ void launch_cache_move(float* kcache, float* vcache, float* weights, uint32_t n_
     if ((uint64_t)dst + n_rows > max_ctx)
         throw Error(SMALLM_ERR_RANGE, "cache_move: dst + n_rows must not pass max_ctx");
     if (n_kv > 65535) throw Error(SMALLM_ERR_RANGE, "cache_move: at most 65535 KV heads");
+    if (n_rows > kCacheMaxRows) throw Error(SMALLM_ERR_RANGE, "cache_move: at most 2^30 rows");
     if ((reinterpret_cast<uintptr_t>(kcache) | reinterpret_cast<uintptr_t>(vcache)) & 15u)
         throw Error(SMALLM_ERR_INVALID, "cache_move: kcache and vcache must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(rows)) & 3u)
+        throw Error(SMALLM_ERR_INVALID, "cache_move: weights and rows must be 4-byte aligned");
     if (!n_kv || !n_rows) return;
     MoveArgs a{rows, n_rows, dst, max_ctx, device_error_flag()};
     uint32_t stride = per_head ? n_rows : 0;

@@ -206,6 +206,10 @@ void launch_kernel_ex(const void* fn, dim3 grid, dim3 block, size_t smem, cudaSt
 // Device address of the current device's kernel error word (see
 // gemv_error_flags).
 unsigned int* device_error_flag();
+// The word's bits that the drafted-token operators raise; a model step leaves
+// them to whoever called the operator.
+constexpr unsigned kErrMoveList = 128u, kErrTreeWait = 256u, kErrMoveWait = 512u, kErrLogprobs = 1024u;
+constexpr unsigned kErrOperators = kErrMoveList | kErrTreeWait | kErrMoveWait | kErrLogprobs;
 
 // Batched prefill (prefill.cu and the embedding in kernels.cu): rows are
 // tokens, T of them at positions pos0 .. pos0 + T - 1.

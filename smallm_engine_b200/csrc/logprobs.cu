@@ -41,7 +41,6 @@ constexpr int kLpVec = 4;                          // float4s of a thread per ch
 constexpr uint32_t kLpChunk = kLpThreads * kLpVec;  // float4s of a CTA per chunk
 constexpr uint32_t kLpStages = 2;
 constexpr uint32_t kLpMaxCluster = 16;
-constexpr unsigned kErrLpWait = 1024u;
 constexpr uint32_t kLpGroups = kLpThreads / 2;
 constexpr uint32_t kLpCut = 128;  // collected keys that make a cut worth its barriers
 constexpr uint32_t kLpLists = (kLpMaxCluster - 1) * kLogprobMaxTop / kLpThreads + 1;  // joined keys of a thread
@@ -348,13 +347,13 @@ __global__ void __launch_bounds__(kLpThreads, 4)
         }
         cluster.sync();
         if (rank) {
-            if (!ok) atomicOr(err, kErrLpWait);
+            if (!ok) atomicOr(err, kErrLogprobs);
             return;
         }
     } else {
         __syncthreads();
     }
-    if (!ok) atomicOr(err, kErrLpWait);
+    if (!ok) atomicOr(err, kErrLogprobs);
     const float nan = __int_as_float(0x7FC00000);
     const float M = sh.m, ls = sh.bad || M == -INFINITY ? nan : logf(sh.s0);
     if (tid == 0) {
@@ -377,6 +376,10 @@ void launch_logprobs(const LogprobArgs& a, cudaStream_t stream) {
     if (a.n_top > kLogprobMaxTop || a.n_top > a.vocab)
         throw Error(SMALLM_ERR_RANGE, "logprobs: at most 64 alternatives, and no more than vocab");
     if (a.n_rows > 1u << 26) throw Error(SMALLM_ERR_RANGE, "logprobs: at most 2^26 rows");
+    if ((reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.tokens) |
+         reinterpret_cast<uintptr_t>(a.logprob) | reinterpret_cast<uintptr_t>(a.entropy) |
+         (a.n_top ? reinterpret_cast<uintptr_t>(a.top_ids) | reinterpret_cast<uintptr_t>(a.top_logprobs) : 0)) & 3u)
+        throw Error(SMALLM_ERR_INVALID, "logprobs: pointers must be 4-byte aligned");
     if (!a.n_rows) return;
     // CTAs per row: two per SM in all, each with a chunk to itself at least
     const uint32_t nq = (a.vocab + 6) / 4, sms = (uint32_t)device_sm_count();

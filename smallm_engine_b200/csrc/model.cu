@@ -628,7 +628,7 @@ void Model::forward(uint32_t token, uint32_t pos, float* out_logits, uint32_t* o
 }
 
 void Model::check_step_errors() {
-    const unsigned int e = *h_err;
+    const unsigned int e = *h_err & ~kErrOperators;
     if (!e) return;
     *h_err = 0;
     gemv_error_flags(true);
@@ -814,7 +814,12 @@ void Model::logprobs(uint32_t token, float* logprob, float* entropy, uint32_t n_
     launch_logprobs(a, stream);
     uint32_t host[kHead + 2 * kLogprobMaxTop];
     SM_CUDA(cudaMemcpyAsync(host, lp_scratch, 4 * (kHead + 2 * n_top), cudaMemcpyDeviceToHost, stream));
+    SM_CUDA(cudaMemcpyAsync(h_err, device_error_flag(), 4, cudaMemcpyDeviceToHost, stream));
     SM_CUDA(cudaStreamSynchronize(stream));
+    if (*h_err & kErrLogprobs) {
+        gemv_error_flags(true);
+        throw Error(SMALLM_ERR_CUDA, "logprobs: a bounded device wait gave up; the results are invalid");
+    }
     if (logprob) std::memcpy(logprob, host + 1, 4);
     if (entropy) std::memcpy(entropy, host + 2, 4);
     if (n_top) {

@@ -89,7 +89,6 @@ constexpr uint32_t kTcRows = 128, kTcKeys = 64, kTcSlots = 2, kTcRing = 8;
 // 2 x 128 rows + 4 x 56 converters + 24 issuer = 504
 constexpr uint32_t kTcThreads = 32 * 28;
 constexpr uint32_t kConvThreads = 256, kConvWarps = kConvThreads / 32;
-constexpr unsigned kErrTreeWait = 256u;
 constexpr float kPShift = 14.f;
 
 template <int HD>

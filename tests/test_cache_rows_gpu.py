@@ -156,6 +156,10 @@ def test_refusals(be):
     assert sel(wp, 2, 64, 64, 65, 0, 0, rp) == _lib.ERR_INVALID
     assert sel(wp, 2, 64, 64, 8, 5, 4, rp) == _lib.ERR_INVALID
     assert sel(wp, 2, 64, 64, 8, 2**32 - 1, 2, rp) == _lib.ERR_INVALID
+    assert sel(wp, 2, 2**31, 2**30 + 1, 8, 0, 0, rp) == _lib.ERR_RANGE
+    assert sel(wp, 65536, 64, 64, 8, 0, 0, rp) == _lib.ERR_RANGE
+    assert sel(wp + 2, 2, 64, 64, 8, 0, 0, rp) == _lib.ERR_INVALID
+    assert sel(wp, 2, 64, 64, 8, 0, 0, rp + 1) == _lib.ERR_INVALID
     assert sel(wp, 0, 64, 64, 8, 0, 0, rp) == _lib.OK
     assert sel(wp, 2, 64, 64, 0, 0, 0, rp) == _lib.OK
     mv = lambda *a: L.smallm_cache_move(be.h, *a, None)  # noqa: E731
@@ -166,6 +170,10 @@ def test_refusals(be):
     assert mv(p + 4, p, None, 2, 32, 64, rp, 0, 4, 0) == _lib.ERR_INVALID
     assert mv(p, p, None, 2, 32, 64, rp, 0, 4, 61) == _lib.ERR_RANGE
     assert mv(p, p, None, 2, 32, 64, rp, 0, 4, 2**32 - 2) == _lib.ERR_RANGE
+    assert mv(p, p, None, 2, 32, 2**31, rp, 0, 2**30 + 1, 0) == _lib.ERR_RANGE
+    assert mv(p, p, None, 65536, 32, 64, rp, 0, 4, 0) == _lib.ERR_RANGE
+    assert mv(p, p, wp + 2, 2, 32, 64, rp, 0, 4, 0) == _lib.ERR_INVALID
+    assert mv(p, p, None, 2, 32, 64, rp + 2, 0, 4, 0) == _lib.ERR_INVALID
     assert mv(p, p, None, 2, 32, 64, rp, 0, 0, 0) == _lib.OK
     torch.cuda.synchronize()
     assert float(x.abs().max()) == 0.0 and int(r.abs().max()) == 0

@@ -10,6 +10,10 @@ by 2 (hd + 8) u D + (2 n + 64) u relative to the weighted values (u = 2^-24, D
 the largest score by magnitude of its terms, below 64 here, n below 256), so
 2 * 72 * 64 u + 576 u < 6e-4; values are moved, not computed, so caches are
 compared for equality."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -169,6 +173,114 @@ def test_two_calls_at_once(be):
         torch.cuda.synchronize()
         for a, b in zip(alone, both):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def chain_of_calls(be, st):
+    """attention with totals, select, move, logprobs of the output, on stream st."""
+    H, kv, hd, n, T = 8, 2, 64, 700, 5
+    g = torch.Generator(device="cuda").manual_seed(11)
+    q = torch.randn(T, H * hd, device="cuda", generator=g)
+    k0, v0 = (torch.randn(kv, n + T, hd, device="cuda", generator=g) for _ in range(2))
+    k, v, w = k0.clone(), v0.clone(), torch.zeros(kv, n + T, device="cuda")
+    need = be.attention_tree_workspace(H, kv, hd, n, T, True)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    out, rows = torch.empty(T, H * hd, device="cuda"), torch.empty(kv, 300, dtype=torch.int32, device="cuda")
+    ent = torch.empty(T, device="cuda")
+    torch.cuda.synchronize()
+
+    def reset():
+        k.copy_(k0), v.copy_(v0), w.zero_()
+
+    def attend_(s):
+        be.attention_tree(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), H, kv, hd, n + T, n, T,
+                          work.data_ptr(), need, weights=w.data_ptr(), stream=s.cuda_stream)
+
+    def evict(s):
+        be.cache_select(w.data_ptr(), kv, n + T, n + T, 300, 4, 16, rows.data_ptr(), stream=s.cuda_stream)
+        be.cache_move(k.data_ptr(), v.data_ptr(), kv, hd, n + T, rows.data_ptr(), 300, 0, per_head=True,
+                      weights=w.data_ptr(), stream=s.cuda_stream)
+
+    def score(s):
+        be.logprobs(out.data_ptr(), T, H * hd, None, None, ent.data_ptr(), 0, None, None, stream=s.cuda_stream)
+    return reset, attend_, evict, score, (k, v, w, out, rows, ent, q, work)
+
+
+def test_captured_with_other_streams(be):
+    """One graph over two streams: scoring beside the eviction, both after the
+    attention, replayed: the same bits as one call after the other."""
+    st, side = torch.cuda.Stream(), torch.cuda.Stream()
+    reset, attend_, evict, score, t = chain_of_calls(be, st)
+    with torch.cuda.stream(st):
+        reset()
+        attend_(st), evict(st), score(st)
+    st.synchronize()
+    want = [x.clone() for x in t[:6]]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        reset()
+        attend_(st)
+        side.wait_stream(st)
+        score(side)
+        evict(st)
+        st.wait_stream(side)
+        t[5].add_(1)
+    for _ in range(3):
+        for x in (t[3], t[4], t[5]):
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want[:5], t)) and torch.equal(want[5] + 1, t[5])
+    assert be.device_errors() == 0
+
+
+FIRST = """
+import sys, torch
+sys.path.insert(0, {tests!r})
+from smallm_engine_b200 import CUDABackend
+from test_draft_run_gpu import chain_of_calls
+be = CUDABackend()
+st = torch.cuda.Stream()
+reset, attend_, evict, score, t = chain_of_calls(be, st)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=st):
+    reset()
+    attend_(st), evict(st), score(st)
+graph.replay()
+torch.cuda.synchronize()
+got = [x.clone() for x in t[:6]]
+with torch.cuda.stream(st):
+    reset()
+    attend_(st), evict(st), score(st)
+st.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, t))
+print("same")
+"""
+
+
+def test_first_calls_captured():
+    """The very first calls of a process may be captured ones."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST.format(tests=here)], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(here))
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stderr[-2000:]
+
+
+def test_bad_list_is_not_a_steps_error(be, gguf_dir):
+    """Bit 7 stays for the caller of cache_move to read; a model steps on."""
+    m = CudaModel(synth.write_gguf(synth.tiny_spec("llama-q4_0"), 8, gguf_dir / "lp-llama2.gguf"))
+    want = m.forward(5, 0)
+    k, v = torch.zeros(2, 1, 64, 32, device="cuda")
+    rows = torch.tensor([3, 3], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    be.device_errors()
+    be.cache_move(k.data_ptr(), v.data_ptr(), 1, 32, 64, rows.data_ptr(), 2, 0)
+    be.synchronize()
+    m.reset_cache()
+    np.testing.assert_array_equal(m.forward(5, 0), want)
+    assert m.logprobs(1).token == 1
+    assert be.device_errors() == 128 and be.device_errors() == 0
+    m.close()
 
 
 def test_model_logprobs_and_generator(gguf_dir):

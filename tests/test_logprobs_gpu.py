@@ -167,6 +167,14 @@ def test_refusals(be):
     assert f(p, 2, 100, 100, None, None, q, 3, q, None) == _lib.ERR_INVALID
     assert f(p, 2, 100, 100, None, None, q, 65, q, q) == _lib.ERR_RANGE
     assert f(p, 2, 10, 10, None, None, q, 11, q, q) == _lib.ERR_RANGE
+    assert f(p, 2**26 + 1, 1, 1, None, None, q, 0, None, None) == _lib.ERR_RANGE
+    assert f(p, 1, 2**30 + 1, 2**30 + 1, None, None, q, 0, None, None) == _lib.ERR_RANGE
+    assert f(p + 2, 2, 10, 10, None, None, q, 0, None, None) == _lib.ERR_INVALID
+    assert f(p, 2, 10, 10, p + 1, q, None, 0, None, None) == _lib.ERR_INVALID
+    assert f(p, 2, 10, 10, p, q + 1, None, 0, None, None) == _lib.ERR_INVALID
+    assert f(p, 2, 10, 10, None, None, q + 2, 0, None, None) == _lib.ERR_INVALID
+    assert f(p, 2, 10, 10, None, None, q, 1, q + 3, q) == _lib.ERR_INVALID
+    assert f(p, 2, 10, 10, None, None, q, 1, q, q + 3) == _lib.ERR_INVALID
     assert f(p, 0, 100, 100, None, None, q, 0, None, None) == _lib.OK
     torch.cuda.synchronize()
     assert float(o.abs().max()) == 0.0
