@@ -126,12 +126,14 @@ __device__ __forceinline__ void tc_scale(uint32_t max_bits, float& mult, float& 
     mult = __uint_as_float(f << 23);
     inv = __uint_as_float((254u - f) << 23);
 }
-// hi = x rounded to f16, lo = (x - hi) rounded to f16, of two values.
+// hi = x rounded to f16, lo = (x - hi) rounded to f16, of two values (the
+// difference as a mixed fma by -1: a mixed subtraction takes the f16 operand
+// first, and the two negations after it cost an instruction each).
 __device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) {
-    asm("{\n .reg .f16 a, b;\n .reg .f32 c, d;\n"
-        " cvt.rn.f16x2.f32 %0, %3, %2;\n mov.b32 {a, b}, %0;\n"
-        " sub.rn.f32.f16 c, a, %2;\n sub.rn.f32.f16 d, b, %3;\n"
-        " neg.f32 c, c;\n neg.f32 d, d;\n cvt.rn.f16x2.f32 %1, d, c;\n}"
+    asm("{\n .reg .f16 a, b, n;\n .reg .f32 c, d;\n"
+        " cvt.rn.f16x2.f32 %0, %3, %2;\n mov.b32 {a, b}, %0;\n mov.b16 n, 0xBC00;\n"
+        " fma.rn.f32.f16 c, a, n, %2;\n fma.rn.f32.f16 d, b, n, %3;\n"
+        " cvt.rn.f16x2.f32 %1, d, c;\n}"
         : "=&r"(hi), "=r"(lo)
         : "f"(x.x), "f"(x.y));
 }
@@ -151,15 +153,10 @@ __device__ __forceinline__ float ex2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// The largest of three magnitudes, NaN if any is; of three values.
+// The largest of three magnitudes, NaN if any is.
 __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     float r;
     asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -684,6 +681,17 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = tid % L4, part = tid / L4;
     const size_t rows = (size_t)a.n_kv * p.R, row = blockIdx.x;
     pdl_wait();
+    // the first splits of each part leave with the maxima (past the last split
+    // the loads repeat it and are dropped)
+    constexpr int PRE = 4;
+    float2 ml[PRE];
+    float4 v[PRE];
+#pragma unroll
+    for (int k = 0; k < PRE; ++k) {
+        const uint32_t s = min((uint32_t)(part + k * PARTS), p.n_split - 1);
+        ml[k] = p.part_ml[s * rows + row];
+        v[k] = reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * HD)[c];
+    }
     float M = -INFINITY;
     for (uint32_t s = tid; s < p.n_split; s += kMergeThreads) M = fmaxf(M, p.part_ml[s * rows + row].x);
     M = warp_max(M);
@@ -695,14 +703,17 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
     const float ref = M == -INFINITY ? 0.f : M;
     float L = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float2 s, float4 x) {
+        const float f = exp2f(s.x - ref);
+        L = fmaf(f, s.y, L);
+        O.x = fmaf(f, x.x, O.x), O.y = fmaf(f, x.y, O.y), O.z = fmaf(f, x.z, O.z), O.w = fmaf(f, x.w, O.w);
+    };
+#pragma unroll
+    for (int k = 0; k < PRE; ++k)
+        if (part + k * PARTS < p.n_split) add(ml[k], v[k]);
 #pragma unroll 4
-    for (uint32_t s = part; s < p.n_split; s += PARTS) {
-        const float2 ml = p.part_ml[s * rows + row];
-        const float4 v = reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * HD)[c];
-        const float f = exp2f(ml.x - ref);
-        L = fmaf(f, ml.y, L);
-        O.x = fmaf(f, v.x, O.x), O.y = fmaf(f, v.y, O.y), O.z = fmaf(f, v.z, O.z), O.w = fmaf(f, v.w, O.w);
-    }
+    for (uint32_t s = part + PRE * PARTS; s < p.n_split; s += PARTS)
+        add(p.part_ml[s * rows + row], reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * HD)[c]);
     acc[part][c] = O;
     if (c == 0) redl[part] = L;
     __syncthreads();
