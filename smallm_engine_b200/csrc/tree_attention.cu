@@ -673,14 +673,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
 // once (one warp walking the splits took 13 to 57 us of dependent loads).
 constexpr int kMergeThreads = 256;
 template <int HD>
-__global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const TreeParams p) {
+__device__ __forceinline__ void merge_row(const TreeParams& p, size_t row) {
     constexpr int L4 = HD / 4, PARTS = kMergeThreads / L4;
     __shared__ float4 acc[PARTS][L4];
     __shared__ float red[32], redl[32];
     const TreeArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = tid % L4, part = tid / L4;
-    const size_t rows = (size_t)a.n_kv * p.R, row = blockIdx.x;
-    pdl_wait();
+    const size_t rows = (size_t)a.n_kv * p.R;
     // the first splits of each part leave with the maxima (past the last split
     // the loads repeat it and are dropped)
     constexpr int PRE = 4;
@@ -729,29 +728,65 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
     const uint32_t g = (uint32_t)(row / p.R), r = (uint32_t)(row % p.R);
     float* o = a.out + (size_t)(r / p.G) * a.out_stride + ((size_t)g * p.G + r % p.G) * HD;
     reinterpret_cast<float4*>(o)[c] = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
-    if (c == 0 && p.scores) p.stats[row] = make_float2(ref, inv);
+    if (c == 0 && p.sc_rows && p.scores) p.stats[row] = make_float2(ref, inv);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const TreeParams p) {
+    pdl_wait();
+    merge_row<HD>(p, blockIdx.x);
 }
 
 // weights[g][k] += sum_r 2^(s c - mc_r) / sum_r, in a fixed order, so that the
 // total does not depend on the launch.  Scores of up to kFewRows rows run along
-// the keys: a lane has a key and walks the rows.  More rows run along
-// themselves: the lanes of a warp have a key's rows, 16 keys at a time, and
-// their sums meet by shuffles.
+// the keys: a lane has a key and walks the rows; the CTAs behind the n_join
+// that join the splits find mc and sum of the rows from the splits themselves,
+// so that neither waits for the other (a kernel after the joining one: 38 us
+// instead of 35 us for one token over 16384 rows).  More rows run along themselves: the
+// lanes of a warp have a key's rows, 16 keys at a time, and their sums meet by
+// shuffles.
 constexpr int kWeightKeys = 16, kWeightWarps = 8;
 constexpr uint32_t kFewRows = 16;
-__global__ void __launch_bounds__(256) smallm_tree_weights_few_kernel(const TreeParams p) {
-    const uint32_t key = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y;
+template <int HD>
+__global__ void __launch_bounds__(kMergeThreads) smallm_tree_weights_few_kernel(const TreeParams p, uint32_t n_join) {
+    __shared__ float2 stats[kFewRows];
     pdl_wait();
-    if (key >= p.n) return;
-    float* w = p.a.weights + (size_t)g * p.a.max_ctx + key;
-    const float* s = p.scores + (size_t)g * p.R * p.sc_keys + key;
-    const float old = *w;
-    float acc = 0.f;
-#pragma unroll 8
-    for (uint32_t r = 0; r < p.R; ++r) {
-        const float2 st = p.stats[(size_t)g * p.R + r];
-        acc = fmaf(exp2f(fmaf(__ldg(s + (size_t)r * p.sc_keys), p.c, -st.x)), st.y, acc);
+    if (blockIdx.x < n_join) {
+        merge_row<HD>(p, blockIdx.x);
+        return;
     }
+    const uint32_t blocks = (p.n + kMergeThreads - 1) / kMergeThreads, at = blockIdx.x - n_join;
+    const uint32_t g = at / blocks, key = at % blocks * kMergeThreads + threadIdx.x, lane = threadIdx.x & 31;
+    // (loads past the last row or key repeat it and are dropped)
+    float* w = p.a.weights + (size_t)g * p.a.max_ctx + min(key, p.n - 1);
+    const float* s = p.scores + (size_t)g * p.R * p.sc_keys + min(key, p.n - 1);
+    const float old = *w;
+    float v[kFewRows];
+#pragma unroll
+    for (uint32_t r = 0; r < kFewRows; ++r) v[r] = __ldg(s + (size_t)min(r, p.R - 1) * p.sc_keys);
+    for (uint32_t r = threadIdx.x >> 5; r < p.R; r += kMergeThreads / 32) {
+        const size_t row = (size_t)g * p.R + r, rows = (size_t)p.a.n_kv * p.R;
+        if (p.n_split == 1) {
+            if (lane == 0) stats[r] = p.stats[row];
+            continue;
+        }
+        float m = -INFINITY, l = 0.f;
+        for (uint32_t i = lane; i < p.n_split; i += 32) {
+            const float2 ml = p.part_ml[i * rows + row];
+            const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top;
+            l = fmaf(l, exp2f(m - ref), ml.y * exp2f(ml.x - ref));
+            m = top;
+        }
+        const float top = warp_max(m), ref = top == -INFINITY ? 0.f : top;
+        l = warp_sum(l * exp2f(m - ref));
+        if (lane == 0) stats[r] = make_float2(ref, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
+    }
+    __syncthreads();
+    if (key >= p.n) return;
+    float acc = 0.f;
+#pragma unroll
+    for (uint32_t r = 0; r < kFewRows; ++r)
+        if (r < p.R) acc = fmaf(exp2f(fmaf(v[r], p.c, -stats[r].x)), stats[r].y, acc);
     *w = old + acc;
 }
 __global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(const TreeParams p) {
@@ -835,14 +870,22 @@ void launch_tree(const TreeParams& p, cudaStream_t stream) {
     TreeParams pp = p;
     void* args[] = {&pp};
     launch_kernel_ex(fn, grid, dim3(kTcThreads), TcTree<HD>::smem, stream, true, args);
-    if (p.n_split > 1) {
-        launch_kernel_ex((const void*)smallm_tree_merge_kernel<HD>, dim3(p.a.n_kv * p.R), dim3(kMergeThreads), 0,
-                         stream, true, args);
+    const uint32_t n_join = p.n_split > 1 ? p.a.n_kv * p.R : 0;
+    if (p.a.weights && !p.sc_rows) {
+        uint32_t join = n_join;
+        void* few[] = {&pp, &join};
+        const uint32_t blocks = (p.n + kMergeThreads - 1) / kMergeThreads;
+        launch_kernel_ex((const void*)smallm_tree_weights_few_kernel<HD>, dim3(n_join + blocks * p.a.n_kv),
+                         dim3(kMergeThreads), 0, stream, true, few);
+        return;
     }
+    if (n_join)
+        launch_kernel_ex((const void*)smallm_tree_merge_kernel<HD>, dim3(n_join), dim3(kMergeThreads), 0, stream, true,
+                         args);
     if (p.a.weights) {
-        const void* sum = p.sc_rows ? (const void*)smallm_tree_weights_kernel : (const void*)smallm_tree_weights_few_kernel;
-        const uint32_t keys = p.sc_rows ? kWeightWarps * kWeightKeys : 256;
-        launch_kernel_ex(sum, dim3((p.n + keys - 1) / keys, p.a.n_kv), dim3(256), 0, stream, true, args);
+        const uint32_t keys = kWeightWarps * kWeightKeys;
+        launch_kernel_ex((const void*)smallm_tree_weights_kernel, dim3((p.n + keys - 1) / keys, p.a.n_kv),
+                         dim3(32 * kWeightWarps), 0, stream, true, args);
     }
 }
 
