@@ -59,36 +59,40 @@ struct TreeParams {
 // that.  The small products are accumulated first.  (The result is nearer the
 // definition in 64 bits than f32 products and sums are: 1.1e-6 of its norm
 // against 3.6e-6 for 64 tokens over 32683 rows.)
-//   - warps 25 (K) and 26 (V) copy f32 rows with bulk copies, half a tile at a
-//     time, into two halves each: 64 KB in flight while the tile before is
-//     converted.  (Loads through registers took the load/store unit twice as
-//     long as these copies and the reads of them.)
-//   - warps 8..15 (K) and 16..23 (V) convert: a group takes a tile into
-//     registers, finds its exponent and writes hi and lo in the MMA's swizzled
-//     layout, two slots for each of K and V;
+//   - warps 25 (K) and 26 (V) copy tiles of f32 rows with bulk copies into
+//     three slots each (six for rows of 64 or fewer).  (Loads through registers
+//     took the load/store unit twice as long as these copies and the reads of
+//     them.)
+//   - warps 16..19 (K) and 20..23 (V) convert in place: a group takes a tile
+//     into registers, finds its exponent and, once all have theirs, writes hi
+//     and lo in the MMA's swizzled layout over it.  (Slots of their own behind
+//     one tile of raw rows, for eight warps each: 3% slower at 64 tokens.)
 //   - warp 24 issues S = Q K^T (Q in tensor memory) and, a tile behind,
 //     O = P V (P in tensor memory, over S's columns; V MN-major);
 //   - warps 0..7, lane = row, two warps for a row: each takes half of the keys
 //     for the running maximum (a whole number in base 2, so rescaling is
 //     exact; the halves meet in shared memory), P = 2^(s - m + 14) as hi and lo
-//     and the sum, and half of the columns of the tile before's O, which it
-//     adds to f32 registers with that tile's exponent and the row's rescaling:
-//     the long sum is made of rounded f32 adds.
-// One token of 32 heads at 128 reads K and V at 6.2 TB/s from 16384 rows on
-// (the slope of its time; copies reach 6.5), after 9 us for two launches, the
-// first tile and the join.  Blocks with all 128 rows take about 3250 cycles
-// a tile, the issue slots 74% busy and the tensor pipe 47%: conversion and
-// softmax bound them, not the products.  Measured and not kept: smaller copies
-// in a longer ring, a scale for each converter warp instead of each tile, f32
-// FMAs for few rows, splits that join through a cluster's shared memory.
+//     and the sum;
+//   - warps 8..15, lane = row, take half of the columns of a tile's O each and
+//     add it to f32 registers with that tile's exponent and the row's
+//     rescaling: the long sum is made of rounded f32 adds.  (By the same warps
+//     as the softmax one token over 16384 rows took 2% longer, with totals 6%.)
+// One token of 32 heads at 128 reads K and V at 6.3 TB/s from 16384 rows on
+// (the slope of its time; copies reach 6.5), after 8 us for two launches, the
+// first tile and the join.  Blocks with all 128 rows take about 2700 cycles a
+// tile where the products take 1536: conversion, softmax and the issue of the
+// products each work for some 2300 of them, in 5 instructions of 8 issue slots.
+// Measured and not kept: smaller copies in a longer ring, a scale for each
+// converter warp instead of each tile, f32 FMAs for few rows, splits that join
+// through a cluster's shared memory.
 // An infinity or NaN of K or V would reach every row through 0 * inf, so it is
 // replaced by 0 and its key marked; rows that see the key turn to NaN.
 // Every wait is bounded; one that gives up raises bit 8 of the error word.
-constexpr uint32_t kTcRows = 128, kTcKeys = 64, kTcSlots = 2, kTcRing = 8;
+constexpr uint32_t kTcRows = 128, kTcKeys = 64, kTcMaxSlots = 6, kTcRing = 8;
 // seven warpgroups; registers per thread 72 at launch (504 over the seven), then
-// 2 x 128 rows + 4 x 56 converters + 24 issuer = 504
+// 2 x 72 rows + 2 x 88 output + 2 x 80 converters + 24 issuer = 504
 constexpr uint32_t kTcThreads = 32 * 28;
-constexpr uint32_t kConvThreads = 256, kConvWarps = kConvThreads / 32;
+constexpr uint32_t kConvThreads = 128, kConvWarps = kConvThreads / 32;
 constexpr float kPShift = 14.f;
 
 template <int HD>
@@ -96,9 +100,11 @@ struct TcTree {
     static constexpr uint32_t chunks = HD < 64 ? 1 : HD / 64;   // 128-byte columns of a tile
     static constexpr uint32_t half = chunks * kTcKeys * 128;    // bytes of a tile's hi or lo
     static constexpr uint32_t slot = 2 * half;
-    static constexpr uint32_t raw = kTcKeys / 2 * HD * 4;       // bytes of half a tile in f32
-    static constexpr size_t smem = 1024 + 2ull * kTcSlots * slot + 4ull * raw + 8192;
-    static_assert(kTcRows * HD * 4 <= kTcSlots * slot, "q and the output pass through the slots");
+    static constexpr uint32_t slots = HD > 64 ? 3 : 6;          // of K and of V each
+    static constexpr size_t smem = 1024 + 2ull * slots * slot + 8192;
+    static_assert(kTcKeys * HD * 4 <= slot, "a tile is converted in place");
+    static_assert(kTcRows * HD * 4 <= 2 * slot, "q and the output pass through two slots");
+    static_assert(slots <= kTcMaxSlots && slots + 2 <= kTcRing, "scales outlive their slots by two tiles");
     static constexpr uint32_t pv_n = HD < 64 ? 64 : HD;         // columns past HD are never read
     // tensor-memory columns; P (hi 32, lo 32) takes the place of its S
     static constexpr uint32_t q_hi = 0, q_lo = 64, s0 = 128, o0 = 256;
@@ -107,8 +113,8 @@ struct TcTree {
 };
 
 struct TcShared {
-    uint64_t k_full[kTcSlots], k_empty[kTcSlots], v_full[kTcSlots], v_empty[kTcSlots];
-    uint64_t raw_full[2][2], raw_empty[2][2];  // [K, V][half]
+    uint64_t k_full[kTcMaxSlots], k_empty[kTcMaxSlots], v_full[kTcMaxSlots], v_empty[kTcMaxSlots];
+    uint64_t raw_full[2][kTcMaxSlots];  // [K, V]
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, done;
     float k_scale[kTcRing], v_scale[kTcRing];
     unsigned long long k_bad[kTcRing], v_bad[kTcRing];
@@ -117,6 +123,8 @@ struct TcShared {
     float part_max[2][2][kTcRows];  // [tile % 2][half]
     float part_sum[2][kTcRows];
     uint32_t q_max[kTcRows];
+    float corr[4][kTcRows];  // [tile % 4] what a tile's maximum leaves of the output before it
+    float factor[kTcRows];
 };
 static_assert(sizeof(TcShared) <= 8192, "shared-memory tail");
 
@@ -137,11 +145,11 @@ __device__ __forceinline__ void split_f16(float2 x, uint32_t& hi, uint32_t& lo) 
         : "=&r"(hi), "=r"(lo)
         : "f"(x.x), "f"(x.y));
 }
-// Barrier of the 256 threads of converter group `id`; true where any says so.
+// Barrier of the 128 threads of converter group `id`; true where any says so.
 __device__ __forceinline__ bool conv_any(int id, bool v) {
     uint32_t r;
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 256, p;\n"
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 128, p;\n"
         " selp.u32 %0, 1, 0, q;\n}"
         : "=r"(r)
         : "r"((uint32_t)v), "r"(id)
@@ -179,78 +187,68 @@ __device__ __forceinline__ unsigned long long tc_seen(const uint32_t* mask, uint
     return m;
 }
 
+// One lane: every copy of tiles before `end` has landed.
+template <int HD>
+__device__ __forceinline__ bool tc_landed(uint32_t end, uint64_t* full) {
+    constexpr uint32_t S = TcTree<HD>::slots;
+    bool ok = true;
+    for (uint32_t t = end - min(end, S); t < end; ++t) ok = mbar_wait_soon(&full[t % S], (t / S) & 1) && ok;
+    return ok;
+}
 // One lane: tiles from .. to - 1 of a CTA's tiles t0 .. (rows of `src` below n)
-// into the two raw halves.
+// into their slots.
 template <int HD>
 __device__ __forceinline__ bool tc_copy(const float* src, uint32_t n, uint32_t t0, uint32_t from, uint32_t to,
-                                        uint8_t* raw, uint64_t* full, uint64_t* empty) {
+                                        uint8_t* slots, uint64_t* full, uint64_t* empty) {
     using C = TcTree<HD>;
-    for (uint32_t i = 2 * from; i < 2 * to; ++i) {
-        const uint32_t t = i >> 1, h = i & 1, row = (t0 + t) * kTcKeys + h * (kTcKeys / 2);
-        if (t && !mbar_wait_soon(&empty[h], (t - 1) & 1)) {
-            // no copy may still be landing when the CTA exits
-            for (uint32_t j = 0; j < 2; ++j) mbar_wait(&full[j], (t - (j >= h)) & 1);
+    for (uint32_t t = from; t < to; ++t) {
+        const uint32_t s = t % C::slots, row = (t0 + t) * kTcKeys, rows = min(n - row, kTcKeys);
+        if (t >= C::slots && !mbar_wait_soon(&empty[s], (t / C::slots - 1) & 1)) {
+            tc_landed<HD>(t, full);  // no copy may still be landing when the CTA exits
             return false;
         }
-        const uint32_t rows = row < n ? min(n - row, kTcKeys / 2) : 0;
-        if (rows) {
-            mbar_arrive_expect_tx(&full[h], rows * HD * 4);
-            bulk_g2s(raw + h * C::raw, src + (size_t)row * HD, rows * HD * 4, &full[h]);
-        } else {
-            mbar_arrive(&full[h]);
-        }
+        mbar_arrive_expect_tx(&full[s], rows * HD * 4);
+        bulk_g2s(slots + s * C::slot, src + (size_t)row * HD, rows * HD * 4, &full[s]);
     }
     return true;
 }
 
-// One converter group: tiles t0 .. t0 + nt - 1 from the raw halves into `slots`.
+// One converter group: tiles t0 .. t0 + nt - 1, in place.
 template <int HD, int GROUP>
 __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt, int tid, uint8_t* smem, TcShared& sh) {
     using C = TcTree<HD>;
-    constexpr int N = (int)kTcKeys * HD / 4 / kConvThreads;  // float4s of a thread, N / 2 from each half
+    constexpr int N = (int)kTcKeys * HD / 4 / kConvThreads;  // float4s of a thread
     constexpr uint32_t W = HD / 4, STEP = kConvThreads / W;  // float4s of a row; rows between two units
     const uint32_t c4 = tid % W, row0 = tid / W;
-    const float4* src = reinterpret_cast<const float4*>(smem + 2 * kTcSlots * C::slot + GROUP * 2 * C::raw) + tid;
-    uint8_t* slots = smem + GROUP * kTcSlots * C::slot;
+    uint8_t* slots = smem + GROUP * C::slots * C::slot;
     uint64_t* full = GROUP ? sh.v_full : sh.k_full;
-    uint64_t* empty = GROUP ? sh.v_empty : sh.k_empty;
     unsigned long long* bads = GROUP ? sh.v_bad : sh.k_bad;
     auto& wmax = sh.wmax[GROUP];
     float4 x[N];
-    // (STEP is a multiple of 8: the swizzle is the same for all units)
+    // (STEP is a multiple of 4: the swizzle of odd units differs in one bit at most)
     const uint32_t dst0 =
         (c4 >> 4) * (kTcKeys * 128) + (c4 & 1) * 8 + row0 * 128 + ((((c4 & 15) >> 1) ^ (row0 & 7)) << 4);
+    constexpr uint32_t FLIP = (STEP & 4) << 4;
     const int lane = tid & 31, cw = tid >> 5;
     for (uint32_t t = 0; t < nt; ++t) {
-        const uint32_t slot = t % kTcSlots, use = t / kTcSlots, ring = t % kTcRing;
+        const uint32_t slot = t % C::slots, ring = t % kTcRing;
         const uint32_t left = n - (t0 + t) * kTcKeys;  // rows from the tile's first to the last
-        bool stuck = false;
+        const bool stuck = !mbar_wait_soon(&sh.raw_full[GROUP][slot], (t / C::slots) & 1);
+        const float4* src = reinterpret_cast<const float4*>(slots + slot * C::slot) + tid;
         float m = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            stuck = stuck || !mbar_wait_soon(&sh.raw_full[GROUP][h], t & 1);
+        for (int i = 0; i < N; ++i) x[i] = src[i * kConvThreads];
+        if (left < kTcKeys) {
 #pragma unroll
-            for (int i = h * N / 2; i < (h + 1) * N / 2; ++i) {
-                x[i] = src[i * kConvThreads];
-            }
-            if (left < kTcKeys) {
-#pragma unroll
-                for (int i = h * N / 2; i < (h + 1) * N / 2; ++i)
-                    if (row0 + i * STEP >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-#pragma unroll
-            for (int i = h * N / 2; i < (h + 1) * N / 2; ++i) {
-                m = max3_abs_nan(max3_abs_nan(m, x[i].x, x[i].y), x[i].z, x[i].w);
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.raw_empty[GROUP][h]);
+            for (int i = 0; i < N; ++i)
+                if (row0 + i * STEP >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = max3_abs_nan(max3_abs_nan(m, x[i].x, x[i].y), x[i].z, x[i].w);
         const uint32_t mw = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
         if (lane == 0) wmax[t & 1][cw] = mw;
         if (tid == 0) bads[ring] = 0;
-        // (V's slots hold q until it is in tensor memory)
-        if (use > 0) stuck = stuck || !mbar_wait_soon(&empty[slot], (use - 1) & 1);
-        else if (GROUP == 1 && t == 0) stuck = stuck || !mbar_wait_soon(&sh.q_full, 0);
+        // (past this barrier every thread has its elements)
         if (conv_any(1 + GROUP, stuck)) return false;
         uint32_t mx = __reduce_max_sync(0xffffffffu, wmax[t & 1][lane % kConvWarps]);
         if (mx >= 0x7F800000u) {  // the same for the whole group: clean the tile
@@ -275,13 +273,14 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
         float mult, inv;
         tc_scale(mx, mult, inv);
         if (tid == 0) (GROUP ? sh.v_scale : sh.k_scale)[ring] = inv;
-        uint8_t* dst = slots + slot * C::slot + dst0;
+        uint8_t* const dsts[2] = {slots + slot * C::slot + dst0, slots + slot * C::slot + (dst0 ^ FLIP)};
         const float2 mult2 = make_float2(mult, mult);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             uint2 hi, lo;
             split_f16(mul2(make_float2(x[i].x, x[i].y), mult2), hi.x, lo.x);
             split_f16(mul2(make_float2(x[i].z, x[i].w), mult2), hi.y, lo.y);
+            uint8_t* dst = dsts[i & 1];
             *reinterpret_cast<uint2*>(dst + i * STEP * 128) = hi;
             *reinterpret_cast<uint2*>(dst + i * STEP * 128 + C::half) = lo;
         }
@@ -300,9 +299,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* ks = smem;
-    uint8_t* vs = smem + kTcSlots * C::slot;
-    uint8_t* raw = vs + kTcSlots * C::slot;  // K's two halves, then V's
-    TcShared& sh = *reinterpret_cast<TcShared*>(raw + 4 * C::raw);
+    uint8_t* vs = smem + C::slots * C::slot;
+    TcShared& sh = *reinterpret_cast<TcShared*>(vs + C::slots * C::slot);
     const TreeArgs& a = p.a;
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t r0 = blockIdx.x * kTcRows, split = blockIdx.y, g = blockIdx.z;
@@ -312,7 +310,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
     pdl_launch_dependents();  // the joining kernel's launch overlaps this one
     const uint32_t quads = min(4u, (p.R - r0 + 31) / 32);  // warps' row quarters that hold rows
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < kTcSlots; ++i) {
+        for (uint32_t i = 0; i < C::slots; ++i) {
             mbar_init(&sh.k_full[i], kConvWarps);
             mbar_init(&sh.k_empty[i], 1);
             mbar_init(&sh.v_full[i], kConvWarps);
@@ -335,17 +333,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pdl_wait();  // what came before on the stream has ended
-    // the first tile's rows are on their way while the CTA is set up
-    // (copying warps: 25 K, 26 V)
+    // the first tiles' rows are on their way while the CTA is set up (copying
+    // warps: 25 K, 26 V; V's second and third slot hold q first)
     if (warp - 25 < 2 && lane == 0) {
         const uint32_t op = warp - 25;
         const float* rows_src = (op ? a.vcache : a.kcache) + (size_t)g * a.max_ctx * HD;
-        for (uint32_t h = 0; h < 2; ++h) {
-            mbar_init(&sh.raw_full[op][h], 1);
-            mbar_init(&sh.raw_empty[op][h], kConvWarps);
-        }
+        for (uint32_t s = 0; s < C::slots; ++s) mbar_init(&sh.raw_full[op][s], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        tc_copy<HD>(rows_src, p.n, t0, 0, 1, raw + op * 2 * C::raw, sh.raw_full[op], sh.raw_empty[op]);
+        tc_copy<HD>(rows_src, p.n, t0, 0, op ? 1 : min(nt, C::slots), op ? vs : ks, sh.raw_full[op], nullptr);
     }
     tc_fence_before();
     __syncthreads();
@@ -354,8 +349,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
     bool ok = true;
 
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
-        constexpr int OC = HD / 2, SC = (int)kTcKeys / 2;  // this thread's columns of O and of S
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 72;");
+        constexpr int SC = (int)kTcKeys / 2;  // this thread's columns of S
         const uint32_t quad = warp & 3, half = warp >> 2;
         const uint32_t rl = quad * 32 + lane, r = r0 + rl;
         const uint32_t lanes = tm + ((quad * 32u) << 16);
@@ -366,7 +361,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             // into V's slots; then each row is scaled and split by its two threads
             // (rows past the last stay as they are: nothing of them is written)
             constexpr int QL = HD / 32;
-            float* stage = reinterpret_cast<float*>(vs);
+            float* stage = reinterpret_cast<float*>(vs + C::slot);
             uint32_t tt = (r0 + warp * 16) / p.G, hh = (r0 + warp * 16) % p.G;
 #pragma unroll 1
             for (uint32_t b = warp * 16; b < warp * 16 + 16 && r0 + b < p.R; b += 8) {
@@ -398,12 +393,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                 }
             }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // V's rows follow
         asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
         // a quarter without rows is done: what the products hold in its lanes is not read
         if (quad < quads) {
         float qinv;
         {
-            const float4* src = reinterpret_cast<const float4*>(vs) + rl * (HD / 4);
+            const float4* src = reinterpret_cast<const float4*>(vs + C::slot) + rl * (HD / 4);
             float mult;
             tc_scale(sh.q_max[rl], mult, qinv);
             const float2 mult2 = make_float2(mult, mult);
@@ -422,50 +418,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         }
         tmem_wait_st();
         tc_fence_before();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full);
 
-        float2 o[OC / 2];
-#pragma unroll
-        for (int i = 0; i < OC / 2; ++i) o[i] = make_float2(0.f, 0.f);
-        float m = -INFINITY, l = 0.f, corr = 1.f;
+        float m = -INFINITY, l = 0.f;
         float* sc = nullptr;
         if constexpr (SCORES == 1) sc = p.scores + ((size_t)g * p.R + r) * p.sc_keys + half * SC;
         if constexpr (SCORES == 2) sc = p.scores + ((size_t)g * p.n + half * SC) * p.sc_rows + r;
-        // o = o * corr + O of tile t
-        auto take_output = [&](uint32_t t) {
-            const uint32_t b = t & 1;
-            ok = ok && mbar_wait_soon(&sh.o_full[b], (t >> 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            tc_fence_after();
-            const float scale = sh.v_scale[t % kTcRing] * 0x1p-14f;
-            if (__any_sync(0xffffffffu, corr != 1.f)) {
-                const float2 corr2 = make_float2(corr, corr);
-#pragma unroll
-                for (int i = 0; i < OC / 2; ++i) o[i] = mul2(o[i], corr2);
-            }
-            const float2 scale2 = make_float2(scale, scale);
-            constexpr int OW = OC < 32 ? 16 : 32;
-#pragma unroll
-            for (int c = 0; c < OC; c += OW) {
-                uint32_t x[OW];
-                if constexpr (OW == 32) tmem_ld32(lanes + C::o0 + b * 128 + half * OC + c, x);
-                else tmem_ld16(lanes + C::o0 + b * 128 + half * OC + c, x);
-#pragma unroll
-                for (int i = 0; i < OW / 2; ++i)
-                    o[c / 2 + i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2,
-                                        o[c / 2 + i]);
-            }
-            const unsigned long long bad = sh.v_bad[t % kTcRing];
-            if (bad && valid && (bad & tc_seen(a.mask, a.n_past, a.n_tokens, tok, (t0 + t) * kTcKeys))) {
-#pragma unroll
-                for (int i = 0; i < OC / 2; ++i)
-                    o[i] = make_float2(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.o_empty[b]);
-        };
         // a wait that gave up leaves the loop running (without waits) to its
         // end, since the two warps of a row meet at a barrier in it
         for (uint32_t t = 0; t < nt; ++t) {
@@ -524,6 +484,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             const float ref = mn == -INFINITY ? 0.f : mn;
             const float corr_t = ex2_approx(m - ref);
             m = mn;
+            if (half == 0) sh.corr[t % 4][rl] = corr_t;
             const float off = kPShift - ref;
             float2 sum = make_float2(0.f, 0.f);
             const float2 ct2 = make_float2(ct, ct), off2 = make_float2(off, off);
@@ -546,10 +507,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.p_full[b]);
-            if (t) take_output(t - 1);
-            corr = corr_t;
         }
-        take_output(nt - 1);
         sh.part_sum[half][rl] = l;
         asm volatile("barrier.cta.sync %0, 64;" ::"r"(4 + quad) : "memory");
         l = (l + sh.part_sum[half ^ 1][rl]) * 0x1p-14f;
@@ -561,10 +519,57 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
             if (SCORES && half == 0 && valid) p.stats[row] = make_float2(m == -INFINITY ? 0.f : m, f);
         }
+        if (half == 0) sh.factor[rl] = f;
+        asm volatile("barrier.cta.sync %0, 128;" ::"r"(8 + quad) : "memory");
+        }
+    } else if (warp < 16) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+        constexpr int OC = HD / 2;  // this thread's columns of O
+        const uint32_t quad = warp & 3, half = warp >> 2 & 1;
+        const uint32_t rl = quad * 32 + lane, r = r0 + rl;
+        const uint32_t lanes = tm + ((quad * 32u) << 16);
+        if (quad < quads) {
+        float2 o[OC / 2];
+#pragma unroll
+        for (int i = 0; i < OC / 2; ++i) o[i] = make_float2(0.f, 0.f);
+        for (uint32_t t = 0; t < nt; ++t) {  // o = o * corr + O of tile t
+            const uint32_t b = t & 1;
+            ok = ok && mbar_wait_soon(&sh.o_full[b], (t >> 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            const float scale = sh.v_scale[t % kTcRing] * 0x1p-14f, corr = sh.corr[t % 4][rl];
+            if (__any_sync(0xffffffffu, corr != 1.f)) {
+                const float2 corr2 = make_float2(corr, corr);
+#pragma unroll
+                for (int i = 0; i < OC / 2; ++i) o[i] = mul2(o[i], corr2);
+            }
+            const float2 scale2 = make_float2(scale, scale);
+            constexpr int OW = 16;
+#pragma unroll
+            for (int c = 0; c < OC; c += OW) {
+                uint32_t x[OW];
+                tmem_ld16(lanes + C::o0 + b * 128 + half * OC + c, x);
+#pragma unroll
+                for (int i = 0; i < OW / 2; ++i)
+                    o[c / 2 + i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2,
+                                        o[c / 2 + i]);
+            }
+            const unsigned long long bad = sh.v_bad[t % kTcRing];
+            if (bad && r < p.R && (bad & tc_seen(a.mask, a.n_past, a.n_tokens, r / p.G, (t0 + t) * kTcKeys))) {
+#pragma unroll
+                for (int i = 0; i < OC / 2; ++i)
+                    o[i] = make_float2(__uint_as_float(0x7FC00000u), __uint_as_float(0x7FC00000u));
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.o_empty[b]);
+        }
+        asm volatile("barrier.cta.sync %0, 128;" ::"r"(8 + quad) : "memory");
+        const float f = sh.factor[rl];
         // rows leave through K's slots (every MMA has completed), so that the
         // stores run along rows
         constexpr int OL = OC / 4, OX = OL < 8 ? OL - 1 : 7;  // float4s of half a row; their permutation
-        float4* stage = reinterpret_cast<float4*>(ks) + warp * 32 * OL;
+        float4* stage = reinterpret_cast<float4*>(ks) + (warp - 8) * 32 * OL;
 #pragma unroll
         for (int i = 0; i < OC; i += 4)
             stage[lane * OL + ((i / 4) ^ (lane & OX))] =
@@ -580,12 +585,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             *reinterpret_cast<float4*>(dst) = stage[i / OL * OL + ((i % OL) ^ (i / OL & OX))];
         }
         }
-    } else if (warp < 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        ok = tc_convert<HD, 0>(p.n, t0, nt, (int)threadIdx.x - 256, smem, sh);
+    } else if (warp < 20) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
+        ok = tc_convert<HD, 0>(p.n, t0, nt, (int)threadIdx.x - 512, smem, sh);
     } else if (warp < 24) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        ok = tc_convert<HD, 1>(p.n, t0, nt, (int)threadIdx.x - 512, smem, sh);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
+        ok = tc_convert<HD, 1>(p.n, t0, nt, (int)threadIdx.x - 640, smem, sh);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
         if (warp == 24) {
@@ -596,8 +601,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             ok = wait(&sh.q_full, 0);
             tc_fence_after();
             auto scores = [&](uint32_t t) -> bool {
-                const uint32_t slot = t % kTcSlots, b = t & 1;
-                if (!wait(&sh.k_full[slot], (t / kTcSlots) & 1)) return false;
+                const uint32_t slot = t % C::slots, b = t & 1;
+                if (!wait(&sh.k_full[slot], (t / C::slots) & 1)) return false;
                 tc_fence_after();
                 const uint64_t desc = smem_desc_sw128(ks + slot * C::slot);
                 const uint32_t d = tm + C::s0 + b * kTcKeys;
@@ -624,8 +629,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                     ok = false;
                     break;
                 }
-                const uint32_t slot = t % kTcSlots, b = t & 1;
-                ok = wait(&sh.v_full[slot], (t / kTcSlots) & 1) && wait(&sh.p_full[b], (t >> 1) & 1) &&
+                const uint32_t slot = t % C::slots, b = t & 1;
+                ok = wait(&sh.v_full[slot], (t / C::slots) & 1) && wait(&sh.p_full[b], (t >> 1) & 1) &&
                      (t < 2 || wait(&sh.o_empty[b], ((t >> 1) - 1) & 1));
                 if (!ok) break;
                 tc_fence_after();
@@ -652,8 +657,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         } else if (warp < 27 && lane == 0) {
             const uint32_t op = warp - 25;
             const float* rows_src = (op ? a.vcache : a.kcache) + (size_t)g * a.max_ctx * HD;
-            ok = tc_copy<HD>(rows_src, p.n, t0, 1, nt, raw + op * 2 * C::raw, sh.raw_full[op], sh.raw_empty[op]);
-            for (uint32_t h = 0; ok && h < 2; ++h) ok = mbar_wait_soon(&sh.raw_full[op][h], (nt - 1) & 1);
+            const uint32_t sent = op ? 1 : min(nt, C::slots);
+            ok = !op || nt == 1 || mbar_wait_soon(&sh.q_full, 0);
+            if (!ok) tc_landed<HD>(sent, sh.raw_full[op]);
+            else ok = tc_copy<HD>(rows_src, p.n, t0, sent, nt, op ? vs : ks, sh.raw_full[op],
+                                  op ? sh.v_empty : sh.k_empty) && tc_landed<HD>(nt, sh.raw_full[op]);
         }
     }
     if (!ok) atomicOr(p.err, kErrTreeWait);
