@@ -27,7 +27,8 @@
 // 8 heads x 16384 of 32768 rows of 128: 65 us (77 us without the streaming
 // hints); with a cluster barrier for each wave 166 us, and rows by bulk copies
 // through shared memory, whatever the buffers, 88 us at best: copies of a row
-// or two are too small for them.
+// or two are too small for them.  Half a wave, with the next one's loads sent
+// before its stores: 74 us; reads and writes do better apart.
 #include <cooperative_groups.h>
 
 #include <algorithm>

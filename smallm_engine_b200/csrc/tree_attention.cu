@@ -750,10 +750,10 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
 // the keys: a lane has a key and walks the rows; the CTAs behind the n_join
 // that join the splits find mc and sum of the rows from the splits themselves,
 // so that neither waits for the other (a kernel after the joining one: 38 us
-// instead of 35 us for one token over 16384 rows).  More rows run along themselves: the
-// lanes of a warp have a key's rows, 16 keys at a time, and their sums meet by
-// shuffles.
-constexpr int kWeightKeys = 16, kWeightWarps = 8;
+// instead of 35 us for one token over 16384 rows).  More rows run along
+// themselves: the lanes of a warp have a key's rows, 8 keys at a time (16: 2%
+// slower for 31 tokens over 12300 rows), and their sums meet by shuffles.
+constexpr int kWeightKeys = 8, kWeightWarps = 8;
 constexpr uint32_t kFewRows = 16;
 template <int HD>
 __global__ void __launch_bounds__(kMergeThreads) smallm_tree_weights_few_kernel(const TreeParams p, uint32_t n_join) {
