@@ -35,7 +35,8 @@ def select(be, w, n, keep, first, last, stream=None):
 @pytest.mark.parametrize("kv,n,keep,first,last", [
     (1, 1, 1, 0, 0), (2, 5, 3, 1, 1), (2, 40, 40, 0, 0), (3, 1000, 1, 0, 0), (2, 1021, 512, 4, 32),
     (8, 4096, 4095, 0, 0), (4, 5000, 300, 16, 284), (2, 70000, 33333, 7, 13), (8, 131072, 65536, 16, 256),
-    (1, 300001, 150000, 3, 0), (130, 500, 77, 5, 5), (3, 2048, 2000, 2000, 0), (3, 2049, 1025, 0, 1025)])
+    (1, 300001, 150000, 3, 0), (130, 500, 77, 5, 5), (3, 2048, 2000, 2000, 0), (3, 2049, 1025, 0, 1025),
+    (1, 400001, 200000, 5, 9), (150, 30001, 12345, 1, 2)])  # the last two: keys that do not fit shared memory
 @pytest.mark.parametrize("kind", ["lognormal", "ties", "equal", "special"])
 def test_select(be, kv, n, keep, first, last, kind):
     rng = np.random.default_rng(n + keep)
