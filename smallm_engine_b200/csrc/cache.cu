@@ -10,7 +10,7 @@
 // summed over the cluster's shared memory, then the bin that holds the rank.
 // (Digits of 11, 11 and 10 bits save a barrier, but then every CTA reads 8 KB
 // from each of 15 others for each digit: 37 us for 8 x 131072 keys where this
-// takes 23 us.)  Every larger key is kept, and of the equal ones the first few
+// takes 20 us.  Histograms read by more threads, fewer reads each: 21 us.)  Every larger key is kept, and of the equal ones the first few
 // in row order; rows come out ascending.  Bound by latency: one read of the
 // totals, five cluster barriers and as many rounds of remote reads.
 //
@@ -76,33 +76,50 @@ __global__ void __launch_bounds__(kSelThreads, 2)
     const uint32_t b0 = min(m, cr * per_cta), len = min(m, b0 + per_cta) - b0;
     const float* w = weights + (size_t)head * stride + n_first + b0;
     uint32_t* out = rows + (size_t)head * n_keep;
+    for (uint32_t i = tid; i < kSelPasses * kSelBins; i += kSelThreads) (&sh.hist[0][0])[i] = 0;
+    __syncthreads();
     pdl_wait();
     if (cr == 0) {
         for (uint32_t i = tid; i < n_first; i += kSelThreads) out[i] = i;
         for (uint32_t i = tid; i < n_last; i += kSelThreads) out[n_first + k + i] = n - n_last + i;
     }
     if (!k) return;
-    for (uint32_t i = tid; i < kSelPasses * kSelBins; i += kSelThreads) (&sh.hist[0][0])[i] = 0;
-    if (cached) {
-#pragma unroll 16
-        for (uint32_t i = tid; i < len; i += kSelThreads) cache[i] = total_key(__ldg(w + i));
+    // keys from the totals, counted by their first digit on the way (eight loads in
+    // flight; past the range they repeat its last total)
+    for (uint32_t i = tid; i < len; i += 8 * kSelThreads) {
+        float v[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) v[j] = __ldg(w + min(i + j * kSelThreads, len - 1));
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const uint32_t key = total_key(v[j]);
+            if (i + j * kSelThreads >= len) continue;
+            if (cached) cache[i + j * kSelThreads] = key;
+            atomicAdd(&sh.hist[0][key >> 23], 1u);
+        }
     }
-    auto key_of = [&](uint32_t i) { return cached ? cache[i] : total_key(w[i]); };
+    // (past the range: its last key)
+    auto key_of = [&](uint32_t i) {
+        i = min(i, len - 1);
+        return cached ? cache[i] : total_key(w[i]);
+    };
     __syncthreads();
     uint32_t prefix = 0, want = k, my_gt = 0;
+#pragma unroll 1
     for (int pass = 0; pass < kSelPasses; ++pass) {
         const int shift = pass == 0 ? 23 : (pass == 1 ? 15 : (pass == 2 ? 7 : 0));
         const uint32_t bins = pass == 0 ? 512u : (pass == 3 ? 128u : 256u);
-        const uint32_t high = pass == 0 ? 0u : ~(bins * (1u << shift) - 1u);
+        const uint32_t high = ~(bins * (1u << shift) - 1u);
         uint32_t* hist = sh.hist[pass];
-        // (four keys of a lane at a time; plain shared-memory adds, even where all
-        // keys share a bin: counting a warp's equal bins first cost more)
-        for (uint32_t i0 = tid; i0 - lane < len; i0 += 4 * kSelThreads) {
+        // (the first digit has been counted; four keys of a lane at a time; plain
+        // shared-memory adds, even where all keys share a bin: counting a warp's
+        // equal bins first cost more)
+        for (uint32_t i0 = tid; pass && i0 - lane < len; i0 += 4 * kSelThreads) {
             uint32_t bin[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t i = i0 + j * kSelThreads;
-                const uint32_t key = key_of(min(i, len - 1));
+                const uint32_t key = key_of(i);
                 bin[j] = i < len && (key & high) == prefix ? key >> shift & (bins - 1) : kSelBins;
             }
 #pragma unroll
@@ -178,7 +195,7 @@ __global__ void __launch_bounds__(kSelThreads, 2)
     uint32_t cg_ = 0, ce = 0;
 #pragma unroll 4
     for (uint32_t i = wb + lane; i - lane < we; i += 32) {
-        const uint32_t key = i < we ? key_of(i) : 0u;
+        const uint32_t key = key_of(i);
         cg_ += __popc(__ballot_sync(0xffffffffu, i < we && key > prefix));
         ce += __popc(__ballot_sync(0xffffffffu, i < we && key == prefix));
     }
@@ -192,7 +209,7 @@ __global__ void __launch_bounds__(kSelThreads, 2)
     const uint32_t lt = (1u << lane) - 1u;
 #pragma unroll 4
     for (uint32_t i = wb + lane; i - lane < we; i += 32) {
-        const uint32_t key = i < we ? key_of(i) : 0u;
+        const uint32_t key = key_of(i);
         const bool gt = i < we && key > prefix, eq = i < we && key == prefix;
         const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
         const uint32_t g = gt0 + __popc(bg & lt), e = eq0 + __popc(be & lt);
