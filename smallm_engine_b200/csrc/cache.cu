@@ -24,7 +24,7 @@
 // others how many waves it has loaded.  The distance rows[i] - (dst + i) never
 // shrinks along the list, so beyond the first few waves of an eviction that
 // has long been the case and nobody waits.  Bound by the bytes moved.
-// 8 heads x 16384 of 32768 rows of 128: 65 us (77 us without the streaming
+// 8 heads x 16384 of 32768 rows of 128: 63 us (77 us without the streaming
 // hints); with a cluster barrier for each wave 166 us, and rows by bulk copies
 // through shared memory, whatever the buffers, 88 us at best: copies of a row
 // or two are too small for them.  Half a wave, with the next one's loads sent
@@ -310,13 +310,20 @@ __global__ void __launch_bounds__(kMoveThreads, 2)
                    blockIdx.x / C * slice + tid % slice;
     const uint32_t pitch = hd / 4, step = kMoveThreads / slice, own = tid / slice;
     totals = totals && blockIdx.z == 0 && blockIdx.x < C ? totals + (size_t)blockIdx.y * a.max_ctx : nullptr;
-    uint32_t src[kMoveUnroll];  // the next wave's source rows
+    // the next wave's source rows, and which of them move (for the others the
+    // list's last row, which is never overwritten, is read and dropped: loads
+    // without conditions)
+    const uint32_t end_row = move_source(a, a.n_rows - 1);
+    uint32_t src[kMoveUnroll], next = 0;
     auto sources = [&](uint32_t w) {
         const uint32_t first = w * wave + cr * per;
+        next = 0;
 #pragma unroll
         for (int u = 0; u < kMoveUnroll; ++u) {
             const uint32_t i = first + own + u * step;
-            src[u] = i < a.n_rows ? move_source(a, i) : a.dst + i;
+            src[u] = move_source(a, min(i, a.n_rows - 1));
+            if (i < a.n_rows && src[u] != a.dst + i) next |= 1u << u;
+            else src[u] = end_row;
         }
     };
     sources(0);
@@ -325,13 +332,10 @@ __global__ void __launch_bounds__(kMoveThreads, 2)
     for (uint32_t w = 0; w < waves; ++w) {
         const uint32_t first = w * wave + cr * per;
         float4 v[kMoveUnroll];
-        uint32_t go = 0, seen = 0;
+        const uint32_t go = next;
+        uint32_t seen = 0;
 #pragma unroll
-        for (int u = 0; u < kMoveUnroll; ++u) {
-            if (src[u] == a.dst + first + own + u * step) continue;
-            v[u] = __ldcs(&base[(size_t)src[u] * pitch]);
-            go |= 1u << u;
-        }
+        for (int u = 0; u < kMoveUnroll; ++u) v[u] = __ldcs(&base[(size_t)src[u] * pitch]);
         float total[kMoveTotals] = {};
         if (totals) {
 #pragma unroll
@@ -346,8 +350,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2)
         if (w + 1 < waves) sources(w + 1);
 #pragma unroll
         for (int u = 0; u < kMoveUnroll; ++u)
-            if (go >> u & 1)
-                seen |= __float_as_uint(v[u].x) | __float_as_uint(v[u].y) | __float_as_uint(v[u].z) | __float_as_uint(v[u].w);
+            seen |= __float_as_uint(v[u].x) | __float_as_uint(v[u].y) | __float_as_uint(v[u].z) | __float_as_uint(v[u].w);
         // every thread's loads have returned (their values are in `seen`)
         asm volatile(
             "{\n .reg .pred p, q;\n setp.ne.u32 p, %0, 0;\n barrier.cta.red.or.pred q, 0, p;\n}" ::"r"(seen) : "memory");
