@@ -444,13 +444,15 @@ void launch_cache_select(const float* weights, uint32_t n_kv, uint32_t max_ctx, 
     if ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(rows)) & 3u)
         throw Error(SMALLM_ERR_INVALID, "cache_select: weights and rows must be 4-byte aligned");
     if (!n_kv || !n_keep) return;
-    // CTAs per head: a couple of keys per thread at least, two CTAs per SM in
-    // all, and no cluster left waiting for another to end
+    // CTAs per head: one up to 8 keys a thread (4 x 2500 keys 6.7 us, two CTAs
+    // 8.4 us), then clusters of 4 to 16 with as many a thread (8 x 8192: 8.5 us by
+    // four CTAs, 9.8 by two, 10.1 by one; 8 x 32768: 11.0 us by 8, 14.0 by 16);
+    // two CTAs per SM in all, and no cluster left waiting for another to end
     const uint32_t m = n - n_first - n_last, sms = (uint32_t)device_sm_count();
     const void* fn = (const void*)smallm_cache_select_kernel;
     set_smem_limit_once(fn, (int)(4 * kSelCached));
     uint32_t C = 1;
-    while (C < kSelMaxCluster && m > C * 2 * kSelThreads && n_kv * C <= sms) C *= 2;
+    while (C < kSelMaxCluster && m > C * 8 * kSelThreads && n_kv * C <= sms) C *= C == 1 ? 4 : 2;
     while (C > 1 && clusters_at_once(fn, C, kSelThreads, 4 * kSelCached) < n_kv) C /= 2;
     uint32_t per_cta = (m + C - 1) / C, cached = per_cta <= kSelCached;
     void* args[] = {&weights, &max_ctx, &n, &n_keep, &n_first, &n_last, &per_cta, &cached, &rows};
