@@ -27,6 +27,8 @@
 // is the cluster's start and barriers and the ranking.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "engine.h"
 #include "smallm_cuda.h"
@@ -381,10 +383,13 @@ void launch_logprobs(const LogprobArgs& a, cudaStream_t stream) {
          (a.n_top ? reinterpret_cast<uintptr_t>(a.top_ids) | reinterpret_cast<uintptr_t>(a.top_logprobs) : 0)) & 3u)
         throw Error(SMALLM_ERR_INVALID, "logprobs: pointers must be 4-byte aligned");
     if (!a.n_rows) return;
-    // CTAs per row: two per SM in all, each with a chunk to itself at least
+    // CTAs per row: one up to two chunks (63 x 8000: 3.4 us, by two CTAs 4.5 us),
+    // then two per SM in all, each with a chunk to itself at least (1 x 12338: 4.2
+    // us by four CTAs, 4.7 us by two; 1 x 32000, twenty alternatives: 7.4 us by
+    // eight, 12 us by two)
     const uint32_t nq = (a.vocab + 6) / 4, sms = (uint32_t)device_sm_count();
     uint32_t C = 1;
-    while (C < kLpMaxCluster && a.n_rows * C < 2 * sms && nq > C * kLpChunk) C *= 2;
+    while (C < kLpMaxCluster && a.n_rows * C < 2 * sms && nq > std::max(C, 2u) * kLpChunk) C *= 2;
     const void* fn = (const void*)smallm_logprobs_kernel;
     if (C > 8) SM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     set_smem_limit_once(fn, (int)sizeof(LpShared));
