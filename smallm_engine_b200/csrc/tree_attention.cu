@@ -754,7 +754,7 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
 // themselves: the lanes of a warp have a key's rows, 8 keys at a time (16: 2%
 // slower for 31 tokens over 12300 rows), and their sums meet by shuffles.  (With
 // mc and sum from the splits as well: 36 us instead of 30 us.)
-constexpr int kWeightKeys = 8, kWeightWarps = 8;
+constexpr int kWeightKeys = 8, kWeightWarps = 8, kWeightRows = 2;
 constexpr uint32_t kFewRows = 16;
 template <int HD>
 __global__ void __launch_bounds__(kMergeThreads) smallm_tree_weights_few_kernel(const TreeParams p, uint32_t n_join) {
@@ -806,17 +806,27 @@ __global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(
 #pragma unroll
     for (int k = 0; k < kWeightKeys; ++k) acc[k] = 0.f;
     // (loads without conditions, so that all are in flight: past the last key
-    // they read it again and the sum is dropped)
+    // or row they read it again and it is dropped)
     float* w = p.a.weights + (size_t)g * p.a.max_ctx;
     const float* s = p.scores + (size_t)g * p.n * p.sc_rows;
     const float old = w[min(key + lane % kWeightKeys, p.n - 1)];
-    for (uint32_t r = lane; r < p.R; r += 32) {
-        const float2 st = p.stats[(size_t)g * p.R + r];
-        float v[kWeightKeys];
+    const float2* stats = p.stats + (size_t)g * p.R;
+    for (uint32_t r = lane; r - lane < p.R; r += 32 * kWeightRows) {
+        float2 st[kWeightRows];
+        float v[kWeightRows][kWeightKeys];
 #pragma unroll
-        for (int k = 0; k < kWeightKeys; ++k) v[k] = __ldg(s + (size_t)min(key + k, p.n - 1) * p.sc_rows + r);
+        for (int j = 0; j < kWeightRows; ++j) {
+            const uint32_t rj = min(r + 32 * j, p.R - 1);
+            st[j] = stats[rj];
 #pragma unroll
-        for (int k = 0; k < kWeightKeys; ++k) acc[k] = fmaf(exp2f(fmaf(v[k], p.c, -st.x)), st.y, acc[k]);
+            for (int k = 0; k < kWeightKeys; ++k) v[j][k] = __ldg(s + (size_t)min(key + k, p.n - 1) * p.sc_rows + rj);
+        }
+#pragma unroll
+        for (int j = 0; j < kWeightRows; ++j) {
+            if (r + 32 * j >= p.R) break;
+#pragma unroll
+            for (int k = 0; k < kWeightKeys; ++k) acc[k] = fmaf(exp2f(fmaf(v[j][k], p.c, -st[j].x)), st[j].y, acc[k]);
+        }
     }
     float mine = 0.f;  // lane k: key k
 #pragma unroll
