@@ -36,11 +36,11 @@ struct TreeParams {
     uint32_t G, R, n, words;
     uint32_t n_split, tiles_per_split;
     uint32_t sc_rows;    // stored scores of a key: R, padded; 0: they run along keys
-    uint32_t sc_keys;    // ... and of a row: n, padded
+    uint32_t sc_keys;    // ... and of a row: n, padded to tiles
     float c;             // log2(e) / sqrt(hd)
     float* part_o;       // [n_split][n_kv * R][hd]
     float2* part_ml;     // [n_split][n_kv * R] (mc, sum)
-    float* scores;       // [n_kv][n][sc_rows] or [n_kv][R][sc_keys], raw q . K, -inf where unseen
+    float* scores;       // [n_kv][sc_keys / 4][sc_rows][4] or [n_kv][R][sc_keys], raw q . K, -inf where unseen
     float2* stats;       // [n_kv * R] (mc of the whole row, 1 / sum or 0)
     unsigned int* err;   // the device error word
 };
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         float m = -INFINITY, l = 0.f;
         float* sc = nullptr;
         if constexpr (SCORES == 1) sc = p.scores + ((size_t)g * p.R + r) * p.sc_keys + half * SC;
-        if constexpr (SCORES == 2) sc = p.scores + ((size_t)g * p.n + half * SC) * p.sc_rows + r;
+        if constexpr (SCORES == 2) sc = p.scores + ((size_t)g * p.sc_keys + half * SC) * p.sc_rows + 4 * r;
         // a wait that gave up leaves the loop running (without waits) to its
         // end, since the two warps of a row meet at a barrier in it
         for (uint32_t t = 0; t < nt; ++t) {
@@ -462,15 +462,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             }
             if (SCORES == 2 && valid) {  // the lanes' rows are neighbours
                 float* at = sc + (size_t)key0 * p.sc_rows;
-                const uint32_t left = p.n - key0 - min(p.n - key0, half * (uint32_t)SC);
-                if (left >= SC) {
 #pragma unroll
-                    for (int i = 0; i < SC; ++i) at[i * p.sc_rows] = s[i] * raw;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < SC; ++i)
-                        if (i < left) at[i * p.sc_rows] = s[i] * raw;
-                }
+                for (int i = 0; i < SC; i += 4)
+                    *reinterpret_cast<float4*>(at + i * p.sc_rows) =
+                        make_float4(s[i] * raw, s[i + 1] * raw, s[i + 2] * raw, s[i + 3] * raw);
             }
             float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -751,11 +746,14 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
 // that join the splits find mc and sum of the rows from the splits themselves,
 // so that neither waits for the other (a kernel after the joining one: 38 us
 // instead of 35 us for one token over 16384 rows).  More rows run along
-// themselves: the lanes of a warp have a key's rows, 8 keys at a time (16: 2%
-// slower for 31 tokens over 12300 rows), and their sums meet by shuffles.  (With
-// mc and sum from the splits as well: 36 us instead of 30 us.)
+// themselves, four keys of a row together: the lanes of a warp have the rows of 8
+// keys, and their sums meet by shuffles.  31 tokens over 12300 rows, 12 heads of
+// 128: 27.3 us, 19.7 us of them without the totals; 29.2 us with 16 keys a warp,
+// 29.1 us with a key's scores each 4 bytes of their own in its rows' stores, 36 us
+// with mc and sum from the splits as well.
 constexpr int kWeightKeys = 8, kWeightWarps = 8, kWeightRows = 2;
 constexpr uint32_t kFewRows = 16;
+static_assert(kTcKeys % (kWeightWarps * kWeightKeys) == 0 && kWeightKeys % 4 == 0, "a CTA's keys lie in a tile");
 template <int HD>
 __global__ void __launch_bounds__(kMergeThreads) smallm_tree_weights_few_kernel(const TreeParams p, uint32_t n_join) {
     __shared__ float2 stats[kFewRows];
@@ -805,27 +803,33 @@ __global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(
     float acc[kWeightKeys];
 #pragma unroll
     for (int k = 0; k < kWeightKeys; ++k) acc[k] = 0.f;
-    // (loads without conditions, so that all are in flight: past the last key
-    // or row they read it again and it is dropped)
+    // (loads without conditions, so that all are in flight: past the last row they
+    // read it again and it is dropped; the keys' scores are stored to a tile's end)
     float* w = p.a.weights + (size_t)g * p.a.max_ctx;
-    const float* s = p.scores + (size_t)g * p.n * p.sc_rows;
+    const float4* s = reinterpret_cast<const float4*>(p.scores + ((size_t)g * p.sc_keys + key) * p.sc_rows);
     const float old = w[min(key + lane % kWeightKeys, p.n - 1)];
     const float2* stats = p.stats + (size_t)g * p.R;
     for (uint32_t r = lane; r - lane < p.R; r += 32 * kWeightRows) {
         float2 st[kWeightRows];
-        float v[kWeightRows][kWeightKeys];
+        float4 v[kWeightRows][kWeightKeys / 4];
 #pragma unroll
         for (int j = 0; j < kWeightRows; ++j) {
             const uint32_t rj = min(r + 32 * j, p.R - 1);
             st[j] = stats[rj];
 #pragma unroll
-            for (int k = 0; k < kWeightKeys; ++k) v[j][k] = __ldg(s + (size_t)min(key + k, p.n - 1) * p.sc_rows + rj);
+            for (int k = 0; k < kWeightKeys / 4; ++k) v[j][k] = __ldg(s + k * p.sc_rows + rj);
         }
 #pragma unroll
         for (int j = 0; j < kWeightRows; ++j) {
             if (r + 32 * j >= p.R) break;
 #pragma unroll
-            for (int k = 0; k < kWeightKeys; ++k) acc[k] = fmaf(exp2f(fmaf(v[j][k], p.c, -st[j].x)), st[j].y, acc[k]);
+            for (int k = 0; k < kWeightKeys / 4; ++k) {
+                const float4 x = v[j][k];
+                acc[4 * k] = fmaf(exp2f(fmaf(x.x, p.c, -st[j].x)), st[j].y, acc[4 * k]);
+                acc[4 * k + 1] = fmaf(exp2f(fmaf(x.y, p.c, -st[j].x)), st[j].y, acc[4 * k + 1]);
+                acc[4 * k + 2] = fmaf(exp2f(fmaf(x.z, p.c, -st[j].x)), st[j].y, acc[4 * k + 2]);
+                acc[4 * k + 3] = fmaf(exp2f(fmaf(x.w, p.c, -st[j].x)), st[j].y, acc[4 * k + 3]);
+            }
         }
     }
     float mine = 0.f;  // lane k: key k
@@ -860,7 +864,7 @@ TreePlan tree_plan(uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t n_past
     t.off_scores = at;
     t.sc_rows = R > kFewRows ? (R + 31) / 32 * 32 : 0;
     t.sc_keys = tiles * kTcKeys;
-    if (weights) at += align256(4 * (size_t)n_kv * (t.sc_rows ? (size_t)n * t.sc_rows : (size_t)R * t.sc_keys));
+    if (weights) at += align256(4 * (size_t)n_kv * (t.sc_rows ? t.sc_rows : R) * t.sc_keys);
     t.off_stats = at;
     if (weights) at += align256(8 * rows);
     t.bytes = at;
