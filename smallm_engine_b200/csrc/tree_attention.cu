@@ -754,9 +754,10 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
 constexpr int kWeightKeys = 8, kWeightWarps = 8, kWeightRows = 2;
 constexpr uint32_t kFewRows = 16;
 static_assert(kTcKeys % (kWeightWarps * kWeightKeys) == 0 && kWeightKeys % 4 == 0, "a CTA's keys lie in a tile");
-template <int HD>
+// ROWS: R at most (half of kFewRows where that does: 2% of one token's call)
+template <int HD, uint32_t ROWS>
 __global__ void __launch_bounds__(kMergeThreads) smallm_tree_weights_few_kernel(const TreeParams p, uint32_t n_join) {
-    __shared__ float2 stats[kFewRows];
+    __shared__ float2 stats[ROWS];
     pdl_wait();
     if (blockIdx.x < n_join) {
         merge_row<HD>(p, blockIdx.x);
@@ -768,9 +769,9 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_weights_few_kernel(
     float* w = p.a.weights + (size_t)g * p.a.max_ctx + min(key, p.n - 1);
     const float* s = p.scores + (size_t)g * p.R * p.sc_keys + min(key, p.n - 1);
     const float old = *w;
-    float v[kFewRows];
+    float v[ROWS];
 #pragma unroll
-    for (uint32_t r = 0; r < kFewRows; ++r) v[r] = __ldg(s + (size_t)min(r, p.R - 1) * p.sc_keys);
+    for (uint32_t r = 0; r < ROWS; ++r) v[r] = __ldg(s + (size_t)min(r, p.R - 1) * p.sc_keys);
     for (uint32_t r = threadIdx.x >> 5; r < p.R; r += kMergeThreads / 32) {
         const size_t row = (size_t)g * p.R + r, rows = (size_t)p.a.n_kv * p.R;
         if (p.n_split == 1) {
@@ -792,7 +793,7 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_weights_few_kernel(
     if (key >= p.n) return;
     float acc = 0.f;
 #pragma unroll
-    for (uint32_t r = 0; r < kFewRows; ++r)
+    for (uint32_t r = 0; r < ROWS; ++r)
         if (r < p.R) acc = fmaf(exp2f(fmaf(v[r], p.c, -stats[r].x)), stats[r].y, acc);
     *w = old + acc;
 }
@@ -898,7 +899,9 @@ void launch_tree(const TreeParams& p, cudaStream_t stream) {
         uint32_t join = n_join;
         void* few[] = {&pp, &join};
         const uint32_t blocks = (p.n + kMergeThreads - 1) / kMergeThreads;
-        launch_kernel_ex((const void*)smallm_tree_weights_few_kernel<HD>, dim3(n_join + blocks * p.a.n_kv),
+        const void* sums = p.R <= kFewRows / 2 ? (const void*)smallm_tree_weights_few_kernel<HD, kFewRows / 2>
+                                               : (const void*)smallm_tree_weights_few_kernel<HD, kFewRows>;
+        launch_kernel_ex(sums, dim3(n_join + blocks * p.a.n_kv),
                          dim3(kMergeThreads), 0, stream, true, few);
         return;
     }
