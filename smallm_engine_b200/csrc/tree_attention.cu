@@ -357,14 +357,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         const bool valid = r < p.R;
         const uint32_t tok = valid ? r / p.G : 0;
         {
-            // q: the eight warps read 16 rows each, and their largest magnitudes,
+            // q: the eight warps read eight rows at a time, and their largest magnitudes,
             // into V's slots; then each row is scaled and split by its two threads
             // (rows past the last stay as they are: nothing of them is written)
             constexpr int QL = HD / 32;
             float* stage = reinterpret_cast<float*>(vs + C::slot);
-            uint32_t tt = (r0 + warp * 16) / p.G, hh = (r0 + warp * 16) % p.G;
 #pragma unroll 1
-            for (uint32_t b = warp * 16; b < warp * 16 + 16 && r0 + b < p.R; b += 8) {
+            for (uint32_t b = warp * 8; b < kTcRows && r0 + b < p.R; b += 64) {
+                uint32_t tt = (r0 + b) / p.G, hh = (r0 + b) % p.G;
                 alignas(16) float x[8][QL];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
