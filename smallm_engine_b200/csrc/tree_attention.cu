@@ -79,12 +79,13 @@ struct TreeParams {
 //     as the softmax one token over 16384 rows took 2% longer, with totals 6%.)
 // One token of 32 heads at 128 reads K and V at 6.3 TB/s from 16384 rows on
 // (the slope of its time; copies reach 6.5), after 8 us for two launches, the
-// first tile and the join.  Blocks with all 128 rows take about 2700 cycles a
-// tile where the products take 1536: conversion, softmax and the issue of the
-// products each work for some 2300 of them, in 5 instructions of 8 issue slots.
+// first tile and the join.  Blocks with all 128 rows take about 2800 cycles a
+// tile where the products take 1536: conversion works for 2600 of them, softmax
+// and the issue of the products for 2000, in 5 instructions of 8 issue slots.
 // Measured and not kept: smaller copies in a longer ring, a scale for each
-// converter warp instead of each tile, f32 FMAs for few rows, splits that join
-// through a cluster's shared memory.
+// converter warp instead of each tile, six converter warps (fewer registers) or
+// eight, f32 FMAs for few rows, splits that join through a cluster's shared
+// memory, the mask read before the wait for the products (spills).
 // An infinity or NaN of K or V would reach every row through 0 * inf, so it is
 // replaced by 0 and its key marked; rows that see the key turn to NaN.
 // Every wait is bounded; one that gives up raises bit 8 of the error word.
