@@ -102,7 +102,7 @@ struct TcTree {
     static constexpr uint32_t half = chunks * kTcKeys * 128;    // bytes of a tile's hi or lo
     static constexpr uint32_t slot = 2 * half;
     static constexpr uint32_t slots = HD > 64 ? 3 : 6;          // of K and of V each
-    static constexpr size_t smem = 1024 + 2ull * slots * slot + 8192;
+    static constexpr size_t smem = 1024 + 2ull * slots * slot + 12288;
     static_assert(kTcKeys * HD * 4 <= slot, "a tile is converted in place");
     static_assert(kTcRows * HD * 4 <= 2 * slot, "q and the output pass through two slots");
     static_assert(slots <= kTcMaxSlots && slots + 2 <= kTcRing, "scales outlive their slots by two tiles");
@@ -117,17 +117,19 @@ struct TcShared {
     uint64_t k_full[kTcMaxSlots], k_empty[kTcMaxSlots], v_full[kTcMaxSlots], v_empty[kTcMaxSlots];
     uint64_t raw_full[2][kTcMaxSlots];  // [K, V]
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, done;
-    float k_scale[kTcRing], v_scale[kTcRing];
+    float k_scale[kTcRing], v_exp[kTcRing];  // what a tile was divided by, V's as its exponent
     unsigned long long k_bad[kTcRing], v_bad[kTcRing];
     uint32_t wmax[2][2][kConvWarps];
     uint32_t tmem;
     float part_max[2][2][kTcRows];  // [tile % 2][half]
     float part_sum[2][kTcRows];
     uint32_t q_max[kTcRows];
-    float corr[4][kTcRows];  // [tile % 4] what a tile's maximum leaves of the output before it
+    // [tile % 4] what a tile's maximum leaves of the output before it, and the
+    // exponent of its own reference over the row's
+    float2 corr[4][kTcRows];
     float factor[kTcRows];
 };
-static_assert(sizeof(TcShared) <= 8192, "shared-memory tail");
+static_assert(sizeof(TcShared) <= 12288, "shared-memory tail");
 
 // 2^(14 - floor(log2 max)) of a magnitude given as f32 bits, and its inverse.
 __device__ __forceinline__ void tc_scale(uint32_t max_bits, float& mult, float& inv) {
@@ -162,6 +164,8 @@ __device__ __forceinline__ float ex2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 2^e of a whole e <= 127; 0 below -126.
+__device__ __forceinline__ float exp2_whole(float e) { return __int_as_float(max(__float2int_rn(e) + 127, 0) << 23); }
 // The largest of three magnitudes, NaN if any is.
 __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     float r;
@@ -273,7 +277,7 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
         }
         float mult, inv;
         tc_scale(mx, mult, inv);
-        if (tid == 0) (GROUP ? sh.v_scale : sh.k_scale)[ring] = inv;
+        if (tid == 0) (GROUP ? sh.v_exp : sh.k_scale)[ring] = GROUP ? (float)(int)(__float_as_uint(inv) >> 23) - 127.f : inv;
         uint8_t* const dsts[2] = {slots + slot * C::slot + dst0, slots + slot * C::slot + (dst0 ^ FLIP)};
         const float2 mult2 = make_float2(mult, mult);
 #pragma unroll
@@ -476,12 +480,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             asm volatile("barrier.cta.sync %0, 64;" ::"r"(4 + quad) : "memory");
             top = fmaxf(top, sh.part_max[b][half ^ 1][rl]);
             const float ct = raw * p.c;
-            const float mn = fmaxf(m, top == -INFINITY ? -INFINITY : ceilf(top * ct));
-            const float ref = mn == -INFINITY ? 0.f : mn;
-            const float corr_t = ex2_approx(m - ref);
+            // P is relative to the tile's own maximum mt: relative to the row's, a
+            // tile of small weights would lose bits that large values bring back
+            const float mt = top == -INFINITY ? -INFINITY : ceilf(top * ct);
+            const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.f : mn;
+            const float corr_t = ex2_approx(m - ref), part = ex2_approx(mt - ref);
             m = mn;
-            if (half == 0) sh.corr[t % 4][rl] = corr_t;
-            const float off = kPShift - ref;
+            if (half == 0) sh.corr[t % 4][rl] = make_float2(corr_t, mt - ref);
+            const float off = kPShift - (mt == -INFINITY ? 0.f : mt);
             float2 sum = make_float2(0.f, 0.f);
             const float2 ct2 = make_float2(ct, ct), off2 = make_float2(off, off);
 #pragma unroll
@@ -498,7 +504,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                 tmem_st8(sp + half * (SC / 2) + i / 2, hi);
                 tmem_st8(sp + 32 + half * (SC / 2) + i / 2, lo);
             }
-            l = fmaf(l, corr_t, sum.x + sum.y);
+            l = fmaf(l, corr_t, (sum.x + sum.y) * part);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -533,18 +539,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             ok = ok && mbar_wait_soon(&sh.o_full[b], (t >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
-            const float scale = sh.v_scale[t % kTcRing] * 0x1p-14f, corr = sh.corr[t % 4][rl];
-            if (__any_sync(0xffffffffu, corr != 1.f)) {
-                const float2 corr2 = make_float2(corr, corr);
+            const float2 tile = sh.corr[t % 4][rl];
+            const float e = tile.y + (sh.v_exp[t % kTcRing] - kPShift);  // O's exponent
+            if (__any_sync(0xffffffffu, tile.x != 1.f)) {
+                const float2 corr2 = make_float2(tile.x, tile.x);
 #pragma unroll
                 for (int i = 0; i < OC / 2; ++i) o[i] = mul2(o[i], corr2);
             }
+            // where 2^e is no normal f32 (tiny values), by 2^-100 and 2^(e + 100)
+            const bool tiny = __any_sync(0xffffffffu, e < -126.f && e > -226.f);
+            const float scale = exp2_whole(tiny ? e + 100.f : e);
             const float2 scale2 = make_float2(scale, scale);
             constexpr int OW = 16;
 #pragma unroll
             for (int c = 0; c < OC; c += OW) {
                 uint32_t x[OW];
                 tmem_ld16(lanes + C::o0 + b * 128 + half * OC + c, x);
+                if (tiny) {
+#pragma unroll
+                    for (int i = 0; i < OW; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * 0x1p-100f);
+                }
 #pragma unroll
                 for (int i = 0; i < OW / 2; ++i)
                     o[c / 2 + i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2,
