@@ -59,13 +59,22 @@ struct TreeParams {
 // that.  The small products are accumulated first.  (The result is nearer the
 // definition in 64 bits than f32 products and sums are: 1.1e-6 of its norm
 // against 3.6e-6 for 64 tokens over 32683 rows.)
+// One scale for a tile holds while no row of it is 2^14 times smaller than
+// another, which leaves every row 2^-25 of its own largest magnitude; else each
+// row has a scale of its own, so that no row takes bits from another, seen or
+// not: a K row's multiplies its scores, a V row's goes into P, which is then
+// relative to the token's largest product p |v| of the tile instead of its
+// largest p.  P therefore waits for V's scales (2% of 64 tokens over 32747 rows,
+// 6% of one token with totals over 16384; looked at before the exponentials: by
+// a wait after them, P in registers meanwhile, it was 13% and 14%).
 //   - warps 25 (K) and 26 (V) copy tiles of f32 rows with bulk copies into
 //     three slots each (six for rows of 64 or fewer).  (Loads through registers
 //     took the load/store unit twice as long as these copies and the reads of
 //     them.)
 //   - warps 16..19 (K) and 20..23 (V) convert in place: a group takes a tile
-//     into registers, finds its exponent and, once all have theirs, writes hi
-//     and lo in the MMA's swizzled layout over it.  (Slots of their own behind
+//     into registers, finds its exponent (or, by way of the slot again, those of
+//     its rows) and, once all have theirs, writes hi and lo in the MMA's
+//     swizzled layout over it.  (Slots of their own behind
 //     one tile of raw rows, for eight warps each: 3% slower at 64 tokens.)
 //   - warp 24 issues S = Q K^T (Q in tensor memory) and, a tile behind,
 //     O = P V (P in tensor memory, over S's columns; V MN-major);
@@ -95,6 +104,8 @@ constexpr uint32_t kTcRows = 128, kTcKeys = 64, kTcMaxSlots = 6, kTcRing = 8;
 constexpr uint32_t kTcThreads = 32 * 28;
 constexpr uint32_t kConvThreads = 128, kConvWarps = kConvThreads / 32;
 constexpr float kPShift = 14.f;
+constexpr float kTinyShift = 100.f;
+constexpr float kWideTile = 0x1p-14f;  // a tile's rows get scales of their own where one is this much smaller
 
 template <int HD>
 struct TcTree {
@@ -102,7 +113,7 @@ struct TcTree {
     static constexpr uint32_t half = chunks * kTcKeys * 128;    // bytes of a tile's hi or lo
     static constexpr uint32_t slot = 2 * half;
     static constexpr uint32_t slots = HD > 64 ? 3 : 6;          // of K and of V each
-    static constexpr size_t smem = 1024 + 2ull * slots * slot + 12288;
+    static constexpr size_t smem = 1024 + 2ull * slots * slot + 16384;
     static_assert(kTcKeys * HD * 4 <= slot, "a tile is converted in place");
     static_assert(kTcRows * HD * 4 <= 2 * slot, "q and the output pass through two slots");
     static_assert(slots <= kTcMaxSlots && slots + 2 <= kTcRing, "scales outlive their slots by two tiles");
@@ -115,21 +126,25 @@ struct TcTree {
 
 struct TcShared {
     uint64_t k_full[kTcMaxSlots], k_empty[kTcMaxSlots], v_full[kTcMaxSlots], v_empty[kTcMaxSlots];
+    uint64_t v_scaled[kTcMaxSlots];
     uint64_t raw_full[2][kTcMaxSlots];  // [K, V]
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, done;
     float k_scale[kTcRing], v_exp[kTcRing];  // what a tile was divided by, V's as its exponent
     unsigned long long k_bad[kTcRing], v_bad[kTcRing];
-    uint32_t wmax[2][2][kConvWarps];
+    uint2 wrange[2][2][kConvWarps];  // [K, V][tile % 2][warp] bits of the largest and smallest magnitude
     uint32_t tmem;
     float part_max[2][2][kTcRows];  // [tile % 2][half]
     float part_sum[2][kTcRows];
     uint32_t q_max[kTcRows];
-    // [tile % 4] what a tile's maximum leaves of the output before it, and the
-    // exponent of its own reference over the row's
+    // [tile % 4] what a tile's maximum leaves of the output before it, and what O is
+    // multiplied by; below f32's normal range -2^kTinyShift times that
     float2 corr[4][kTcRows];
     float factor[kTcRows];
+    float part_z[2][kTcRows];
+    // the rows' own scales, V's as exponents, for tiles with k_scale or v_exp infinite
+    alignas(16) float row_scale[2][kTcRing][kTcKeys];
 };
-static_assert(sizeof(TcShared) <= 12288, "shared-memory tail");
+static_assert(sizeof(TcShared) <= 16384, "shared-memory tail");
 
 // 2^(14 - floor(log2 max)) of a magnitude given as f32 bits, and its inverse.
 __device__ __forceinline__ void tc_scale(uint32_t max_bits, float& mult, float& inv) {
@@ -137,6 +152,8 @@ __device__ __forceinline__ void tc_scale(uint32_t max_bits, float& mult, float& 
     mult = __uint_as_float(f << 23);
     inv = __uint_as_float((254u - f) << 23);
 }
+// The exponent of an inverse that tc_scale gave: -126 to 114.
+__device__ __forceinline__ int scale_exp(float inv) { return (int)(__float_as_uint(inv) >> 23) - 127; }
 // hi = x rounded to f16, lo = (x - hi) rounded to f16, of two values (the
 // difference as a mixed fma by -1: a mixed subtraction takes the f16 operand
 // first, and the two negations after it cost an instruction each).
@@ -171,6 +188,31 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     float r;
     asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+__device__ __forceinline__ float f4_at(const float4& v, int i) {
+    return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+}
+// x = f(column, x) over N * 8 f32 columns of this thread's lane of tensor
+// memory, in a loop: for paths that are rarely taken and shall not hold
+// registers or much code.
+template <int N, typename F>
+__device__ __forceinline__ void tmem_map8(uint32_t taddr, F f) {
+#pragma unroll 1
+    for (int c = 0; c < 8 * N; c += 8) {
+        uint32_t x[8];
+        tmem_ld8(taddr + c, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(f(c + i, __uint_as_float(x[i])));
+        tmem_st8(taddr + c, x);
+    }
+    tmem_wait_st();
 }
 
 // Bits of the 64 keys from key0 that row token t sees.
@@ -228,7 +270,7 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
     uint8_t* slots = smem + GROUP * C::slots * C::slot;
     uint64_t* full = GROUP ? sh.v_full : sh.k_full;
     unsigned long long* bads = GROUP ? sh.v_bad : sh.k_bad;
-    auto& wmax = sh.wmax[GROUP];
+    auto& wrange = sh.wrange[GROUP];
     float4 x[N];
     // (STEP is a multiple of 4: the swizzle of odd units differs in one bit at most)
     const uint32_t dst0 =
@@ -240,44 +282,95 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
         const uint32_t left = n - (t0 + t) * kTcKeys;  // rows from the tile's first to the last
         const bool stuck = !mbar_wait_soon(&sh.raw_full[GROUP][slot], (t / C::slots) & 1);
         const float4* src = reinterpret_cast<const float4*>(slots + slot * C::slot) + tid;
-        float m = 0.f;
+        // the largest magnitude, and the smallest of three elements' largest ones: no
+        // row of the tile is smaller
+        float m = 0.f, low = INFINITY;
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = src[i * kConvThreads];
         if (left < kTcKeys) {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
+            for (int i = 0; i < N; ++i) {
                 if (row0 + i * STEP >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+                const float u = max3_abs_nan(x[i].x, x[i].y, x[i].z);
+                m = max3_abs_nan(m, u, x[i].w);
+                if (row0 + i * STEP < left) low = fminf(low, u);
+            }
+        } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) m = max3_abs_nan(max3_abs_nan(m, x[i].x, x[i].y), x[i].z, x[i].w);
-        const uint32_t mw = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-        if (lane == 0) wmax[t & 1][cw] = mw;
+            for (int i = 0; i < N; i += 2) {
+                const float u = max3_abs_nan(x[i].x, x[i].y, x[i].z);
+                const float v = max3_abs_nan(x[i + 1].x, x[i + 1].y, x[i + 1].z);
+                m = max3_abs_nan(max3_abs_nan(m, u, x[i].w), v, x[i + 1].w);
+                low = min3(low, u, v);
+            }
+        }
+        auto put_range = [&](float most, float least) {
+            const uint32_t a = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+            const uint32_t b = __reduce_min_sync(0xffffffffu, __float_as_uint(least));
+            if (lane == 0) wrange[t & 1][cw] = make_uint2(a, b);
+        };
+        uint32_t mx;
+        auto get_range = [&] {  // true: rows may differ too much for one scale
+            const uint2 r = wrange[t & 1][lane % kConvWarps];
+            mx = __reduce_max_sync(0xffffffffu, r.x);
+            return __uint_as_float(__reduce_min_sync(0xffffffffu, r.y)) < __uint_as_float(mx) * kWideTile;
+        };
+        put_range(m, low);
         if (tid == 0) bads[ring] = 0;
         // (past this barrier every thread has its elements)
         if (conv_any(1 + GROUP, stuck)) return false;
-        uint32_t mx = __reduce_max_sync(0xffffffffu, wmax[t & 1][lane % kConvWarps]);
-        if (mx >= 0x7F800000u) {  // the same for the whole group: clean the tile
-            m = 0.f;
-            uint32_t hurt = 0;  // this thread's units that held any
-            auto clean = [&](float& v, int i) {
-                if (!(fabsf(v) < INFINITY)) {
-                    v = 0.f;
-                    hurt |= 1u << i;
-                }
-                m = fmaxf(m, fabsf(v));
-            };
+        bool wide = get_range();
+        if (wide || mx >= 0x7F800000u) {  // the same for the whole group; by way of the slot, to spare registers
+            float4* own = reinterpret_cast<float4*>(slots + slot * C::slot) + tid;
+            auto row_max = [&](const float4& v) {
+                float r = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 #pragma unroll
-            for (int i = 0; i < N; ++i) clean(x[i].x, i), clean(x[i].y, i), clean(x[i].z, i), clean(x[i].w, i);
-            for (; hurt; hurt &= hurt - 1) atomicOr(&bads[ring], 1ull << (row0 + (__ffs(hurt) - 1) * STEP));
-            const uint32_t m2 = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-            conv_any(1 + GROUP, false);  // wmax has been read by all
-            if (lane == 0) wmax[t & 1][cw] = m2;
+                for (int o = W / 2; o > 0; o >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, o));
+                return r;
+            };
+            // whole rows' magnitudes, infinities and NaN cleaned; rows of zeros do not count
+            m = 0.f, low = INFINITY;
+#pragma unroll 1
+            for (uint32_t i = 0, row = row0; i < (uint32_t)N; ++i, row += STEP) {
+                float4 v = own[i * kConvThreads];
+                if (row >= left) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                bool hurt = false;
+                auto clean = [&](float& e) {
+                    if (!(fabsf(e) < INFINITY)) e = 0.f, hurt = true;
+                };
+                clean(v.x), clean(v.y), clean(v.z), clean(v.w);
+                if (hurt) atomicOr(&bads[ring], 1ull << row);
+                own[i * kConvThreads] = v;
+                const float r = row_max(v);
+                m = fmaxf(m, r);
+                if (r > 0.f) low = fminf(low, r);
+            }
+            conv_any(1 + GROUP, false);  // the ranges have been read by all
+            put_range(m, low);
             conv_any(1 + GROUP, false);
-            mx = __reduce_max_sync(0xffffffffu, wmax[t & 1][lane % kConvWarps]);
+            wide = get_range();
+            if (wide) {
+#pragma unroll 1
+                for (uint32_t i = 0, row = row0; i < (uint32_t)N; ++i, row += STEP) {
+                    float4 v = own[i * kConvThreads];
+                    float mult, inv;
+                    tc_scale(__float_as_uint(row_max(v)), mult, inv);
+                    own[i * kConvThreads] = make_float4(v.x * mult, v.y * mult, v.z * mult, v.w * mult);
+                    if (c4 == 0) sh.row_scale[GROUP][ring][row] = GROUP ? (float)scale_exp(inv) : inv;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = src[i * kConvThreads];
+            conv_any(1 + GROUP, false);  // as above: every thread has its elements
         }
         float mult, inv;
         tc_scale(mx, mult, inv);
-        if (tid == 0) (GROUP ? sh.v_exp : sh.k_scale)[ring] = GROUP ? (float)(int)(__float_as_uint(inv) >> 23) - 127.f : inv;
+        if (tid == 0) (GROUP ? sh.v_exp : sh.k_scale)[ring] = wide ? INFINITY : (GROUP ? (float)scale_exp(inv) : inv);
+        if (wide) mult = 1.f;
+        if (GROUP) {  // P needs V's scales, and sooner than the products need V
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.v_scaled[slot]);
+        }
         uint8_t* const dsts[2] = {slots + slot * C::slot + dst0, slots + slot * C::slot + (dst0 ^ FLIP)};
         const float2 mult2 = make_float2(mult, mult);
 #pragma unroll
@@ -314,11 +407,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
 
     pdl_launch_dependents();  // the joining kernel's launch overlaps this one
     const uint32_t quads = min(4u, (p.R - r0 + 31) / 32);  // warps' row quarters that hold rows
+    const uint32_t v_first = C::slots - (quads * (32 * HD * 4) + C::slot - 1) / C::slot;  // V's slots before q's
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < C::slots; ++i) {
             mbar_init(&sh.k_full[i], kConvWarps);
             mbar_init(&sh.k_empty[i], 1);
             mbar_init(&sh.v_full[i], kConvWarps);
+            mbar_init(&sh.v_scaled[i], kConvWarps);
             mbar_init(&sh.v_empty[i], 1);
         }
         for (uint32_t b = 0; b < 2; ++b) {
@@ -339,13 +434,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
     }
     pdl_wait();  // what came before on the stream has ended
     // the first tiles' rows are on their way while the CTA is set up (copying
-    // warps: 25 K, 26 V; V's second and third slot hold q first)
+    // warps: 25 K, 26 V; the last of V's slots hold q first)
     if (warp - 25 < 2 && lane == 0) {
         const uint32_t op = warp - 25;
         const float* rows_src = (op ? a.vcache : a.kcache) + (size_t)g * a.max_ctx * HD;
         for (uint32_t s = 0; s < C::slots; ++s) mbar_init(&sh.raw_full[op][s], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        tc_copy<HD>(rows_src, p.n, t0, 0, op ? 1 : min(nt, C::slots), op ? vs : ks, sh.raw_full[op], nullptr);
+        tc_copy<HD>(rows_src, p.n, t0, 0, min(nt, op ? v_first : C::slots), op ? vs : ks, sh.raw_full[op], nullptr);
     }
     tc_fence_before();
     __syncthreads();
@@ -366,7 +461,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             // into V's slots; then each row is scaled and split by its two threads
             // (rows past the last stay as they are: nothing of them is written)
             constexpr int QL = HD / 32;
-            float* stage = reinterpret_cast<float*>(vs + C::slot);
+            float* stage = reinterpret_cast<float*>(vs + v_first * C::slot);
 #pragma unroll 1
             for (uint32_t b = warp * 8; b < kTcRows && r0 + b < p.R; b += 64) {
                 uint32_t tt = (r0 + b) / p.G, hh = (r0 + b) % p.G;
@@ -404,7 +499,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         if (quad < quads) {
         float qinv;
         {
-            const float4* src = reinterpret_cast<const float4*>(vs + C::slot) + rl * (HD / 4);
+            const float4* src = reinterpret_cast<const float4*>(vs + v_first * C::slot) + rl * (HD / 4);
             float mult;
             tc_scale(sh.q_max[rl], mult, qinv);
             const float2 mult2 = make_float2(mult, mult);
@@ -435,22 +530,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         // end, since the two warps of a row meet at a barrier in it
         for (uint32_t t = 0; t < nt; ++t) {
             const uint32_t b = t & 1, key0 = (t0 + t) * kTcKeys, ring = t % kTcRing;
-            ok = ok && mbar_wait_soon(&sh.s_full[b], (t >> 1) & 1);
+            ok = ok && mbar_wait_soon(&sh.v_scaled[t % C::slots], (t / C::slots) & 1) &&
+                 mbar_wait_soon(&sh.s_full[b], (t >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             const uint32_t sp = lanes + C::s0 + b * kTcKeys;
             const float k_scale = sh.k_scale[ring];
             const unsigned long long bad = sh.k_bad[ring];
             float s[SC];
-            {
-                uint32_t x[32];
-                tmem_ld32(sp + half * SC, x);
+            auto get_scores = [&] {
+                tmem_ld32(sp + half * SC, reinterpret_cast<uint32_t(&)[SC]>(s));
+            };
+            auto put_scores = [&] {
 #pragma unroll
-                for (int i = 0; i < SC; ++i) s[i] = __uint_as_float(x[i]);
-            }
+                for (int i = 0; i < SC; i += 8)
+                    tmem_st8(sp + half * SC + i, reinterpret_cast<const uint32_t(&)[8]>(s[i]));
+                tmem_wait_st();
+            };
+            get_scores();
             // (never 0: an unseen key's -inf times it stays -inf)
-            const float raw = fmaxf(qinv * k_scale, 0x1p-120f);
-            if (key0 + kTcKeys > a.n_past || bad) {
+            const float raw = k_scale == INFINITY ? 1.f : fmaxf(qinv * k_scale, 0x1p-120f);
+            if (key0 + kTcKeys > a.n_past || bad || k_scale == INFINITY) {
+                if (k_scale == INFINITY) {
+                    // the keys' own scales, by way of tensor memory (spares registers); q's
+                    // first where it is below 1: no overflow on the way
+                    const float4* ks = reinterpret_cast<const float4*>(&sh.row_scale[0][ring][half * SC]);
+                    const float qa = fminf(qinv, 1.f), qb = fmaxf(qinv, 1.f);
+                    tmem_map8<SC / 8>(sp + half * SC,
+                                      [&](int i, float x) { return x * qa * f4_at(ks[i / 4], i) * qb; });
+                    get_scores();
+                }
                 const uint32_t seen = (uint32_t)(tc_seen(a.mask, a.n_past, a.n_tokens, tok, key0) >> (half * SC));
                 const uint32_t hurt = (uint32_t)(bad >> (half * SC));
 #pragma unroll
@@ -479,15 +588,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             sh.part_max[b][half][rl] = top;
             asm volatile("barrier.cta.sync %0, 64;" ::"r"(4 + quad) : "memory");
             top = fmaxf(top, sh.part_max[b][half ^ 1][rl]);
-            const float ct = raw * p.c;
+            float ct = raw * p.c;
             // P is relative to the tile's own maximum mt: relative to the row's, a
             // tile of small weights would lose bits that large values bring back
             const float mt = top == -INFINITY ? -INFINITY : ceilf(top * ct);
             const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.f : mn;
             const float corr_t = ex2_approx(m - ref), part = ex2_approx(mt - ref);
             m = mn;
-            if (half == 0) sh.corr[t % 4][rl] = make_float2(corr_t, mt - ref);
-            const float off = kPShift - (mt == -INFINITY ? 0.f : mt);
+            float off = kPShift - (mt == -INFINITY ? 0.f : mt);
+            float z = 0.f, wsum = 0.f;  // P's exponent besides mt's; sum of the weights where P holds more
+            const float v_exp = sh.v_exp[ring];
+            const bool wide_v = v_exp == INFINITY;
+            if (wide_v) {
+                // P takes up the scales of V's rows, relative to the token's largest
+                // product among the keys that it sees (the halves meet as above)
+                const float4* vx = reinterpret_cast<const float4*>(&sh.row_scale[1][ring][half * SC]);
+                z = -INFINITY;
+                put_scores();
+                tmem_map8<SC / 8>(sp + half * SC, [&](int i, float x) {
+                    const float y = fmaf(x, ct, off);
+                    wsum += ex2_approx(y);
+                    z = fmaxf(z, y + f4_at(vx[i / 4], i));
+                    return y + f4_at(vx[i / 4], i);
+                });
+                get_scores();
+                sh.part_z[half][rl] = z;
+                asm volatile("barrier.cta.sync %0, 64;" ::"r"(4 + quad) : "memory");
+                z = fmaxf(z, sh.part_z[half ^ 1][rl]);
+                z = z == -INFINITY ? 0.f : ceilf(z) - kPShift;
+                ct = 1.f, off = -z;
+            }
             float2 sum = make_float2(0.f, 0.f);
             const float2 ct2 = make_float2(ct, ct), off2 = make_float2(off, off);
 #pragma unroll
@@ -504,7 +634,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                 tmem_st8(sp + half * (SC / 2) + i / 2, hi);
                 tmem_st8(sp + 32 + half * (SC / 2) + i / 2, lo);
             }
-            l = fmaf(l, corr_t, (sum.x + sum.y) * part);
+            if (!wide_v) wsum = sum.x + sum.y;
+            if (half == 0) {
+                const float e = mt - ref + z + (wide_v ? 0.f : v_exp) - kPShift;  // O's exponent
+                const bool tiny = e < -126.f && e > -126.f - kTinyShift;
+                sh.corr[t % 4][rl] = make_float2(corr_t, tiny ? -exp2_whole(e + kTinyShift) : exp2_whole(e));
+            }
+            l = fmaf(l, corr_t, wsum * part);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -540,25 +676,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             const float2 tile = sh.corr[t % 4][rl];
-            const float e = tile.y + (sh.v_exp[t % kTcRing] - kPShift);  // O's exponent
-            if (__any_sync(0xffffffffu, tile.x != 1.f)) {
+            if (__any_sync(0xffffffffu, tile.x != 1.f || tile.y < 0.f)) {
+                if (__any_sync(0xffffffffu, tile.y < 0.f)) {
+                    const float down = tile.y < 0.f ? exp2_whole(-kTinyShift) : 1.f;
+                    tmem_map8<OC / 8>(lanes + C::o0 + b * 128 + half * OC, [&](int, float x) { return x * down; });
+                }
                 const float2 corr2 = make_float2(tile.x, tile.x);
 #pragma unroll
                 for (int i = 0; i < OC / 2; ++i) o[i] = mul2(o[i], corr2);
             }
-            // where 2^e is no normal f32 (tiny values), by 2^-100 and 2^(e + 100)
-            const bool tiny = __any_sync(0xffffffffu, e < -126.f && e > -226.f);
-            const float scale = exp2_whole(tiny ? e + 100.f : e);
+            const float scale = fabsf(tile.y);
             const float2 scale2 = make_float2(scale, scale);
             constexpr int OW = 16;
 #pragma unroll
             for (int c = 0; c < OC; c += OW) {
                 uint32_t x[OW];
                 tmem_ld16(lanes + C::o0 + b * 128 + half * OC + c, x);
-                if (tiny) {
-#pragma unroll
-                    for (int i = 0; i < OW; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * 0x1p-100f);
-                }
 #pragma unroll
                 for (int i = 0; i < OW / 2; ++i)
                     o[c / 2 + i] = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2,
@@ -680,8 +813,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         } else if (warp < 27 && lane == 0) {
             const uint32_t op = warp - 25;
             const float* rows_src = (op ? a.vcache : a.kcache) + (size_t)g * a.max_ctx * HD;
-            const uint32_t sent = op ? 1 : min(nt, C::slots);
-            ok = !op || nt == 1 || mbar_wait_soon(&sh.q_full, 0);
+            const uint32_t sent = min(nt, op ? v_first : C::slots);
+            ok = !op || nt == sent || mbar_wait_soon(&sh.q_full, 0);
             if (!ok) tc_landed<HD>(sent, sh.raw_full[op]);
             else ok = tc_copy<HD>(rows_src, p.n, t0, sent, nt, op ? vs : ks, sh.raw_full[op],
                                   op ? sh.v_empty : sh.k_empty) && tc_landed<HD>(nt, sh.raw_full[op]);

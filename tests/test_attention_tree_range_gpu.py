@@ -1,6 +1,13 @@
-"""Attention of drafted tokens where magnitudes differ widely, against the definition in
-64 bits with the tolerance derived in test_attention_tree_gpu.py, unless a test says
-otherwise."""
+"""Attention of drafted tokens where magnitudes differ widely: large finite rows
+that a token does not see or gives no weight, scores beyond f32's range or too
+large for a weight to be told from its neighbour's, sums of values beyond f32's
+range, and totals of rows that a token whose result is not finite does not see.
+
+Against the definition in 64 bits with the tolerance derived in
+test_attention_tree_gpu.py, unless a test says otherwise.  That tolerance also
+covers how rows enter: an element is off by at most 2^-23 of itself or 2^-25 of
+its row's largest magnitude, and a weight's product with its row by 2^-39 of
+the token's largest such product among 64 keys."""
 import numpy as np
 import pytest
 import torch
@@ -22,6 +29,51 @@ def unit_rows(shape, seed):
     return 2 * torch.rand(shape, device="cuda", generator=g) - 1
 
 
+@pytest.mark.parametrize("H,kv,hd", [(8, 2, 128), (6, 3, 64), (4, 1, 32)])
+@pytest.mark.parametrize("T", [6, 70])
+@pytest.mark.parametrize("which", ["k", "v", "kv"])
+@pytest.mark.parametrize("f", BIG)
+def test_large_unseen_row(be, H, kv, hd, T, which, f):
+    """A drafted row that only one token sees holds large finite values, as an
+    unwritten slot may: the other tokens answer as if it were not there."""
+    n = 61
+    seen = chain(T)
+    seen[:, 2] = False
+    seen[4, 2] = True
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 5)
+    for x, name in ((k, "k"), (v, "v")):
+        if name in which:
+            x[:, n + 2] = f * unit_rows((kv, hd), 3)
+    w = torch.zeros(kv, n + T, device="cuda")
+    out = run(be, q, k, v, H, n, T, mask=words_of(seen))
+    seen[4, 2] = False
+    k[:, n + 2] = 0
+    v[:, n + 2] = 0
+    ref = run(be, q, k, v, H, n, T, mask=words_of(seen), weights=w)
+    check(ref, q, k, v, H, n, T, seen, w, torch.zeros_like(w))
+    out[4] = ref[4]
+    check(out, q, k, v, H, n, T, seen)
+
+
+@pytest.mark.parametrize("T", [1, 33])
+@pytest.mark.parametrize("f", BIG)
+@pytest.mark.parametrize("drop", [0.0, 1e-13, 1e-25, 0.03])
+def test_large_value_of_small_weight(be, T, f, drop):
+    """A seen row whose V is large: what its weight makes of it is the result,
+    and where that is nothing the other rows are.  Its key takes the score down
+    (or, at `drop` 0, far below what f32 can weigh)."""
+    H, kv, hd, n = 8, 2, 128, 300
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 13)
+    q[:, 0::hd] = 8.0
+    k[:, :, 0] = 0.0
+    down = 1000.0 if drop == 0.0 else -np.log(drop)
+    k[:, 77, 0] = -down * hd ** 0.5 / 8.0
+    v[:, 77] = f * unit_rows((kv, hd), 2)
+    w = torch.zeros(kv, n + T, device="cuda")
+    out = run(be, q, k, v, H, n, T, weights=w)
+    check(out, q, k, v, H, n, T, chain(T), w, torch.zeros_like(w))
+
+
 @pytest.mark.parametrize("T", [1, 33])
 @pytest.mark.parametrize("n", [190, 5000])
 @pytest.mark.parametrize("f,drop", [(1e12, 1e-9), (1e20, 1e-15), (1e30, 1e-25)])
@@ -35,6 +87,37 @@ def test_tile_of_large_values_with_small_weights(be, T, n, f, drop):
     v[:, 64:128] *= f
     out = run(be, q, k, v, H, n, T)
     check(out, q, k, v, H, n, T, chain(T))
+
+
+@pytest.mark.parametrize("T", [1, 33])
+@pytest.mark.parametrize("f", BIG[1:])
+def test_large_key_far_below(be, T, f):
+    """A seen row with a large key that every token scores far below the others
+    (beyond f32's range for the largest) has no weight and changes nothing."""
+    H, kv, hd, n = 8, 2, 128, 300
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 19)
+    q[:, 0::hd] = 8.0
+    k[:, 77] = 0.0
+    k[:, 77, 0] = -f
+    w = torch.zeros(kv, n + T, device="cuda")
+    out = run(be, q, k, v, H, n, T, weights=w)
+    assert float(w[:, 77].abs().max()) == 0.0
+    rows = [r for r in range(n + T) if r != 77]
+    check(out, q, k[:, rows], v[:, rows], H, n - 1, T, chain(T), w[:, rows], torch.zeros_like(w[:, rows]))
+
+
+@pytest.mark.parametrize("T", [1, 33])
+def test_rows_of_every_size(be, T):
+    """Every row of K and V has a size of its own, over fifty powers of ten; the
+    scores stay ordinary, since q is small where K is large."""
+    H, kv, hd, n = 8, 2, 64, 500
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 23)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    k *= torch.pow(10.0, -30.0 * torch.rand(kv, n + T, 1, device="cuda", generator=g))
+    v *= torch.pow(10.0, 50.0 * torch.rand(kv, n + T, 1, device="cuda", generator=g) - 25.0)
+    w = torch.zeros(kv, n + T, device="cuda")
+    out = run(be, q, k, v, H, n, T, weights=w)
+    check(out, q, k, v, H, n, T, chain(T), w, torch.zeros_like(w))
 
 
 @pytest.mark.parametrize("n,T", [(60, 1), (4000, 1), (4000, 33), (20000, 2)])
