@@ -240,9 +240,9 @@ int smallm_attention_noalloc(smallm_ctx* ctx, const float* q_dev, const float* k
  * hold, NaN and infinities included; where a seen row or q holds them, or a
  * score passes f32's range, the output is not finite.
  *
- * Accuracy: an element of q, K or V enters to 2^-23 of itself or 2^-25 of the
+ * Accuracy: an element of q, K or V enters to 2^-22 of itself or 2^-25 of the
  * largest magnitude of its row of head_dim, a weight's product with its row of
- * V to 2^-23 of itself or 2^-39 of the token's largest such product among 64
+ * V to 2^-22 of itself or 2^-39 of the token's largest such product among 64
  * neighbouring rows; products and sums are f32's.  A weight below 2^-126 of
  * the token's largest may count as 0.
  *

@@ -522,6 +522,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full);
 
+        // the largest of the warp's rows (as bits: no sign, no NaN)
+        const float qtop = __uint_as_float(__reduce_max_sync(0xffffffffu, valid ? __float_as_uint(qinv) : 0u));
         float m = -INFINITY, l = 0.f;
         float* sc = nullptr;
         if constexpr (SCORES == 1) sc = p.scores + ((size_t)g * p.R + r) * p.sc_keys + half * SC;
@@ -549,15 +551,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             };
             get_scores();
             // (never 0: an unseen key's -inf times it stays -inf)
-            const float raw = k_scale == INFINITY ? 1.f : fmaxf(qinv * k_scale, 0x1p-120f);
-            if (key0 + kTcKeys > a.n_past || bad || k_scale == INFINITY) {
-                if (k_scale == INFINITY) {
-                    // the keys' own scales, by way of tensor memory (spares registers); q's
-                    // first where it is below 1: no overflow on the way
-                    const float4* ks = reinterpret_cast<const float4*>(&sh.row_scale[0][ring][half * SC]);
+            // keys with scales of their own, or a factor beyond f32's range (which no score need be)
+            const bool far = !(qtop * k_scale < INFINITY);
+            const float raw = far ? 1.f : fmaxf(qinv * k_scale, 0x1p-120f);
+            if (key0 + kTcKeys > a.n_past || bad || far) {
+                if (far) {
+                    // scores of their own size, by way of tensor memory (spares registers);
+                    // q's scale first where it is below 1: no overflow on the way
+                    const float* ks = &sh.row_scale[0][ring][half * SC];
                     const float qa = fminf(qinv, 1.f), qb = fmaxf(qinv, 1.f);
-                    tmem_map8<SC / 8>(sp + half * SC,
-                                      [&](int i, float x) { return x * qa * f4_at(ks[i / 4], i) * qb; });
+                    tmem_map8<SC / 8>(sp + half * SC, [&](int i, float x) {
+                        return x * qa * (k_scale == INFINITY ? ks[i] : k_scale) * qb;
+                    });
                     get_scores();
                 }
                 const uint32_t seen = (uint32_t)(tc_seen(a.mask, a.n_past, a.n_tokens, tok, key0) >> (half * SC));

@@ -5,7 +5,7 @@ range, and totals of rows that a token whose result is not finite does not see.
 
 Against the definition in 64 bits with the tolerance derived in
 test_attention_tree_gpu.py, unless a test says otherwise.  That tolerance also
-covers how rows enter: an element is off by at most 2^-23 of itself or 2^-25 of
+covers how rows enter: an element is off by at most 2^-22 of itself or 2^-25 of
 its row's largest magnitude, and a weight's product with its row by 2^-39 of
 the token's largest such product among 64 keys."""
 import numpy as np
@@ -118,6 +118,19 @@ def test_rows_of_every_size(be, T):
     w = torch.zeros(kv, n + T, device="cuda")
     out = run(be, q, k, v, H, n, T, weights=w)
     check(out, q, k, v, H, n, T, chain(T), w, torch.zeros_like(w))
+
+
+@pytest.mark.parametrize("T", [1, 33])
+def test_scales_beyond_f32_with_scores_of_zero(be, T):
+    """q and K of 1e30, orthogonal: every score is 0, the output V's mean."""
+    H, kv, hd, n = 8, 2, 64, 100
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 29)
+    q.zero_()
+    q[:, 0::hd] = 1e30
+    k[:, :, 0] = 0.0
+    k *= 1e30
+    out = run(be, q, k, v, H, n, T)
+    check(out, torch.zeros_like(q), torch.zeros_like(k), v, H, n, T, chain(T))
 
 
 @pytest.mark.parametrize("n,T", [(60, 1), (4000, 1), (4000, 33), (20000, 2)])
