@@ -238,7 +238,8 @@ int smallm_attention_noalloc(smallm_ctx* ctx, const float* q_dev, const float* k
  * are ignored).  mask_dev NULL is a chain: u <= t.  A token that sees nothing
  * gets zeros.  Rows that a token does not see do not affect it, whatever they
  * hold, NaN and infinities included; where a seen row or q holds them, or a
- * score passes f32's range, the output is not finite.
+ * score lies above f32's range or all of a token's scores below it, the output
+ * is not finite.
  *
  * Accuracy: an element of q, K or V enters to 2^-22 of itself or 2^-25 of the
  * largest magnitude of its row of head_dim, a weight's product with its row of

@@ -22,6 +22,7 @@
 // All launches are programmatic dependents: their set-up overlaps what ran
 // before (2 to 3 us of a call), and they wait for it before any access.
 #include <algorithm>
+#include <cfloat>
 
 #include "common.cuh"
 #include "engine.h"
@@ -190,6 +191,11 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     return r;
 }
 
+// 1 / sum of a row with maximum m; 0 where it sees nothing, NaN where its scores
+// leave no sum.
+__device__ __forceinline__ float row_inverse(float m, float sum) {
+    return sum > 0.f ? 1.f / sum : (m == -INFINITY && sum == 0.f ? 0.f : __int_as_float(0x7FC00000));
+}
 __device__ __forceinline__ float min3(float a, float b, float c) {
     float r;
     asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -596,11 +602,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             float ct = raw * p.c;
             // P is relative to the tile's own maximum mt: relative to the row's, a
             // tile of small weights would lose bits that large values bring back
-            const float mt = top == -INFINITY ? -INFINITY : ceilf(top * ct);
+            // (-inf only where nothing is seen: scores that are all below f32's range end
+            // with a sum of 0 at a finite maximum, one above it with a NaN)
+            const float mt = top == -INFINITY ? -INFINITY : fmaxf(ceilf(top * ct), -FLT_MAX);
             const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.f : mn;
             const float corr_t = ex2_approx(m - ref), part = ex2_approx(mt - ref);
             m = mn;
-            float off = kPShift - (mt == -INFINITY ? 0.f : mt);
+            float off = mt == INFINITY ? __uint_as_float(0x7FC00000u) : kPShift - (mt == -INFINITY ? 0.f : mt);
             float z = 0.f, wsum = 0.f;  // P's exponent besides mt's; sum of the weights where P holds more
             const float v_exp = sh.v_exp[ring];
             const bool wide_v = v_exp == INFINITY;
@@ -659,7 +667,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         if (p.n_split > 1) {
             if (half == 0 && valid) p.part_ml[(size_t)split * a.n_kv * p.R + row] = make_float2(m, l);
         } else {
-            f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+            f = row_inverse(m, l);
             if (SCORES && half == 0 && valid) p.stats[row] = make_float2(m == -INFINITY ? 0.f : m, f);
         }
         if (half == 0) sh.factor[rl] = f;
@@ -893,7 +901,7 @@ __device__ __forceinline__ void merge_row(const TreeParams& p, size_t row) {
         O.x += v.x, O.y += v.y, O.z += v.z, O.w += v.w;
         L += redl[k];
     }
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    const float inv = row_inverse(M, L);
     const uint32_t g = (uint32_t)(row / p.R), r = (uint32_t)(row % p.R);
     float* o = a.out + (size_t)(r / p.G) * a.out_stride + ((size_t)g * p.G + r % p.G) * HD;
     reinterpret_cast<float4*>(o)[c] = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
@@ -953,7 +961,7 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_weights_few_kernel(
         }
         const float top = warp_max(m), ref = top == -INFINITY ? 0.f : top;
         l = warp_sum(l * exp2f(m - ref));
-        if (lane == 0) stats[r] = make_float2(ref, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l));
+        if (lane == 0) stats[r] = make_float2(ref, row_inverse(top, l));
     }
     __syncthreads();
     if (key >= p.n) return;

@@ -133,6 +133,56 @@ def test_scales_beyond_f32_with_scores_of_zero(be, T):
     check(out, torch.zeros_like(q), torch.zeros_like(k), v, H, n, T, chain(T))
 
 
+@pytest.mark.parametrize("n,T", [(20, 2), (100, 2), (300, 30), (4000, 2), (4000, 30)])
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+def test_a_score_above_f32s_range_is_not_a_zero(be, n, T, where):
+    """One seen row scores beyond f32's largest value for token 0 alone: its
+    output is not finite.  (For the others that row's other elements lie more
+    than 2^-25 below its largest, so their scores of it are not known.)"""
+    H, kv, hd = 8, 2, 64
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 31)
+    at = {"first": 0, "middle": n // 2, "last": n - 1}[where]
+    q[:, 0::hd] = 0.0
+    k[:, :, 0] = 0.0
+    k[:, at, 0] = 1e20
+    q[0, 0::hd] = 1e20
+    w = torch.zeros(kv, n + T, device="cuda")
+    out = run(be, q, k, v, H, n, T, weights=w)
+    assert not bool(torch.isfinite(out[0]).any()) and bool(torch.isfinite(out[1:]).all())
+    assert not bool(torch.isfinite(w[:, :n + 1]).any())
+
+
+@pytest.mark.parametrize("n,T", [(20, 2), (300, 30), (4000, 2), (4000, 30)])
+def test_a_score_above_f32s_range_of_a_row_of_ones_own(be, n, T):
+    """The same of a drafted row that token 0 alone sees: the others are right."""
+    H, kv, hd = 8, 2, 64
+    seen = np.eye(T, dtype=bool)
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 31)
+    q[0, 0::hd] = 1e20
+    k[:, :, 0] = 0.0
+    k[:, n, 0] = 1e20
+    out = run(be, q, k, v, H, n, T, mask=words_of(seen))
+    assert not bool(torch.isfinite(out[0]).any())
+    q[0, 0::hd] = 0.0
+    k[:, n, 0] = 0.0
+    ref = run(be, q, k, v, H, n, T, mask=words_of(seen))
+    check(ref, q, k, v, H, n, T, seen)
+    out[0] = ref[0]
+    check(out, q, k, v, H, n, T, seen)
+
+
+@pytest.mark.parametrize("n", [3, 100, 4000])
+def test_all_scores_below_f32s_range_are_not_an_empty_row(be, n):
+    """Not finite, as the header says, rather than the zeros of a token that
+    sees nothing."""
+    H, kv, hd, T = 8, 2, 64, 1
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 37)
+    q[:, 0::hd] = 1e20
+    k[:, :, 0] = -1e20
+    out = run(be, q, k, v, H, n, T)
+    assert not bool(torch.isfinite(out).any())
+
+
 @pytest.mark.parametrize("n,T", [(60, 1), (4000, 1), (4000, 33), (20000, 2)])
 @pytest.mark.parametrize("f", [1e-34, 1e-30, 1e-26])
 def test_tiny_values_keep_their_bits(be, n, T, f):
