@@ -127,7 +127,7 @@ struct TcTree {
 
 struct TcShared {
     uint64_t k_full[kTcMaxSlots], k_empty[kTcMaxSlots], v_full[kTcMaxSlots], v_empty[kTcMaxSlots];
-    uint64_t v_scaled[kTcMaxSlots];
+    uint64_t v_scaled[kTcMaxSlots], z_full[4];
     uint64_t raw_full[2][kTcMaxSlots];  // [K, V]
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, done;
     float k_scale[kTcRing], v_exp[kTcRing];  // what a tile was divided by, V's as its exponent
@@ -428,6 +428,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             mbar_init(&sh.o_full[b], 2);
             mbar_init(&sh.o_empty[b], 2 * quads);
         }
+        for (uint32_t i = 0; i < 4; ++i) mbar_init(&sh.z_full[i], 2);
         mbar_init(&sh.q_full, 2 * quads);
         mbar_init(&sh.done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -531,6 +532,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         // the largest of the warp's rows (as bits: no sign, no NaN)
         const float qtop = __uint_as_float(__reduce_max_sync(0xffffffffu, valid ? __float_as_uint(qinv) : 0u));
         float m = -INFINITY, l = 0.f;
+        uint32_t wides = 0;  // tiles with scales of V's rows so far
         float* sc = nullptr;
         if constexpr (SCORES == 1) sc = p.scores + ((size_t)g * p.R + r) * p.sc_keys + half * SC;
         if constexpr (SCORES == 2) sc = p.scores + ((size_t)g * p.sc_keys + half * SC) * p.sc_rows + 4 * r;
@@ -614,7 +616,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             const bool wide_v = v_exp == INFINITY;
             if (wide_v) {
                 // P takes up the scales of V's rows, relative to the token's largest
-                // product among the keys that it sees (the halves meet as above)
+                // product among the keys that it sees, of both halves
                 const float4* vx = reinterpret_cast<const float4*>(&sh.row_scale[1][ring][half * SC]);
                 z = -INFINITY;
                 put_scores();
@@ -625,8 +627,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                     return y + f4_at(vx[i / 4], i);
                 });
                 get_scores();
+                // (a bounded wait: after one that gave up the two warps may disagree here)
                 sh.part_z[half][rl] = z;
-                asm volatile("barrier.cta.sync %0, 64;" ::"r"(4 + quad) : "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.z_full[quad]);
+                ok = __all_sync(0xffffffffu, ok && mbar_wait_soon(&sh.z_full[quad], wides++ & 1));
                 z = fmaxf(z, sh.part_z[half ^ 1][rl]);
                 z = z == -INFINITY ? 0.f : ceilf(z) - kPShift;
                 ct = 1.f, off = -z;
