@@ -23,6 +23,7 @@
 // before (2 to 3 us of a call), and they wait for it before any access.
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "common.cuh"
 #include "engine.h"
@@ -106,6 +107,7 @@ constexpr uint32_t kTcThreads = 32 * 28;
 constexpr uint32_t kConvThreads = 128, kConvWarps = kConvThreads / 32;
 constexpr float kPShift = 14.f;
 constexpr float kTinyShift = 100.f;
+constexpr float kLargeScore = 0x1p22f;  // exponents from here on have less than two fractional bits
 constexpr float kWideTile = 0x1p-14f;  // a tile's rows get scales of their own where one is this much smaller
 
 template <int HD>
@@ -195,6 +197,15 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
 // leave no sum.
 __device__ __forceinline__ float row_inverse(float m, float sum) {
     return sum > 0.f ? 1.f / sum : (m == -INFINITY && sum == 0.f ? 0.f : __int_as_float(0x7FC00000));
+}
+// A row's totals are plain where its maximum is no large score.
+__device__ __forceinline__ bool row_plain(float2 stats) { return fabsf(stats.x) < kLargeScore; }
+// The weight 2^(s c - mc) / sum of a stored score; in other rows the product is
+// rounded as the kernel's.
+template <bool PLAIN>
+__device__ __forceinline__ float add_weight(float acc, float s, float c, float2 stats) {
+    const float y = PLAIN ? fmaf(s, c, -stats.x) : __fadd_rn(__fmul_rn(s, c), -stats.x);
+    return fmaf(exp2f(y), stats.y, acc);
 }
 __device__ __forceinline__ float min3(float a, float b, float c) {
     float r;
@@ -532,7 +543,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         // the largest of the warp's rows (as bits: no sign, no NaN)
         const float qtop = __uint_as_float(__reduce_max_sync(0xffffffffu, valid ? __float_as_uint(qinv) : 0u));
         float m = -INFINITY, l = 0.f;
-        uint32_t wides = 0;  // tiles with scales of V's rows so far
+        uint32_t meets = 0;  // tiles so far in which the halves met once more
         float* sc = nullptr;
         if constexpr (SCORES == 1) sc = p.scores + ((size_t)g * p.R + r) * p.sc_keys + half * SC;
         if constexpr (SCORES == 2) sc = p.scores + ((size_t)g * p.sc_keys + half * SC) * p.sc_rows + 4 * r;
@@ -560,7 +571,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             get_scores();
             // (never 0: an unseen key's -inf times it stays -inf)
             // keys with scales of their own, or a factor beyond f32's range (which no score need be)
-            const bool far = !(qtop * k_scale < INFINITY);
+            const float factor = qtop * k_scale, v_exp = sh.v_exp[ring];
+            const bool wide_v = v_exp == INFINITY;
+            const bool far = !(factor < INFINITY);
             const float raw = far ? 1.f : fmaxf(qinv * k_scale, 0x1p-120f);
             if (key0 + kTcKeys > a.n_past || bad || far) {
                 if (far) {
@@ -610,30 +623,37 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.f : mn;
             const float corr_t = ex2_approx(m - ref), part = ex2_approx(mt - ref);
             m = mn;
-            float off = mt == INFINITY ? __uint_as_float(0x7FC00000u) : kPShift - (mt == -INFINITY ? 0.f : mt);
+            const float tref = mt == INFINITY ? __uint_as_float(0x7FC00000u) : (mt == -INFINITY ? 0.f : mt);
+            float off = kPShift - tref;
             float z = 0.f, wsum = 0.f;  // P's exponent besides mt's; sum of the weights where P holds more
-            const float v_exp = sh.v_exp[ring];
-            const bool wide_v = v_exp == INFINITY;
-            if (wide_v) {
-                // P takes up the scales of V's rows, relative to the token's largest
-                // product among the keys that it sees, of both halves
-                const float4* vx = reinterpret_cast<const float4*>(&sh.row_scale[1][ring][half * SC]);
-                z = -INFINITY;
+            if (wide_v || !(factor < 0x1p-13f)) {  // (below it hd products below 2^30 give no large score)
+                const bool large = fabsf(tref) >= kLargeScore;
+                // exponents of their own first, by way of tensor memory.  A product of a large
+                // score is rounded before the maximum's is taken from it: by an fma the
+                // maximum itself could end up anywhere between 2^-128 and 2^128.
+                if (wide_v) z = -INFINITY;
+                const float* vx = &sh.row_scale[1][ring][half * SC];
                 put_scores();
                 tmem_map8<SC / 8>(sp + half * SC, [&](int i, float x) {
-                    const float y = fmaf(x, ct, off);
+                    float y = large ? __fadd_rn(__fadd_rn(__fmul_rn(x, ct), -tref), kPShift) : fmaf(x, ct, off);
                     wsum += ex2_approx(y);
-                    z = fmaxf(z, y + f4_at(vx[i / 4], i));
-                    return y + f4_at(vx[i / 4], i);
+                    if (wide_v) {
+                        y += vx[i];
+                        z = fmaxf(z, y);
+                    }
+                    return y;
                 });
                 get_scores();
-                // (a bounded wait: after one that gave up the two warps may disagree here)
+                // The halves meet: P goes where the other half's scores were, and takes up the
+                // scales of V's rows relative to the token's largest product among the keys
+                // that it sees.  (A bounded wait: after one that gave up the two warps may
+                // disagree about this path.)
                 sh.part_z[half][rl] = z;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.z_full[quad]);
-                ok = __all_sync(0xffffffffu, ok && mbar_wait_soon(&sh.z_full[quad], wides++ & 1));
+                ok = __all_sync(0xffffffffu, ok && mbar_wait_soon(&sh.z_full[quad], meets++ & 1));
                 z = fmaxf(z, sh.part_z[half ^ 1][rl]);
-                z = z == -INFINITY ? 0.f : ceilf(z) - kPShift;
+                if (wide_v) z = z == -INFINITY ? 0.f : ceilf(z) - kPShift;
                 ct = 1.f, off = -z;
             }
             float2 sum = make_float2(0.f, 0.f);
@@ -973,7 +993,8 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_weights_few_kernel(
     float acc = 0.f;
 #pragma unroll
     for (uint32_t r = 0; r < ROWS; ++r)
-        if (r < p.R) acc = fmaf(exp2f(fmaf(v[r], p.c, -stats[r].x)), stats[r].y, acc);
+        if (r < p.R)
+            acc = row_plain(stats[r]) ? add_weight<true>(acc, v[r], p.c, stats[r]) : add_weight<false>(acc, v[r], p.c, stats[r]);
     *w = old + acc;
 }
 __global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(const TreeParams p) {
@@ -1002,14 +1023,19 @@ __global__ void __launch_bounds__(32 * kWeightWarps) smallm_tree_weights_kernel(
 #pragma unroll
         for (int j = 0; j < kWeightRows; ++j) {
             if (r + 32 * j >= p.R) break;
+            auto add = [&](auto plain) {
 #pragma unroll
-            for (int k = 0; k < kWeightKeys / 4; ++k) {
-                const float4 x = v[j][k];
-                acc[4 * k] = fmaf(exp2f(fmaf(x.x, p.c, -st[j].x)), st[j].y, acc[4 * k]);
-                acc[4 * k + 1] = fmaf(exp2f(fmaf(x.y, p.c, -st[j].x)), st[j].y, acc[4 * k + 1]);
-                acc[4 * k + 2] = fmaf(exp2f(fmaf(x.z, p.c, -st[j].x)), st[j].y, acc[4 * k + 2]);
-                acc[4 * k + 3] = fmaf(exp2f(fmaf(x.w, p.c, -st[j].x)), st[j].y, acc[4 * k + 3]);
-            }
+                for (int k = 0; k < kWeightKeys / 4; ++k) {
+                    const float4 x = v[j][k];
+                    constexpr bool P = decltype(plain)::value;
+                    acc[4 * k] = add_weight<P>(acc[4 * k], x.x, p.c, st[j]);
+                    acc[4 * k + 1] = add_weight<P>(acc[4 * k + 1], x.y, p.c, st[j]);
+                    acc[4 * k + 2] = add_weight<P>(acc[4 * k + 2], x.z, p.c, st[j]);
+                    acc[4 * k + 3] = add_weight<P>(acc[4 * k + 3], x.w, p.c, st[j]);
+                }
+            };
+            if (row_plain(st[j])) add(std::true_type{});
+            else add(std::false_type{});
         }
     }
     float mine = 0.f;  // lane k: key k

@@ -183,6 +183,33 @@ def test_all_scores_below_f32s_range_are_not_an_empty_row(be, n):
     assert not bool(torch.isfinite(out).any())
 
 
+@pytest.mark.parametrize("e", range(10, 16))
+@pytest.mark.parametrize("n,T", [(60, 1), (700, 1), (700, 33)])
+@pytest.mark.parametrize("winners", [1, 2])
+def test_large_scores(be, e, n, T, winners):
+    """Scores up to 2^27 whose gaps (2^13 at least) are far above their error
+    (2^-22 of them, 2^5): the largest takes everything, two equal ones half
+    each, and the output is one row or the mean of two: V's and the weights'
+    2^-22 each, and 8 u for two sums, the reciprocal and the products."""
+    H, kv, hd = 4, 2, 64
+    for shift in range(3):
+        q, k, v = inputs(H, kv, hd, n, T, n + T, 41 + shift)
+        q.zero_()
+        q[:, 0::hd] = 2.0 ** e + shift
+        k.zero_()
+        k[:, :, 0] = 2.0 ** e - 64 - (torch.arange(n + T, device="cuda") % 53)
+        best = [5, n - 3][:winners]
+        k[:, best, 0] = 2.0 ** e + 3 * shift
+        w = torch.zeros(kv, n + T, device="cuda")
+        out = run(be, q, k, v, H, n, T, weights=w)
+        want = v[:, best].double().mean(1).repeat_interleave(H // kv, 0).reshape(1, H * hd)
+        tol = (4 * U + 4 * U + 8 * U) * v[:, best].abs().amax().double()
+        assert bool(((out.double() - want).abs() <= tol).all()), float((out.double() - want).abs().max())
+        total = torch.zeros_like(w)
+        total[:, best] = T * (H // kv) / winners
+        assert bool(((w - total).abs() <= 4 * T * H * U * total).all())
+
+
 @pytest.mark.parametrize("n,T", [(60, 1), (4000, 1), (4000, 33), (20000, 2)])
 @pytest.mark.parametrize("f", [1e-34, 1e-30, 1e-26])
 def test_tiny_values_keep_their_bits(be, n, T, f):
