@@ -255,7 +255,8 @@ int smallm_attention_noalloc(smallm_ctx* ctx, const float* q_dev, const float* k
  * weights_dev, unless NULL, is [n_kv_heads][max_ctx]: row k of KV head g gains
  * the weight that it got in this call, summed over the tokens and the query
  * heads of g (smallm_cache_select reads these totals); rows at
- * n_past + n_tokens and above are left as they are.
+ * n_past + n_tokens and above are left as they are.  A token without finite
+ * weights leaves NaN in the totals of the rows that it sees, and of no others.
  *
  * work_dev: at least smallm_attention_tree_workspace bytes, 16-byte aligned,
  * contents irrelevant before and after.  Calls that may overlap in time need

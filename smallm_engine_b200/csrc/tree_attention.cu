@@ -198,14 +198,16 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
 __device__ __forceinline__ float row_inverse(float m, float sum) {
     return sum > 0.f ? 1.f / sum : (m == -INFINITY && sum == 0.f ? 0.f : __int_as_float(0x7FC00000));
 }
-// A row's totals are plain where its maximum is no large score.
-__device__ __forceinline__ bool row_plain(float2 stats) { return fabsf(stats.x) < kLargeScore; }
+// A row's weights are plain where its maximum is no large score and it has a sum.
+__device__ __forceinline__ bool row_plain(float2 stats) {
+    return fabsf(stats.x) < kLargeScore && fabsf(stats.y) < INFINITY;
+}
 // The weight 2^(s c - mc) / sum of a stored score; in other rows the product is
-// rounded as the kernel's.
+// rounded as the kernel's, and an unseen key has none even where the sum is NaN.
 template <bool PLAIN>
 __device__ __forceinline__ float add_weight(float acc, float s, float c, float2 stats) {
     const float y = PLAIN ? fmaf(s, c, -stats.x) : __fadd_rn(__fmul_rn(s, c), -stats.x);
-    return fmaf(exp2f(y), stats.y, acc);
+    return !PLAIN && s == -INFINITY ? acc : fmaf(exp2f(y), stats.y, acc);
 }
 __device__ __forceinline__ float min3(float a, float b, float c) {
     float r;

@@ -226,3 +226,44 @@ def test_tiny_values_keep_their_bits(be, n, T, f):
         # (every partial sum is rounded to f32's smallest step at most n times)
         tol = (2 * (n + T) + 64) * U * mean + (n + T) * 2.0 ** -149
         assert bool(((out[t] - mean[:, None]).abs() <= tol[:, None]).all()), float(((out[t] - mean[:, None]).abs() / tol[:, None]).max())
+
+
+@pytest.mark.parametrize("T", [3, 6, 70])
+@pytest.mark.parametrize("n", [40, 3000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_totals_of_rows_that_a_spoiled_token_does_not_see(be, T, n, bad):
+    """Token 1's q is not finite: the rows that it sees have no total any more,
+    the others get the other tokens' weight."""
+    H, kv, hd = 4, 2, 64
+    seen = chain(T)
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 53)
+    w0, w = (torch.zeros(kv, n + T, device="cuda") for _ in range(2))
+    ref = run(be, q, k, v, H, n, T, mask=words_of(seen), weights=w0)
+    check(ref, q, k, v, H, n, T, seen, w0, torch.zeros_like(w0))
+    q[1] = bad
+    out = run(be, q, k, v, H, n, T, mask=words_of(seen), weights=w)
+    assert not bool(torch.isfinite(out[1]).any()) and not bool(torch.isfinite(w[:, :n + 2]).any())
+    assert torch.equal(w[:, n + 2:], w0[:, n + 2:])
+    keep = [t for t in range(T) if t != 1]
+    assert torch.equal(out[keep], ref[keep])
+
+
+@pytest.mark.parametrize("T", [4, 70])
+def test_totals_of_a_spoiled_key(be, T):
+    """Drafted key 2 is NaN and token 3 alone sees it: rows that token 3 sees
+    have no total, the others' are as without it.  (Both runs are within the
+    derived tolerance of the definition: 2 * 72 u D, D below 30 for 64 products
+    of q and k, and (40 + 70 + 140 + 64) u; twice that is below 6e-4.)"""
+    H, kv, hd, n = 4, 2, 64, 40
+    seen = np.eye(T, dtype=bool)
+    seen[3, 2] = True
+    seen[2, 2] = False
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 59)
+    w0, w = (torch.zeros(kv, n + T, device="cuda") for _ in range(2))
+    run(be, q, k, v, H, n, T, mask=words_of(seen), weights=w0)
+    k[:, n + 2] = float("nan")
+    run(be, q, k, v, H, n, T, mask=words_of(seen), weights=w)
+    lost = [*range(n), n + 2, n + 3]
+    rest = [r for r in range(n + T) if r not in lost]
+    assert not bool(torch.isfinite(w[:, lost]).any())
+    assert bool(((w - w0)[:, rest].abs() <= 6e-4 * w0[:, rest]).all())
