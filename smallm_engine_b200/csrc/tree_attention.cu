@@ -23,6 +23,7 @@
 // before (2 to 3 us of a call), and they wait for it before any access.
 #include <algorithm>
 #include <cfloat>
+#include <cmath>
 #include <type_traits>
 
 #include "common.cuh"
@@ -40,7 +41,9 @@ struct TreeParams {
     uint32_t sc_rows;    // stored scores of a key: R, padded; 0: they run along keys
     uint32_t sc_keys;    // ... and of a row: n, padded to tiles
     float c;             // log2(e) / sqrt(hd)
-    float* part_o;       // [n_split][n_kv * R][hd]
+    float o_below;       // outputs are summed as 2^-head of them, so that n values fit: kPShift + head
+    float head_up;       // 2^head
+    float* part_o;       // [n_split][n_kv * R][hd], 2^-head of the sums
     float2* part_ml;     // [n_split][n_kv * R] (mc, sum)
     float* scores;       // [n_kv][sc_keys / 4][sc_rows][4] or [n_kv][R][sc_keys], raw q . K, -inf where unseen
     float2* stats;       // [n_kv * R] (mc of the whole row, 1 / sum or 0)
@@ -132,7 +135,7 @@ struct TcShared {
     uint64_t v_scaled[kTcMaxSlots], z_full[4];
     uint64_t raw_full[2][kTcMaxSlots];  // [K, V]
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], q_full, done;
-    float k_scale[kTcRing], v_exp[kTcRing];  // what a tile was divided by, V's as its exponent
+    float k_scale[kTcRing], v_exp[kTcRing];  // what a tile was divided by; V's as O's exponent
     unsigned long long k_bad[kTcRing], v_bad[kTcRing];
     uint2 wrange[2][2][kConvWarps];  // [K, V][tile % 2][warp] bits of the largest and smallest magnitude
     uint32_t tmem;
@@ -279,9 +282,10 @@ __device__ __forceinline__ bool tc_copy(const float* src, uint32_t n, uint32_t t
     return true;
 }
 
-// One converter group: tiles t0 .. t0 + nt - 1, in place.
+// One converter group: tiles t0 .. t0 + nt - 1, in place.  V's exponents are
+// left as O's.
 template <int HD, int GROUP>
-__device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt, int tid, uint8_t* smem, TcShared& sh) {
+__device__ __forceinline__ bool tc_convert(const TreeParams& p, uint32_t t0, uint32_t nt, int tid, uint8_t* smem, TcShared& sh) {
     using C = TcTree<HD>;
     constexpr int N = (int)kTcKeys * HD / 4 / kConvThreads;  // float4s of a thread
     constexpr uint32_t W = HD / 4, STEP = kConvThreads / W;  // float4s of a row; rows between two units
@@ -298,7 +302,7 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
     const int lane = tid & 31, cw = tid >> 5;
     for (uint32_t t = 0; t < nt; ++t) {
         const uint32_t slot = t % C::slots, ring = t % kTcRing;
-        const uint32_t left = n - (t0 + t) * kTcKeys;  // rows from the tile's first to the last
+        const uint32_t left = p.n - (t0 + t) * kTcKeys;  // rows from the tile's first to the last
         const bool stuck = !mbar_wait_soon(&sh.raw_full[GROUP][slot], (t / C::slots) & 1);
         const float4* src = reinterpret_cast<const float4*>(slots + slot * C::slot) + tid;
         // the largest magnitude, and the smallest of three elements' largest ones: no
@@ -384,7 +388,7 @@ __device__ __forceinline__ bool tc_convert(uint32_t n, uint32_t t0, uint32_t nt,
         }
         float mult, inv;
         tc_scale(mx, mult, inv);
-        if (tid == 0) (GROUP ? sh.v_exp : sh.k_scale)[ring] = wide ? INFINITY : (GROUP ? (float)scale_exp(inv) : inv);
+        if (tid == 0) (GROUP ? sh.v_exp : sh.k_scale)[ring] = wide ? INFINITY : (GROUP ? (float)scale_exp(inv) - p.o_below : inv);
         if (wide) mult = 1.f;
         if (GROUP) {  // P needs V's scales, and sooner than the products need V
             __syncwarp();
@@ -627,13 +631,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             m = mn;
             const float tref = mt == INFINITY ? __uint_as_float(0x7FC00000u) : (mt == -INFINITY ? 0.f : mt);
             float off = kPShift - tref;
-            float z = 0.f, wsum = 0.f;  // P's exponent besides mt's; sum of the weights where P holds more
+            float o_exp = v_exp, wsum = 0.f;  // O's exponent besides mt's; sum of the weights where P holds more
             if (wide_v || !(factor < 0x1p-13f)) {  // (below it hd products below 2^30 give no large score)
                 const bool large = fabsf(tref) >= kLargeScore;
                 // exponents of their own first, by way of tensor memory.  A product of a large
                 // score is rounded before the maximum's is taken from it: by an fma the
                 // maximum itself could end up anywhere between 2^-128 and 2^128.
-                if (wide_v) z = -INFINITY;
+                float z = wide_v ? -INFINITY : 0.f;  // P's exponent besides mt's
                 const float* vx = &sh.row_scale[1][ring][half * SC];
                 put_scores();
                 tmem_map8<SC / 8>(sp + half * SC, [&](int i, float x) {
@@ -655,7 +659,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                 if (lane == 0) mbar_arrive(&sh.z_full[quad]);
                 ok = __all_sync(0xffffffffu, ok && mbar_wait_soon(&sh.z_full[quad], meets++ & 1));
                 z = fmaxf(z, sh.part_z[half ^ 1][rl]);
-                if (wide_v) z = z == -INFINITY ? 0.f : ceilf(z) - kPShift;
+                if (wide_v) {
+                    z = z == -INFINITY ? 0.f : ceilf(z) - kPShift;
+                    o_exp = z - p.o_below;
+                }
                 ct = 1.f, off = -z;
             }
             float2 sum = make_float2(0.f, 0.f);
@@ -676,7 +683,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             }
             if (!wide_v) wsum = sum.x + sum.y;
             if (half == 0) {
-                const float e = mt - ref + z + (wide_v ? 0.f : v_exp) - kPShift;  // O's exponent
+                const float e = mt - ref + o_exp;  // O's exponent
                 const bool tiny = e < -126.f && e > -126.f - kTinyShift;
                 sh.corr[t % 4][rl] = make_float2(corr_t, tiny ? -exp2_whole(e + kTinyShift) : exp2_whole(e));
             }
@@ -690,14 +697,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         asm volatile("barrier.cta.sync %0, 64;" ::"r"(4 + quad) : "memory");
         l = (l + sh.part_sum[half ^ 1][rl]) * 0x1p-14f;
         const size_t row = (size_t)g * p.R + r;
-        float f = 1.f;
+        float f = 0.f;
         if (p.n_split > 1) {
             if (half == 0 && valid) p.part_ml[(size_t)split * a.n_kv * p.R + row] = make_float2(m, l);
         } else {
             f = row_inverse(m, l);
             if (SCORES && half == 0 && valid) p.stats[row] = make_float2(m == -INFINITY ? 0.f : m, f);
         }
-        if (half == 0) sh.factor[rl] = f;
+        if (half == 0) sh.factor[rl] = p.n_split > 1 ? 1.f : f * p.head_up;
         asm volatile("barrier.cta.sync %0, 128;" ::"r"(8 + quad) : "memory");
         }
     } else if (warp < 16) {
@@ -783,10 +790,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
         }
     } else if (warp < 20) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
-        ok = tc_convert<HD, 0>(p.n, t0, nt, (int)threadIdx.x - 512, smem, sh);
+        ok = tc_convert<HD, 0>(p, t0, nt, (int)threadIdx.x - 512, smem, sh);
     } else if (warp < 24) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
-        ok = tc_convert<HD, 1>(p.n, t0, nt, (int)threadIdx.x - 640, smem, sh);
+        ok = tc_convert<HD, 1>(p, t0, nt, (int)threadIdx.x - 640, smem, sh);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
         if (warp == 24) {
@@ -929,9 +936,10 @@ __device__ __forceinline__ void merge_row(const TreeParams& p, size_t row) {
         L += redl[k];
     }
     const float inv = row_inverse(M, L);
+    const float up = inv * p.head_up;
     const uint32_t g = (uint32_t)(row / p.R), r = (uint32_t)(row % p.R);
     float* o = a.out + (size_t)(r / p.G) * a.out_stride + ((size_t)g * p.G + r % p.G) * HD;
-    reinterpret_cast<float4*>(o)[c] = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+    reinterpret_cast<float4*>(o)[c] = make_float4(O.x * up, O.y * up, O.z * up, O.w * up);
     if (c == 0 && p.sc_rows && p.scores) p.stats[row] = make_float2(ref, inv);
 }
 
@@ -1161,6 +1169,10 @@ void launch_attention_tree(const TreeArgs& a, void* work, size_t work_bytes, cud
     p.sc_rows = t.sc_rows;
     p.sc_keys = t.sc_keys;
     p.c = (float)(1.4426950408889634 / sqrt((double)a.hd));
+    uint32_t head = 1;  // the weights' sum is below n, and rounded up once more by what P and V round
+    while (p.n >> (head - 1)) ++head;
+    p.o_below = kPShift + (float)head;
+    p.head_up = ldexpf(1.f, (int)head);
     p.err = device_error_flag();
     uint8_t* w = static_cast<uint8_t*>(work);
     p.part_o = reinterpret_cast<float*>(w);

@@ -133,6 +133,8 @@ def test_scales_beyond_f32_with_scores_of_zero(be, T):
     check(out, torch.zeros_like(q), torch.zeros_like(k), v, H, n, T, chain(T))
 
 
+# ------------------------------------------------------------ large scores --
+
 @pytest.mark.parametrize("n,T", [(20, 2), (100, 2), (300, 30), (4000, 2), (4000, 30)])
 @pytest.mark.parametrize("where", ["first", "middle", "last"])
 def test_a_score_above_f32s_range_is_not_a_zero(be, n, T, where):
@@ -210,6 +212,21 @@ def test_large_scores(be, e, n, T, winners):
         assert bool(((w - total).abs() <= 4 * T * H * U * total).all())
 
 
+# ------------------------------------------------------------ large values --
+
+@pytest.mark.parametrize("n,T", [(60, 1), (4000, 1), (4000, 33), (20000, 2)])
+@pytest.mark.parametrize("f", [1e36, 3.3e38])
+def test_mean_of_values_whose_sum_passes_f32(be, n, T, f):
+    """Equal scores: a mean of V near f32's largest value is finite."""
+    H, kv, hd = 8, 2, 64
+    q, k, v = inputs(H, kv, hd, n, T, n + T, 43)
+    k.zero_()
+    v = f * (0.5 + 0.5 * unit_rows(v.shape, 6).abs())
+    out = run(be, q, k, v, H, n, T)
+    assert bool(torch.isfinite(out).all())
+    check(out, q, k, v, H, n, T, chain(T))
+
+
 @pytest.mark.parametrize("n,T", [(60, 1), (4000, 1), (4000, 33), (20000, 2)])
 @pytest.mark.parametrize("f", [1e-34, 1e-30, 1e-26])
 def test_tiny_values_keep_their_bits(be, n, T, f):
@@ -227,6 +244,8 @@ def test_tiny_values_keep_their_bits(be, n, T, f):
         tol = (2 * (n + T) + 64) * U * mean + (n + T) * 2.0 ** -149
         assert bool(((out[t] - mean[:, None]).abs() <= tol[:, None]).all()), float(((out[t] - mean[:, None]).abs() / tol[:, None]).max())
 
+
+# ------------------------------------------------------------------ totals --
 
 @pytest.mark.parametrize("T", [3, 6, 70])
 @pytest.mark.parametrize("n", [40, 3000])
