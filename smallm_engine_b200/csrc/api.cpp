@@ -355,7 +355,7 @@ int smallm_ctx_device_errors(smallm_ctx* ctx, uint32_t* flags, int clear) {
         need(ctx && flags, "NULL argument");
         set_dev(ctx->device);
         SM_CUDA(cudaDeviceSynchronize());
-        *flags = smallm::gemv_error_flags(clear != 0);
+        *flags = smallm::gemv_error_flags(clear ? ~0u : 0u);
     });
 }
 

@@ -127,8 +127,9 @@ struct GemvPlan {
 };
 GemvPlan gemv_plan(const QMat& m, size_t smem_cap = 0);
 
-// Error bits raised by GEMV kernels whose bounded waits gave up (0 = none).
-unsigned int gemv_error_flags(bool clear);
+// Error bits raised by kernels whose bounded waits gave up (0 = none); those of
+// them in `clear` are reset, the others stay for whoever reads them.
+unsigned int gemv_error_flags(unsigned int clear);
 
 // Dequantize a QMat to f32 [rows][cols] (bit-identical to the reference).
 void launch_qmat_dequant(const QMat& m, float* y, cudaStream_t stream);

@@ -510,6 +510,8 @@ void rope_table(uint32_t hd, uint32_t positions, float base, std::vector<float2>
 
 __device__ unsigned int g_gemv_err;  // set by a bounded wait that gave up
 
+__global__ void smallm_keep_bits_kernel(unsigned int* word, unsigned int keep) { atomicAnd(word, keep); }
+
 template <class Fmt, int W>
 static const void* pick(int pro, int epi) {
     if (pro == PRO_PLAIN && epi == EPI_STORE) return (const void*)smallm_qgemv_kernel<Fmt, PRO_PLAIN, EPI_STORE, W>;
@@ -685,12 +687,15 @@ void launch_gemv(const QMat& m, int pro, int epi, const GemvArgs& a, cudaStream_
     launch_kernel_ex(fn, dim3(grid), dim3((pl.warps + 1) * 32), pl.smem, stream, pdl, args);
 }
 
-unsigned int gemv_error_flags(bool clear) {
+unsigned int gemv_error_flags(unsigned int clear) {
     unsigned int v = 0;
     SM_CUDA(cudaMemcpyFromSymbol(&v, g_gemv_err, sizeof(v)));
-    if (clear && v) {
-        unsigned int z = 0;
-        SM_CUDA(cudaMemcpyToSymbol(g_gemv_err, &z, sizeof(z)));
+    if (v & clear) {  // atomically: another stream's kernel may raise a bit meanwhile
+        unsigned int* word = device_error_flag();
+        unsigned int keep = ~(v & clear);
+        void* args[] = {&word, &keep};
+        SM_CUDA(cudaLaunchKernel((const void*)smallm_keep_bits_kernel, dim3(1), dim3(1), args, 0, nullptr));
+        SM_CUDA(cudaStreamSynchronize(nullptr));
     }
     return v;
 }

@@ -631,7 +631,7 @@ void Model::check_step_errors() {
     const unsigned int e = *h_err & ~kErrOperators;
     if (!e) return;
     *h_err = 0;
-    gemv_error_flags(true);
+    gemv_error_flags(~kErrOperators);
     reset_step_state();
     throw Error(SMALLM_ERR_CUDA, "a bounded device wait gave up during the step (flags " + std::to_string(e) +
                                      "); its results are invalid");
@@ -817,7 +817,7 @@ void Model::logprobs(uint32_t token, float* logprob, float* entropy, uint32_t n_
     SM_CUDA(cudaMemcpyAsync(h_err, device_error_flag(), 4, cudaMemcpyDeviceToHost, stream));
     SM_CUDA(cudaStreamSynchronize(stream));
     if (*h_err & kErrLogprobs) {
-        gemv_error_flags(true);
+        gemv_error_flags(kErrLogprobs);
         throw Error(SMALLM_ERR_CUDA, "logprobs: a bounded device wait gave up; the results are invalid");
     }
     if (logprob) std::memcpy(logprob, host + 1, 4);
