@@ -285,6 +285,7 @@ struct LogprobArgs {
     uint32_t n_top;
     uint32_t* top_ids;       // [n_rows][n_top]
     float* top_logprobs;
+    unsigned int* err;       // raised by a wait that gave up; null: the device error word
 };
 constexpr uint32_t kLogprobMaxTop = 64;
 void launch_logprobs(const LogprobArgs& a, cudaStream_t stream);

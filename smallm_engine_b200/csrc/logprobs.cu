@@ -409,7 +409,7 @@ void launch_logprobs(const LogprobArgs& a, cudaStream_t stream) {
     cfg.numAttrs = 2;
     LogprobArgs aa = a;
     uint32_t per_cta = (nq + C - 1) / C;
-    unsigned int* err = device_error_flag();
+    unsigned int* err = a.err ? a.err : device_error_flag();
     void* args[] = {&aa, &per_cta, &err};
     SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
 }

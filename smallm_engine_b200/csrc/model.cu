@@ -802,8 +802,10 @@ void Model::logprobs(uint32_t token, float* logprob, float* entropy, uint32_t n_
     a.n_rows = 1;
     a.vocab = a.stride = vocab;
     float* out = reinterpret_cast<float*>(lp_scratch);
+    uint32_t host[kHead + 2 * kLogprobMaxTop] = {token};  // token, its log probability, entropy, this call's errors
+    SM_CUDA(cudaMemcpyAsync(lp_scratch, host, 4 * kHead, cudaMemcpyHostToDevice, stream));
+    a.err = lp_scratch + 3;
     if (logprob) {
-        SM_CUDA(cudaMemcpyAsync(lp_scratch, &token, 4, cudaMemcpyHostToDevice, stream));
         a.tokens = lp_scratch;
         a.logprob = out + 1;
     }
@@ -812,14 +814,9 @@ void Model::logprobs(uint32_t token, float* logprob, float* entropy, uint32_t n_
     a.top_ids = lp_scratch + kHead;
     a.top_logprobs = out + kHead + n_top;
     launch_logprobs(a, stream);
-    uint32_t host[kHead + 2 * kLogprobMaxTop];
     SM_CUDA(cudaMemcpyAsync(host, lp_scratch, 4 * (kHead + 2 * n_top), cudaMemcpyDeviceToHost, stream));
-    SM_CUDA(cudaMemcpyAsync(h_err, device_error_flag(), 4, cudaMemcpyDeviceToHost, stream));
     SM_CUDA(cudaStreamSynchronize(stream));
-    if (*h_err & kErrLogprobs) {
-        gemv_error_flags(kErrLogprobs);
-        throw Error(SMALLM_ERR_CUDA, "logprobs: a bounded device wait gave up; the results are invalid");
-    }
+    if (host[3]) throw Error(SMALLM_ERR_CUDA, "logprobs: a bounded device wait gave up; the results are invalid");
     if (logprob) std::memcpy(logprob, host + 1, 4);
     if (entropy) std::memcpy(entropy, host + 2, 4);
     if (n_top) {

@@ -89,7 +89,7 @@ struct Model {
     // Log probabilities from the last step's logits (logprobs.cu), to the host.
     void logprobs(uint32_t token, float* logprob, float* entropy, uint32_t n_top, uint32_t* top_ids,
                   float* top_logprobs);
-    uint32_t* lp_scratch = nullptr;    // token, its log probability, entropy, then ids and log probabilities
+    uint32_t* lp_scratch = nullptr;    // token, its log probability, entropy, errors, then ids and log probabilities
     uint32_t* samp_scratch = nullptr;  // 4 * vocab + 4 u32
     // Batched prefill: f16 copies of the layer matrices in storage row order
     // (made at the first prefill from the bit-exact dequantized values), GEMMs

@@ -31,6 +31,19 @@ def raise_bit_3(be):
     torch.cuda.synchronize()
 
 
+def test_logprobs_of_a_model_answers_for_itself(be, gguf_dir):
+    """What the word holds from others neither fails the call nor is cleared."""
+    m = CudaModel(synth.write_gguf(synth.tiny_spec("llama-q4_0"), 8, gguf_dir / "errors-lp.gguf"))
+    m.forward(5, 0)
+    want = m.logprobs(7, 4)
+    assert be.device_errors() == 0
+    raise_bit_7(be)
+    raise_bit_3(be)
+    assert m.logprobs(7, 4) == want and m.logprobs().entropy == want.entropy
+    assert be.device_errors() == 128 + 8 and be.device_errors() == 0
+    m.close()
+
+
 def test_a_steps_error_leaves_the_operators_bits(be, gguf_dir):
     """A step that finds a step's bit answers for that one: the bad list's stays
     for the caller of smallm_cache_move."""
