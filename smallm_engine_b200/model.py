@@ -42,8 +42,10 @@ class ModelConfig:
 
 @dataclass
 class TokenLogprobs:
-    """A token's log probability in the distribution it was taken from, that
-    distribution's entropy and its most likely tokens (id, log probability)."""
+    """A token's log probability under softmax(logits), that distribution's
+    entropy and its most likely tokens (id, log probability).  It is the model's
+    distribution: a sampler's temperature, top-k or top-p come after it and do
+    not enter."""
     token: int | None
     logprob: float | None
     entropy: float
