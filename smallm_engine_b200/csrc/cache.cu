@@ -10,9 +10,10 @@
 // summed over the cluster's shared memory, then the bin that holds the rank.
 // (Digits of 11, 11 and 10 bits save a barrier, but then every CTA reads 8 KB
 // from each of 15 others for each digit: 37 us for 8 x 131072 keys where this
-// takes 20 us.  Histograms read by more threads, fewer reads each: 21 us.)  Every larger key is kept, and of the equal ones the first few
-// in row order; rows come out ascending.  Bound by latency: one read of the
-// totals, five cluster barriers and as many rounds of remote reads.
+// takes 20 us.  Histograms read by more threads, fewer reads each: 21 us.)
+// Every larger key is kept, and of the equal ones the first few in row order;
+// rows come out ascending.  Bound by latency: one read of the totals, five
+// cluster barriers and four rounds of remote reads.
 //
 // move: row dst + i of K and V (and the totals) becomes row rows[i], for a
 // strictly ascending list with rows[i] >= dst + i.  In place: a cluster owns a
@@ -385,25 +386,6 @@ __global__ void __launch_bounds__(kMoveThreads, 2)
     cluster.sync();  // peers may still write here
 }
 
-void launch_cluster(const void* fn, dim3 grid, uint32_t threads, size_t smem, uint32_t C, cudaStream_t stream,
-                    void** args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = C;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
-}
-
 // Clusters of C CTAs that run at once on the current device (asked once for
 // each kernel, size and device).
 uint32_t clusters_at_once(const void* fn, uint32_t C, uint32_t threads, size_t smem) {
@@ -415,7 +397,7 @@ uint32_t clusters_at_once(const void* fn, uint32_t C, uint32_t threads, size_t s
     const auto key = std::make_tuple(dev, fn, C, smem);
     const auto it = known.find(key);
     if (it != known.end()) return it->second;
-    if (C > 8) SM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (C > 8) allow_large_clusters_once(fn);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(C);
     cfg.blockDim = dim3(threads);
@@ -448,6 +430,9 @@ void launch_cache_select(const float* weights, uint32_t n_kv, uint32_t max_ctx, 
     // 8.4 us), then clusters of 4 to 16 with as many a thread (8 x 8192: 8.5 us by
     // four CTAs, 9.8 by two, 10.1 by one; 8 x 32768: 11.0 us by 8, 14.0 by 16);
     // two CTAs per SM in all, and no cluster left waiting for another to end
+    // (64 x 8192: 11.5 us by four CTAs, 23.9 by eight in two rounds; where a
+    // CTA's keys then do not fit shared memory two rounds would be better:
+    // 64 x 131072 80 us by four CTAs, 62 us by eight)
     const uint32_t m = n - n_first - n_last, sms = (uint32_t)device_sm_count();
     const void* fn = (const void*)smallm_cache_select_kernel;
     set_smem_limit_once(fn, (int)(4 * kSelCached));
@@ -456,7 +441,7 @@ void launch_cache_select(const float* weights, uint32_t n_kv, uint32_t max_ctx, 
     while (C > 1 && clusters_at_once(fn, C, kSelThreads, 4 * kSelCached) < n_kv) C /= 2;
     uint32_t per_cta = (m + C - 1) / C, cached = per_cta <= kSelCached;
     void* args[] = {&weights, &max_ctx, &n, &n_keep, &n_first, &n_last, &per_cta, &cached, &rows};
-    launch_cluster(fn, dim3(n_kv * C), kSelThreads, cached ? 4ull * per_cta : 0, C, stream, args);
+    launch_cluster_ex(fn, dim3(n_kv * C), dim3(kSelThreads), cached ? 4ull * per_cta : 0, C, stream, args);
 }
 
 void launch_cache_move(float* kcache, float* vcache, float* weights, uint32_t n_kv, uint32_t hd, uint32_t max_ctx,
@@ -491,7 +476,7 @@ void launch_cache_move(float* kcache, float* vcache, float* weights, uint32_t n_
     while (C > 1 && clusters_at_once(fn, C, kMoveThreads, 0) < 2 * n_kv * slices) C /= 2;
     uint32_t slice = hd / 4 / slices;
     void* args[] = {&kcache, &vcache, &weights, &hd, &slice, &a, &stride};
-    launch_cluster(fn, dim3(slices * C, n_kv, 2), kMoveThreads, 0, C, stream, args);
+    launch_cluster_ex(fn, dim3(slices * C, n_kv, 2), dim3(kMoveThreads), 0, C, stream, args);
 }
 
 }  // namespace smallm

@@ -204,6 +204,10 @@ void launch_attention_static(const float* q, const float* kcache, const float* v
 // cudaLaunchKernelExC with optional programmatic dependent launch.
 void launch_kernel_ex(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl,
                       void** args);
+// The same, as a programmatic dependent, with clusters of C CTAs along x; more
+// than 8 once they have been allowed for the kernel on the current device.
+void launch_cluster_ex(const void* fn, dim3 grid, dim3 block, size_t smem, uint32_t C, cudaStream_t stream, void** args);
+void allow_large_clusters_once(const void* fn);
 // Device address of the current device's kernel error word (see
 // gemv_error_flags).
 unsigned int* device_error_flag();

@@ -607,6 +607,36 @@ unsigned int* device_error_flag() {
     return it->second;
 }
 
+void allow_large_clusters_once(const void* fn) {
+    static std::mutex mu;
+    static std::set<std::pair<int, const void*>> done;  // (device, kernel)
+    int dev = 0;
+    SM_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> g(mu);
+    if (done.count({dev, fn})) return;
+    SM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    done.insert({dev, fn});
+}
+
+void launch_cluster_ex(const void* fn, dim3 grid, dim3 block, size_t smem, uint32_t C, cudaStream_t stream,
+                       void** args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
+}
+
 void set_smem_limit_once(const void* fn, int bytes) {
     static std::mutex mu;
     static std::set<std::tuple<int, const void*, int>> done;  // (device, kernel, bytes)

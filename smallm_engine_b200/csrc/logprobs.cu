@@ -391,27 +391,13 @@ void launch_logprobs(const LogprobArgs& a, cudaStream_t stream) {
     uint32_t C = 1;
     while (C < kLpMaxCluster && a.n_rows * C < 2 * sms && nq > std::max(C, 2u) * kLpChunk) C *= 2;
     const void* fn = (const void*)smallm_logprobs_kernel;
-    if (C > 8) SM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (C > 8) allow_large_clusters_once(fn);
     set_smem_limit_once(fn, (int)sizeof(LpShared));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.n_rows * C);
-    cfg.blockDim = dim3(kLpThreads);
-    cfg.dynamicSmemBytes = sizeof(LpShared);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = C;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
     LogprobArgs aa = a;
     uint32_t per_cta = (nq + C - 1) / C;
     unsigned int* err = a.err ? a.err : device_error_flag();
     void* args[] = {&aa, &per_cta, &err};
-    SM_CUDA(cudaLaunchKernelExC(&cfg, fn, args));
+    launch_cluster_ex(fn, dim3(a.n_rows * C), dim3(kLpThreads), sizeof(LpShared), C, stream, args);
 }
 
 }  // namespace smallm

@@ -36,7 +36,7 @@ namespace {
 
 struct TreeParams {
     TreeArgs a;
-    uint32_t G, R, n, words;
+    uint32_t G, R, n;
     uint32_t n_split, tiles_per_split;
     uint32_t sc_rows;    // stored scores of a key: R, padded; 0: they run along keys
     uint32_t sc_keys;    // ... and of a row: n, padded to tiles
@@ -1163,7 +1163,6 @@ void launch_attention_tree(const TreeArgs& a, void* work, size_t work_bytes, cud
     p.G = a.n_heads / a.n_kv;
     p.R = a.n_tokens * p.G;
     p.n = a.n_past + a.n_tokens;
-    p.words = (a.n_tokens + 31) / 32;
     p.n_split = t.n_split;
     p.tiles_per_split = t.tiles_per_split;
     p.sc_rows = t.sc_rows;
