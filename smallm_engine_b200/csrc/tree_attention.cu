@@ -70,8 +70,9 @@ struct TreeParams {
 // not: a K row's multiplies its scores, a V row's goes into P, which is then
 // relative to the token's largest product p |v| of the tile instead of its
 // largest p.  P therefore waits for V's scales (2% of 64 tokens over 32747 rows,
-// 6% of one token with totals over 16384; looked at before the exponentials: by
-// a wait after them, P in registers meanwhile, it was 13% and 14%).
+// 5% of one token with totals over 16384; looked at before the exponentials: by
+// a wait after them, P in registers meanwhile, it was 13% and 14%).  With such
+// rows in every tile 64 tokens take 2.2 times as long.
 //   - warps 25 (K) and 26 (V) copy tiles of f32 rows with bulk copies into
 //     three slots each (six for rows of 64 or fewer).  (Loads through registers
 //     took the load/store unit twice as long as these copies and the reads of
@@ -196,6 +197,11 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     return r;
 }
 
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
 // 1 / sum of a row with maximum m; 0 where it sees nothing, NaN where its scores
 // leave no sum.
 __device__ __forceinline__ float row_inverse(float m, float sum) {
@@ -211,15 +217,6 @@ template <bool PLAIN>
 __device__ __forceinline__ float add_weight(float acc, float s, float c, float2 stats) {
     const float y = PLAIN ? fmaf(s, c, -stats.x) : __fadd_rn(__fmul_rn(s, c), -stats.x);
     return !PLAIN && s == -INFINITY ? acc : fmaf(exp2f(y), stats.y, acc);
-}
-__device__ __forceinline__ float min3(float a, float b, float c) {
-    float r;
-    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
-__device__ __forceinline__ float f4_at(const float4& v, int i) {
-    return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
 }
 // x = f(column, x) over N * 8 f32 columns of this thread's lane of tensor
 // memory, in a loop: for paths that are rarely taken and shall not hold
@@ -305,31 +302,30 @@ __device__ __forceinline__ bool tc_convert(const TreeParams& p, uint32_t t0, uin
         const uint32_t left = p.n - (t0 + t) * kTcKeys;  // rows from the tile's first to the last
         const bool stuck = !mbar_wait_soon(&sh.raw_full[GROUP][slot], (t / C::slots) & 1);
         const float4* src = reinterpret_cast<const float4*>(slots + slot * C::slot) + tid;
-        // the largest magnitude, and the smallest of three elements' largest ones: no
-        // row of the tile is smaller
-        float m = 0.f, low = INFINITY;
+        // the largest magnitude, and the smallest (as bits less 1, so that zeros do not
+        // count) of four elements' largest ones: no row of the tile is smaller.  (Of
+        // three, ordinary rows beside a channel 1000 times larger are looked at more
+        // closely again and again: 10% longer.)
+        float m = 0.f;
+        uint32_t low = ~0u;
+        auto unit_max = [](const float4& v) { return max_abs_nan(max3_abs_nan(v.x, v.y, v.z), v.w); };
+        auto below = [](uint32_t least, float v) { return __viaddmin_u32(__float_as_uint(v), ~0u, least); };
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = src[i * kConvThreads];
         if (left < kTcKeys) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
+            for (int i = 0; i < N; ++i)
                 if (row0 + i * STEP >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                const float u = max3_abs_nan(x[i].x, x[i].y, x[i].z);
-                m = max3_abs_nan(m, u, x[i].w);
-                if (row0 + i * STEP < left) low = fminf(low, u);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i += 2) {
-                const float u = max3_abs_nan(x[i].x, x[i].y, x[i].z);
-                const float v = max3_abs_nan(x[i + 1].x, x[i + 1].y, x[i + 1].z);
-                m = max3_abs_nan(max3_abs_nan(m, u, x[i].w), v, x[i + 1].w);
-                low = min3(low, u, v);
-            }
         }
-        auto put_range = [&](float most, float least) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float u = unit_max(x[i]), v = unit_max(x[i + 1]);
+            m = max3_abs_nan(m, u, v);
+            low = below(below(low, u), v);
+        }
+        auto put_range = [&](float most, uint32_t least) {
             const uint32_t a = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-            const uint32_t b = __reduce_min_sync(0xffffffffu, __float_as_uint(least));
+            const uint32_t b = __reduce_min_sync(0xffffffffu, least);
             if (lane == 0) wrange[t & 1][cw] = make_uint2(a, b);
         };
         uint32_t mx;
@@ -347,13 +343,17 @@ __device__ __forceinline__ bool tc_convert(const TreeParams& p, uint32_t t0, uin
             float4* own = reinterpret_cast<float4*>(slots + slot * C::slot) + tid;
             auto row_max = [&](const float4& v) {
                 float r = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+                if constexpr (W == 32) {
+                    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(r)));
+                } else {
 #pragma unroll
-                for (int o = W / 2; o > 0; o >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, o));
-                return r;
+                    for (int o = W / 2; o > 0; o >>= 1) r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, o));
+                    return r;
+                }
             };
             // whole rows' magnitudes, infinities and NaN cleaned; rows of zeros do not count
-            m = 0.f, low = INFINITY;
-#pragma unroll 1
+            m = 0.f, low = ~0u;
+#pragma unroll 4
             for (uint32_t i = 0, row = row0; i < (uint32_t)N; ++i, row += STEP) {
                 float4 v = own[i * kConvThreads];
                 if (row >= left) v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -366,14 +366,14 @@ __device__ __forceinline__ bool tc_convert(const TreeParams& p, uint32_t t0, uin
                 own[i * kConvThreads] = v;
                 const float r = row_max(v);
                 m = fmaxf(m, r);
-                if (r > 0.f) low = fminf(low, r);
+                low = below(low, r);
             }
             conv_any(1 + GROUP, false);  // the ranges have been read by all
             put_range(m, low);
             conv_any(1 + GROUP, false);
             wide = get_range();
             if (wide) {
-#pragma unroll 1
+#pragma unroll 4
                 for (uint32_t i = 0, row = row0; i < (uint32_t)N; ++i, row += STEP) {
                     float4 v = own[i * kConvThreads];
                     float mult, inv;
@@ -575,11 +575,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
                 tmem_wait_st();
             };
             get_scores();
-            // (never 0: an unseen key's -inf times it stays -inf)
             // keys with scales of their own, or a factor beyond f32's range (which no score need be)
             const float factor = qtop * k_scale, v_exp = sh.v_exp[ring];
             const bool wide_v = v_exp == INFINITY;
             const bool far = !(factor < INFINITY);
+            // (never 0: an unseen key's -inf times it stays -inf)
             const float raw = far ? 1.f : fmaxf(qinv * k_scale, 0x1p-120f);
             if (key0 + kTcKeys > a.n_past || bad || far) {
                 if (far) {
@@ -632,8 +632,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) smallm_tree_kernel(const TreePa
             const float tref = mt == INFINITY ? __uint_as_float(0x7FC00000u) : (mt == -INFINITY ? 0.f : mt);
             float off = kPShift - tref;
             float o_exp = v_exp, wsum = 0.f;  // O's exponent besides mt's; sum of the weights where P holds more
-            if (wide_v || !(factor < 0x1p-13f)) {  // (below it hd products below 2^30 give no large score)
-                const bool large = fabsf(tref) >= kLargeScore;
+            // (from a factor of 2^-13 on hd products below 2^30 can give a large score)
+            const bool large = fabsf(tref) >= kLargeScore;
+            if (wide_v || (!(factor < 0x1p-13f) && __any_sync(0xffffffffu, valid && large))) {
                 // exponents of their own first, by way of tensor memory.  A product of a large
                 // score is rounded before the maximum's is taken from it: by an fma the
                 // maximum itself could end up anywhere between 2^-128 and 2^128.
