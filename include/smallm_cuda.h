@@ -236,14 +236,14 @@ int smallm_attention_noalloc(smallm_ctx* ctx, const float* q_dev, const float* k
  * u % 32 of mask_dev[t * words + u / 32] is set (words = ceil(n_tokens / 32);
  * a token sees itself only if its own bit is set; bits at n_tokens and above
  * are ignored).  mask_dev NULL is a chain: u <= t.  A token that sees nothing
- * gets zeros.  Rows that a token does not see do not affect it, whatever they
- * hold, NaN and infinities included; where a seen row or q holds them, or a
+ * gets zeros.  Rows that a token does not see do not affect it (beyond the
+ * accuracy below), whatever they hold, NaN and infinities included; where a seen row or q holds them, or a
  * score lies above f32's range or all of a token's scores below it, the output
  * is not finite.
  *
  * Accuracy: an element of q, K or V enters to 2^-22 of itself or 2^-25 of the
  * largest magnitude of its row of head_dim, a weight's product with its row of
- * V to 2^-22 of itself or 2^-39 of the token's largest such product among 64
+ * V to 2^-22 of itself or 2^-24 of the token's largest such product among 64
  * neighbouring rows; products and sums are f32's.  A weight below 2^-126 of
  * the token's largest may count as 0.
  *

@@ -86,13 +86,13 @@ struct TreeParams {
 //     O = P V (P in tensor memory, over S's columns; V MN-major);
 //   - warps 0..7, lane = row, two warps for a row: each takes half of the keys
 //     for the running maximum (a whole number in base 2, so rescaling is
-//     exact; the halves meet in shared memory), P = 2^(s - m + 14) as hi and lo
-//     and the sum;
+//     exact; the halves meet in shared memory), P = 2^(s - mt + 14) as hi and lo,
+//     mt the tile's own maximum, and the sum;
 //   - warps 8..15, lane = row, take half of the columns of a tile's O each and
 //     add it to f32 registers with that tile's exponent and the row's
 //     rescaling: the long sum is made of rounded f32 adds.  (By the same warps
 //     as the softmax one token over 16384 rows took 2% longer, with totals 6%.)
-// One token of 32 heads at 128 reads K and V at 6.3 TB/s from 16384 rows on
+// One token of 32 heads at 128 reads K and V at 5.9 TB/s from 16384 rows on
 // (the slope of its time; copies reach 6.5), after 8 us for two launches, the
 // first tile and the join.  Blocks with all 128 rows take about 2800 cycles a
 // tile where the products take 1536: conversion works for 2600 of them, softmax
@@ -954,8 +954,8 @@ __global__ void __launch_bounds__(kMergeThreads) smallm_tree_merge_kernel(const 
 // total does not depend on the launch.  Scores of up to kFewRows rows run along
 // the keys: a lane has a key and walks the rows; the CTAs behind the n_join
 // that join the splits find mc and sum of the rows from the splits themselves,
-// so that neither waits for the other (a kernel after the joining one: 38 us
-// instead of 35 us for one token over 16384 rows).  More rows run along
+// so that neither waits for the other (a kernel after the joining one: 8% longer
+// for one token over 16384 rows).  More rows run along
 // themselves, four keys of a row together: the lanes of a warp have the rows of 8
 // keys, and their sums meet by shuffles.  31 tokens over 12300 rows, 12 heads of
 // 128: 27.3 us, 19.7 us of them without the totals; 29.2 us with 16 keys a warp,

@@ -6,7 +6,7 @@ range, and totals of rows that a token whose result is not finite does not see.
 Against the definition in 64 bits with the tolerance derived in
 test_attention_tree_gpu.py, unless a test says otherwise.  That tolerance also
 covers how rows enter: an element is off by at most 2^-22 of itself or 2^-25 of
-its row's largest magnitude, and a weight's product with its row by 2^-39 of
+its row's largest magnitude, and a weight's product with its row by 2^-24 of
 the token's largest such product among 64 keys."""
 import numpy as np
 import pytest
