@@ -312,6 +312,7 @@ class Generator:
     def generate(self, prompt: list[int], max_new_tokens: int) -> list[int]:
         import time
         self.stats = GenerationStats()
+        self.logprobs = []
         tokens = [int(t) for t in prompt]
         if not tokens:
             return []
@@ -339,7 +340,6 @@ class Generator:
                 self.stats.prefill_tokens += 1
         self.stats.prefill_ms = (time.perf_counter() - t0) * 1e3
         out: list[int] = []
-        self.logprobs = []
         generated = list(tokens)
         t0 = time.perf_counter()
         for _ in range(max_new_tokens):
