@@ -324,6 +324,7 @@ class Generator:
             shared = len(tokens) - 1
         self.stats.reused_tokens = shared
         self.model.truncate_cache(shared)
+        self.cached_tokens = tokens[:shared]  # all that is known to be there if this call fails
         pos = shared
         # samplers that run on the device read the model's logits in place
         on_device = hasattr(self.sampler, "sample_model")
